@@ -296,6 +296,50 @@ SSM_API int ssm_conv1d_bwd(const ssm_conv1d_args* args, void* workspace, size_t 
  * out (batch, dim) = act(bias + sum_k weight[k] window[k]). */
 SSM_API int ssm_conv1d_update(const ssm_conv1d_args* args, void* stream);
 
+/* ---- linear attention with a decay for each head --------------------------------------------
+ * The layer that hybrid stacks put between Mamba layers; no counterpart in the reference.  Per
+ * (batch row, head h) a state S of (dk, dv) float32, w = exp(log_decay[h]):
+ *   S_t = w S_{t-1} + k_t v_t^T,   out_t = scale * q_t^T S_t,   S_{-1} = initial_state or 0
+ * q, k, v, out and their gradients are (batch, seqlen, heads, channels) with any batch, token
+ * and head strides and unit channel stride; q, k and v may have fewer heads (each count divides
+ * `heads`; head h reads head h / (heads / count)).  dk and dv are 1 to 128.  States are
+ * (batch, heads, dk, dv) float32 contiguous.  `length` (batch) int64, clamped to [0, seqlen]:
+ * tokens from length[b] on take no part, out and the gradients are zero there, and last_state
+ * is the state after length[b] tokens.  log_decay = -inf is a decay of zero. */
+typedef struct ssm_linear_attn_args {
+    int64_t batch, seqlen, heads, dk, dv;
+    int64_t q_heads, k_heads, v_heads;
+    int32_t dtype;                 /* SSM_F32 or SSM_BF16, for q, k, v, out and their gradients */
+    float scale;
+    const void* q;       int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void* k;       int64_t k_batch_stride, k_token_stride, k_head_stride;
+    const void* v;       int64_t v_batch_stride, v_token_stride, v_head_stride;
+    const float* log_decay;        /* (heads) */
+    const float* initial_state;    /* may be NULL (zero) */
+    const int64_t* length;         /* may be NULL */
+    void* out;           int64_t out_batch_stride, out_token_stride, out_head_stride; /* forward */
+    float* last_state;             /* forward; may be NULL */
+    /* backward */
+    const void* dout;    int64_t dout_batch_stride, dout_token_stride, dout_head_stride;
+    const float* dlast_state;      /* may be NULL (zero) */
+    void* dq;            int64_t dq_batch_stride, dq_token_stride, dq_head_stride;   /* (.., q_heads, dk) */
+    void* dk_;           int64_t dk_batch_stride, dk_token_stride, dk_head_stride;   /* (.., k_heads, dk) */
+    void* dv_;           int64_t dv_batch_stride, dv_token_stride, dv_head_stride;   /* (.., v_heads, dv) */
+    float* dinitial_state;         /* may be NULL */
+} ssm_linear_attn_args;
+
+/* Bytes of device workspace of the forward (backward = 0) or the backward (backward = 1): the
+ * states of the segments that a long row is cut into, and per-head gradients of shared heads.
+ * May be 0 (also on an error: ssm_last_error() is then non-empty and the call itself fails). */
+SSM_API size_t ssm_linear_attn_workspace_size(const ssm_linear_attn_args* args, int backward);
+/* Forward in chunks.  The workspace is 256-byte aligned. */
+SSM_API int ssm_linear_attn_fwd(const ssm_linear_attn_args* args, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* Backward: dq, dk_, dv_ and (optional) dinitial_state from q, k, v, dout, dlast_state.
+ * Overwrites them; deterministic (gradients of shared heads are summed in head order). */
+SSM_API int ssm_linear_attn_bwd(const ssm_linear_attn_args* args, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 /* Reads and clears the device-side error words of the current device -- the library's own
  * and the one in ssm_scan_bwd_noalloc's static scratch -- (synchronizes `stream`; allocates
  * nothing).  Returns SSM_OK with *code = 0, or SSM_ERR_DEVICE with *code set to the

@@ -15,6 +15,7 @@
 #include <string>
 
 #include "../../include/ssm_b200.h"
+#include "linattn.h"
 #include "params.h"
 #include "scan_layout.h"
 #include <nvtx3/nvToolsExt.h>
@@ -47,6 +48,8 @@ cudaError_t launch_conv1d(const ConvParams& p, int is_bf16, int width, int kind,
 cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width, float* dw, int64_t dw_sd,
                                  float* dbias, int sms, cudaStream_t stream);
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
+cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
+cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream);
 size_t bwd_smem_bytes(int is_bf16, int lpc, int spt, int dt, int dstate, int has_z);
 cudaError_t launch_scan_bwd_pair(const BwdParams& p, int is_bf16, int cpl, const CUtensorMap* maps,
                                  cudaStream_t stream);
@@ -945,6 +948,181 @@ int ssm_conv1d_update(const ssm_conv1d_args* a, void* stream) {
                                          static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "conv1d_update launch");
     return SSM_OK;
+}
+
+// ---- linear attention --------------------------------------------------------------------------
+static int la_common(const char* name, const ssm_linear_attn_args* a) {
+    if (!a) return fail(SSM_ERR_INVALID, "%s: args is NULL", name);
+    if (a->batch < 1 || a->seqlen < 1 || a->heads < 1)
+        return fail(SSM_ERR_INVALID, "%s: sizes must be positive", name);
+    if (a->seqlen > (1 << 30) || a->batch > (1 << 30) || a->heads > (1 << 30) ||
+        a->batch * a->heads > (1 << 24))
+        return fail(SSM_ERR_INVALID, "%s: seqlen must be <= 2^30 and batch * heads <= 2^24", name);
+    if (a->dk < 1 || a->dk > 128 || a->dv < 1 || a->dv > 128)
+        return fail(SSM_ERR_INVALID, "%s: dk and dv must be 1 to 128", name);
+    for (int64_t n : {a->q_heads, a->k_heads, a->v_heads})
+        if (n < 1 || a->heads % n != 0)
+            return fail(SSM_ERR_INVALID, "%s: q_heads, k_heads and v_heads must divide heads", name);
+    if (!valid_dtype(a->dtype)) return fail(SSM_ERR_INVALID, "%s: dtype must be SSM_F32 or SSM_BF16", name);
+    if (!a->q || !a->k || !a->v || !a->log_decay)
+        return fail(SSM_ERR_INVALID, "%s: q, k, v and log_decay are required", name);
+    return SSM_OK;
+}
+
+// Tokens per segment: a multiple of the longest chunk.  Cutting a row in n segments costs
+// another reading of b and c, so it is done only where the (batch, head) pairs alone give the
+// SMs less than two CTAs each.
+static int la_plan_segments(const ssm_linear_attn_args* a, int sms, int* seglen) {
+    const int64_t rows = a->batch * a->heads;
+    int64_t want = (2 * (int64_t)sms + rows - 1) / rows;
+    const int64_t most = a->seqlen / 512;      // at least 512 tokens each
+    if (want > most) want = most;
+    if (want > 16) want = 16;                  // every CTA folds the states of those before it
+    if (want < 1) want = 1;
+    int64_t len = (a->seqlen + want - 1) / want;
+    len = (len + 127) / 128 * 128;
+    *seglen = (int)len;
+    return (int)((a->seqlen + len - 1) / len);
+}
+
+namespace {
+// Workspace: per role the segment states, then the per-head gradients of shared heads.
+struct LaPlan {
+    int nseg, seglen;
+    size_t seg[3], part[3], bytes;             // byte offsets
+};
+}  // namespace
+
+static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
+    LaPlan pl;
+    memset(&pl, 0, sizeof(pl));
+    pl.nseg = la_plan_segments(a, sms, &pl.seglen);
+    const int nroles = backward ? 3 : 1;
+    auto take = [&](size_t n) {
+        const size_t at = pl.bytes;
+        pl.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    if (pl.nseg > 1)
+        for (int i = 0; i < nroles; i++)
+            pl.seg[i] = take((size_t)a->batch * a->heads * pl.nseg * a->dk * a->dv * sizeof(float));
+    if (backward) {
+        const int64_t heads[3] = {a->q_heads, a->v_heads, a->k_heads}, d[3] = {a->dk, a->dv, a->dk};
+        for (int i = 0; i < 3; i++)
+            if (heads[i] != a->heads)
+                pl.part[i] = take((size_t)a->batch * a->seqlen * a->heads * d[i] * sizeof(float));
+    }
+    return pl;
+}
+
+static LaTensor la_tensor(const ssm_linear_attn_args* a, const void* p, int64_t sb, int64_t st, int64_t sh,
+                          int64_t heads) {
+    const int64_t es = a->dtype == SSM_BF16 ? 2 : 4;
+    LaTensor t;
+    t.p = p; t.sb = sb; t.st = st; t.sh = sh; t.share = (int)(a->heads / heads);
+    t.vec = aligned16(p) && (a->batch == 1 || ((sb * es) & 15) == 0) && (a->seqlen == 1 || ((st * es) & 15) == 0) &&
+            (heads == 1 || ((sh * es) & 15) == 0);
+    return t;
+}
+
+size_t ssm_linear_attn_workspace_size(const ssm_linear_attn_args* a, int backward) {
+    g_err.clear();
+    if (la_common("ssm_linear_attn_workspace_size", a)) return 0;
+    DevInfo* di = nullptr;
+    if (device_info(&di)) return 0;
+    return la_plan(a, backward, di->sms).bytes;
+}
+
+static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward, void* workspace, size_t ws_bytes,
+                   void* stream_) {
+    int rc = la_common(name, a);
+    if (rc) return rc;
+    if (!backward && !a->out) return fail(SSM_ERR_INVALID, "%s: out is required", name);
+    if (backward && (!a->dout || !a->dq || !a->dk_ || !a->dv_))
+        return fail(SSM_ERR_INVALID, "%s: dout, dq, dk_ and dv_ are required", name);
+    DevInfo* di = nullptr;
+    if ((rc = device_info(&di))) return rc;
+    const LaPlan pl = la_plan(a, backward, di->sms);
+    if (pl.bytes && (!workspace || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+        return fail(SSM_ERR_WORKSPACE, "%s: workspace needs %zu bytes, 256-byte aligned", name, pl.bytes);
+    char* ws = static_cast<char*>(workspace);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+
+    LaParams p;
+    memset(&p, 0, sizeof(p));
+    p.batch = (int)a->batch; p.seqlen = (int)a->seqlen; p.heads = (int)a->heads;
+    p.nseg = pl.nseg; p.seglen = pl.seglen;
+    p.log_decay = a->log_decay; p.length = a->length; p.err = di->err;
+    const LaTensor q = la_tensor(a, a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads);
+    const LaTensor k = la_tensor(a, a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads);
+    const LaTensor v = la_tensor(a, a->v, a->v_batch_stride, a->v_token_stride, a->v_head_stride, a->v_heads);
+    const int dk = (int)a->dk, dv = (int)a->dv, H = (int)a->heads;
+    auto role = [&](int i, const LaTensor& ra, const LaTensor& rb, const LaTensor& rc_, int db, int dc, int reverse,
+                    bool transposed) {
+        LaRole& r = p.role[i];
+        r.a = ra; r.b = rb; r.c = rc_; r.db = db; r.dc = dc; r.reverse = reverse;
+        r.alpha = a->scale; r.beta = reverse ? 1.f : a->scale; r.sigma = reverse ? a->scale : 1.f;
+        r.s_i = transposed ? 1 : dv;           // the state tensors are (dk, dv)
+        r.s_j = transposed ? dv : 1;
+        r.seg = pl.nseg > 1 ? reinterpret_cast<float*>(ws + pl.seg[i]) : nullptr;
+    };
+    // a gradient goes straight to its tensor, or as float32 per-head partials to the workspace
+    auto dest = [&](int i, void* out, int64_t sb, int64_t st, int64_t sh, int64_t heads, int d) {
+        LaRole& r = p.role[i];
+        if (heads == H) {
+            const LaTensor t = la_tensor(a, out, sb, st, sh, heads);
+            r.out = out; r.o_sb = sb; r.o_st = st; r.o_sh = sh; r.out_vec = t.vec;
+        } else {
+            r.out = ws + pl.part[i]; r.out_f32 = 1; r.out_vec = d % 4 == 0;
+            r.o_sh = d; r.o_st = (int64_t)H * d; r.o_sb = a->seqlen * r.o_st;
+        }
+    };
+    if (!backward) {
+        p.nroles = 1;
+        role(0, q, k, v, dk, dv, 0, false);
+        dest(0, a->out, a->out_batch_stride, a->out_token_stride, a->out_head_stride, H, dv);
+        p.role[0].state0 = a->initial_state;
+        p.role[0].state_out = a->last_state;
+    } else {
+        const LaTensor dout = la_tensor(a, a->dout, a->dout_batch_stride, a->dout_token_stride, a->dout_head_stride, H);
+        p.nroles = 3;
+        role(0, dout, v, k, dv, dk, 0, true);
+        dest(0, a->dq, a->dq_batch_stride, a->dq_token_stride, a->dq_head_stride, a->q_heads, dk);
+        p.role[0].state0 = a->initial_state;
+        role(1, k, q, dout, dk, dv, 1, false);
+        dest(1, a->dv_, a->dv_batch_stride, a->dv_token_stride, a->dv_head_stride, a->v_heads, dv);
+        p.role[1].state0 = a->dlast_state;
+        p.role[1].state_out = a->dinitial_state;
+        role(2, v, dout, q, dv, dk, 1, true);
+        dest(2, a->dk_, a->dk_batch_stride, a->dk_token_stride, a->dk_head_stride, a->k_heads, dk);
+        p.role[2].state0 = a->dlast_state;
+    }
+    const int is_bf16 = a->dtype == SSM_BF16;
+    cudaError_t e = launch_linattn_simt(p, is_bf16, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
+    for (int i = 0; backward && i < 3; i++) {
+        if (!p.role[i].out_f32) continue;
+        LaGroupParams g;
+        memset(&g, 0, sizeof(g));
+        g.src = static_cast<const float*>(p.role[i].out);
+        g.batch = p.batch; g.seqlen = p.seqlen; g.heads = H; g.d = p.role[i].dc;
+        if (i == 0) { g.out = a->dq; g.o_sb = a->dq_batch_stride; g.o_st = a->dq_token_stride; g.o_sh = a->dq_head_stride; g.share = q.share; }
+        if (i == 1) { g.out = a->dv_; g.o_sb = a->dv_batch_stride; g.o_st = a->dv_token_stride; g.o_sh = a->dv_head_stride; g.share = v.share; }
+        if (i == 2) { g.out = a->dk_; g.o_sb = a->dk_batch_stride; g.o_st = a->dk_token_stride; g.o_sh = a->dk_head_stride; g.share = k.share; }
+        e = launch_linattn_group(g, is_bf16, di->sms, stream);
+        if (e != cudaSuccess) return cuda_fail(e, "linear attention head-sum launch");
+    }
+    return SSM_OK;
+}
+
+int ssm_linear_attn_fwd(const ssm_linear_attn_args* a, void* workspace, size_t ws_bytes, void* stream) {
+    NvtxRange r_("ssm_linear_attn_fwd");
+    return la_impl("ssm_linear_attn_fwd", a, 0, workspace, ws_bytes, stream);
+}
+
+int ssm_linear_attn_bwd(const ssm_linear_attn_args* a, void* workspace, size_t ws_bytes, void* stream) {
+    NvtxRange r_("ssm_linear_attn_bwd");
+    return la_impl("ssm_linear_attn_bwd", a, 1, workspace, ws_bytes, stream);
 }
 
 int ssm_exp2_compare(const float* x, float* y_fma, float* y_mufu, int64_t n, void* stream) {

@@ -509,6 +509,125 @@ at::Tensor conv1d_update(const at::Tensor& x, const at::Tensor& state, const at:
     return out;
 }
 
+// ---- linear attention with a decay for each head -----------------------------------------------
+// (batch, seqlen, n, d) with unit channel stride, n dividing heads
+void check_blhd(const at::Tensor& t, const char* name, int64_t B, int64_t L, int64_t H, int64_t d, at::ScalarType st) {
+    check_cuda(t, name);
+    TORCH_CHECK(t.dim() == 4, name, " must be a 4D tensor");
+    TORCH_CHECK(t.scalar_type() == st, name, " must have dtype ", st);
+    TORCH_CHECK(t.size(0) == B && t.size(1) == L && t.size(2) > 0 && H % t.size(2) == 0 && t.size(3) == d, name,
+                " must have shape (", B, ", ", L, ", n, ", d, ") with n dividing ", H);
+    TORCH_CHECK(t.stride(3) == 1 || d == 1, name, " must have unit channel stride");
+}
+
+void check_state(const std::optional<at::Tensor>& t, const char* name, int64_t B, int64_t H, int64_t K, int64_t V) {
+    if (!t) return;
+    check_f32(*t, name, {B, H, K, V});
+    TORCH_CHECK(t->is_contiguous(), name, " must be contiguous");
+}
+
+ssm_linear_attn_args la_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                             const at::Tensor& log_decay, double scale,
+                             const std::optional<at::Tensor>& initial_state,
+                             const std::optional<at::Tensor>& length) {
+    check_cuda(q, "q");
+    TORCH_CHECK(q.dim() == 4, "q must be a 4D tensor");
+    TORCH_CHECK(v.dim() == 4, "v must be a 4D tensor");
+    TORCH_CHECK(log_decay.is_cuda() && log_decay.dim() == 1 && log_decay.size(0) > 0 &&
+                    log_decay.scalar_type() == at::kFloat && log_decay.is_contiguous(),
+                "log_decay must be a contiguous float32 CUDA tensor of shape (heads,)");
+    const int64_t B = q.size(0), L = q.size(1), H = log_decay.size(0), K = q.size(3), V = v.size(3);
+    ssm_linear_attn_args a;
+    memset(&a, 0, sizeof(a));
+    a.dtype = dtype_code(q);
+    check_blhd(q, "q", B, L, H, K, q.scalar_type());
+    check_blhd(k, "k", B, L, H, K, q.scalar_type());
+    check_blhd(v, "v", B, L, H, V, q.scalar_type());
+    for (auto* t : {&k, &v, &log_decay})
+        TORCH_CHECK(t->device() == q.device(), "q, k, v and log_decay must be on one device");
+    check_state(initial_state, "initial_state", B, H, K, V);
+    if (length)
+        TORCH_CHECK(length->is_cuda() && length->scalar_type() == at::kLong && length->dim() == 1 &&
+                        length->size(0) == B && length->is_contiguous(),
+                    "lengths must be a contiguous CUDA long tensor of shape (batch,)");
+    a.batch = B; a.seqlen = L; a.heads = H; a.dk = K; a.dv = V; a.scale = (float)scale;
+    a.q_heads = q.size(2); a.k_heads = k.size(2); a.v_heads = v.size(2);
+    a.q = q.data_ptr(); a.q_batch_stride = q.stride(0); a.q_token_stride = q.stride(1); a.q_head_stride = q.stride(2);
+    a.k = k.data_ptr(); a.k_batch_stride = k.stride(0); a.k_token_stride = k.stride(1); a.k_head_stride = k.stride(2);
+    a.v = v.data_ptr(); a.v_batch_stride = v.stride(0); a.v_token_stride = v.stride(1); a.v_head_stride = v.stride(2);
+    a.log_decay = log_decay.data_ptr<float>();
+    a.initial_state = ptr<const float>(initial_state);
+    a.length = ptr<const int64_t>(length);
+    return a;
+}
+
+at::Tensor la_workspace(const ssm_linear_attn_args& a, int backward, const at::Tensor& like, size_t* bytes) {
+    *bytes = ssm_linear_attn_workspace_size(&a, backward);
+    TORCH_CHECK(*bytes > 0 || ssm_last_error()[0] == 0, ssm_last_error());
+    return *bytes ? at::empty({(int64_t)*bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// Returns [out (batch, seqlen, heads, dv), last_state (batch, heads, dk, dv) float32 or undefined].
+std::vector<at::Tensor> linear_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                        const at::Tensor& log_decay, double scale,
+                                        const std::optional<at::Tensor>& initial_state,
+                                        const std::optional<at::Tensor>& length, bool want_last) {
+    ssm_linear_attn_args a = la_args(q, k, v, log_decay, scale, initial_state, length);
+    c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = at::empty({a.batch, a.seqlen, a.heads, a.dv}, q.options());
+    at::Tensor last;
+    if (want_last) last = at::empty({a.batch, a.heads, a.dk, a.dv}, log_decay.options());
+    // nothing to launch: no rows, or no tokens (the state then stays what it was)
+    if (a.batch == 0 || a.seqlen == 0) {
+        if (want_last) {
+            if (initial_state) last.copy_(*initial_state);
+            else last.zero_();
+        }
+        return {out, last};
+    }
+    a.out = out.data_ptr(); a.out_batch_stride = out.stride(0); a.out_token_stride = out.stride(1); a.out_head_stride = out.stride(2);
+    a.last_state = want_last ? last.data_ptr<float>() : nullptr;
+    size_t bytes = 0;
+    at::Tensor ws = la_workspace(a, 0, q, &bytes);
+    ok(ssm_linear_attn_fwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, at::cuda::getCurrentCUDAStream().stream()));
+    return {out, last};
+}
+
+// Returns [dq, dk, dv, dinitial_state or undefined].
+std::vector<at::Tensor> linear_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                        const at::Tensor& log_decay, double scale,
+                                        const std::optional<at::Tensor>& initial_state,
+                                        const std::optional<at::Tensor>& length, const at::Tensor& dout,
+                                        const std::optional<at::Tensor>& dlast_state, bool want_dinitial) {
+    ssm_linear_attn_args a = la_args(q, k, v, log_decay, scale, initial_state, length);
+    c10::cuda::CUDAGuard guard(q.device());
+    check_blhd(dout, "dout", a.batch, a.seqlen, a.heads, a.dv, q.scalar_type());
+    TORCH_CHECK(dout.size(2) == a.heads, "dout must have ", a.heads, " heads");
+    check_state(dlast_state, "dlast_state", a.batch, a.heads, a.dk, a.dv);
+    at::Tensor dq = at::empty(q.sizes(), q.options());
+    at::Tensor dk = at::empty(k.sizes(), k.options());
+    at::Tensor dv = at::empty(v.sizes(), v.options());
+    at::Tensor di;
+    if (want_dinitial) di = at::empty({a.batch, a.heads, a.dk, a.dv}, log_decay.options());
+    if (a.batch == 0 || a.seqlen == 0) {
+        if (want_dinitial) {
+            if (dlast_state) di.copy_(*dlast_state);
+            else di.zero_();
+        }
+        return {dq, dk, dv, di};
+    }
+    a.dout = dout.data_ptr(); a.dout_batch_stride = dout.stride(0); a.dout_token_stride = dout.stride(1); a.dout_head_stride = dout.stride(2);
+    a.dlast_state = ptr<const float>(dlast_state);
+    a.dq = dq.data_ptr(); a.dq_batch_stride = dq.stride(0); a.dq_token_stride = dq.stride(1); a.dq_head_stride = dq.stride(2);
+    a.dk_ = dk.data_ptr(); a.dk_batch_stride = dk.stride(0); a.dk_token_stride = dk.stride(1); a.dk_head_stride = dk.stride(2);
+    a.dv_ = dv.data_ptr(); a.dv_batch_stride = dv.stride(0); a.dv_token_stride = dv.stride(1); a.dv_head_stride = dv.stride(2);
+    a.dinitial_state = want_dinitial ? di.data_ptr<float>() : nullptr;
+    size_t bytes = 0;
+    at::Tensor ws = la_workspace(a, 1, q, &bytes);
+    ok(ssm_linear_attn_bwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, at::cuda::getCurrentCUDAStream().stream()));
+    return {dq, dk, dv, di};
+}
+
 int64_t check_device_error() {
     int code = 0;
     ssm_check_device_error(&code, at::cuda::getCurrentCUDAStream().stream());
@@ -529,6 +648,8 @@ PYBIND11_MODULE(_C, m) {
     m.def("conv1d_fwd", &conv1d_fwd, "causal depthwise conv1d (+ SiLU) forward");
     m.def("conv1d_bwd", &conv1d_bwd, "causal depthwise conv1d (+ SiLU) backward");
     m.def("conv1d_update", &conv1d_update, "causal depthwise conv1d (+ SiLU) decode step");
+    m.def("linear_attn_fwd", &linear_attn_fwd, "linear attention with a decay for each head, forward");
+    m.def("linear_attn_bwd", &linear_attn_bwd, "linear attention with a decay for each head, backward");
     m.def("ckpt_from_reference", &ckpt_from_reference, "compact checkpoints from reference chunk states");
     m.def("state_update", &state_update, "one decode step");
     m.def("ckpt_len", [](int64_t n) { return ssm_scan_ckpt_len(n); });
