@@ -340,6 +340,52 @@ SSM_API int ssm_linear_attn_fwd(const ssm_linear_attn_args* args, void* workspac
 SSM_API int ssm_linear_attn_bwd(const ssm_linear_attn_args* args, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* One decode step: state (batch, heads, dk, dv) float32 with unit dv stride becomes
+ * w state + k v^T in place; out (batch, heads, dv) = scale * q^T state.  q, k (batch, heads, dk)
+ * and v (batch, heads, dv) as above without the token dimension.  Launched with programmatic
+ * dependent launch: it waits for the previous kernel in the stream before reading any input. */
+typedef struct ssm_linear_attn_update_args {
+    int64_t batch, heads, dk, dv;
+    int64_t q_heads, k_heads, v_heads;
+    int32_t dtype;                 /* for q, k, v, out */
+    float scale;
+    const void* q;       int64_t q_batch_stride, q_head_stride;
+    const void* k;       int64_t k_batch_stride, k_head_stride;
+    const void* v;       int64_t v_batch_stride, v_head_stride;
+    const float* log_decay;        /* (heads) */
+    float* state;        int64_t state_batch_stride, state_head_stride, state_k_stride;
+    void* out;           int64_t out_batch_stride, out_head_stride;
+} ssm_linear_attn_update_args;
+
+SSM_API int ssm_linear_attn_update(const ssm_linear_attn_update_args* args, void* stream);
+
+/* ---- layer norm over the last dimension -------------------------------------------------------
+ * The norm in front of each layer of a stack (the reference's blocks have an RMS norm in plain
+ * torch, modules/rms_norm.py:4-30).  Per row of dim elements (unit element stride, any row
+ * stride): y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps). */
+typedef struct ssm_layer_norm_args {
+    int64_t rows, dim;
+    int32_t dtype;                 /* SSM_F32 or SSM_BF16, for x, y, dy, dx */
+    float eps;
+    const void* x;       int64_t x_row_stride;
+    const float* weight;           /* (dim) or NULL (ones) */
+    const float* bias;             /* (dim) or NULL (zeros) */
+    void* y;             int64_t y_row_stride;     /* forward */
+    float* mean;                   /* (rows): forward outputs, NULL if no backward follows; */
+    float* rstd;                   /*         backward inputs */
+    const void* dy;      int64_t dy_row_stride;    /* backward */
+    void* dx;            int64_t dx_row_stride;    /* backward */
+    float* dweight;                /* backward, (dim) or NULL */
+    float* dbias;                  /* backward, (dim) or NULL */
+} ssm_layer_norm_args;
+
+SSM_API int ssm_layer_norm_fwd(const ssm_layer_norm_args* args, void* stream);
+/* Bytes of device workspace ssm_layer_norm_bwd needs (partial sums of dweight and dbias). */
+SSM_API size_t ssm_layer_norm_bwd_workspace_size(const ssm_layer_norm_args* args);
+/* Backward: dx, dweight, dbias from x, dy, mean and rstd.  Overwrites them; deterministic. */
+SSM_API int ssm_layer_norm_bwd(const ssm_layer_norm_args* args, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* Reads and clears the device-side error words of the current device -- the library's own
  * and the one in ssm_scan_bwd_noalloc's static scratch -- (synchronizes `stream`; allocates
  * nothing).  Returns SSM_OK with *code = 0, or SSM_ERR_DEVICE with *code set to the

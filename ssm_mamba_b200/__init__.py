@@ -15,7 +15,8 @@ The kernels sit behind the C ABI in include/ssm_b200.h (lib/libssm_b200.so).
 __version__ = "0.1.0"
 
 _OPS = ("SelectiveScanFn", "SelectiveUpdateFn", "causal_conv1d_fn", "causal_conv1d_update",
-        "linear_attention_fn", "selective_scan_fn", "selective_state_update")
+        "layer_norm_fn", "linear_attention_fn",
+        "linear_attention_update", "selective_scan_fn", "selective_state_update")
 __all__ = list(_OPS)
 
 

@@ -50,6 +50,9 @@ cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream);
+cudaError_t launch_linattn_update(const LaUpdParams& p, int is_bf16, int vec, cudaStream_t stream);
+cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream);
+int layer_norm_parts(int64_t rows, int dim, int sms);
 size_t bwd_smem_bytes(int is_bf16, int lpc, int spt, int dt, int dstate, int has_z);
 cudaError_t launch_scan_bwd_pair(const BwdParams& p, int is_bf16, int cpl, const CUtensorMap* maps,
                                  cudaStream_t stream);
@@ -1123,6 +1126,107 @@ int ssm_linear_attn_fwd(const ssm_linear_attn_args* a, void* workspace, size_t w
 int ssm_linear_attn_bwd(const ssm_linear_attn_args* a, void* workspace, size_t ws_bytes, void* stream) {
     NvtxRange r_("ssm_linear_attn_bwd");
     return la_impl("ssm_linear_attn_bwd", a, 1, workspace, ws_bytes, stream);
+}
+
+int ssm_linear_attn_update(const ssm_linear_attn_update_args* a, void* stream) {
+    NvtxRange r_("ssm_linear_attn_update");
+    const char* name = "ssm_linear_attn_update";
+    if (!a) return fail(SSM_ERR_INVALID, "%s: args is NULL", name);
+    if (a->batch < 1 || a->heads < 1 || a->batch > (1 << 30) || a->heads > (1 << 30) ||
+        a->batch * a->heads > (1 << 30))
+        return fail(SSM_ERR_INVALID, "%s: batch and heads must be positive, batch * heads <= 2^30", name);
+    if (a->dk < 1 || a->dk > 128 || a->dv < 1 || a->dv > 128)
+        return fail(SSM_ERR_INVALID, "%s: dk and dv must be 1 to 128", name);
+    for (int64_t n : {a->q_heads, a->k_heads, a->v_heads})
+        if (n < 1 || a->heads % n != 0)
+            return fail(SSM_ERR_INVALID, "%s: q_heads, k_heads and v_heads must divide heads", name);
+    if (!valid_dtype(a->dtype)) return fail(SSM_ERR_INVALID, "%s: dtype must be SSM_F32 or SSM_BF16", name);
+    if (!a->q || !a->k || !a->v || !a->log_decay || !a->state || !a->out)
+        return fail(SSM_ERR_INVALID, "%s: q, k, v, log_decay, state and out are required", name);
+    LaUpdParams p;
+    memset(&p, 0, sizeof(p));
+    p.batch = (int)a->batch; p.heads = (int)a->heads; p.dk = (int)a->dk; p.dv = (int)a->dv; p.scale = a->scale;
+    p.q = a->q; p.q_sb = a->q_batch_stride; p.q_sh = a->q_head_stride; p.q_share = (int)(a->heads / a->q_heads);
+    p.k = a->k; p.k_sb = a->k_batch_stride; p.k_sh = a->k_head_stride; p.k_share = (int)(a->heads / a->k_heads);
+    p.v = a->v; p.v_sb = a->v_batch_stride; p.v_sh = a->v_head_stride; p.v_share = (int)(a->heads / a->v_heads);
+    p.log_decay = a->log_decay;
+    p.state = a->state; p.st_sb = a->state_batch_stride; p.st_sh = a->state_head_stride; p.st_sk = a->state_k_stride;
+    p.out = a->out; p.o_sb = a->out_batch_stride; p.o_sh = a->out_head_stride;
+    const int vec = a->dv % 4 == 0 && aligned16(a->state) && (a->batch == 1 || p.st_sb % 4 == 0) &&
+                    (a->heads == 1 || p.st_sh % 4 == 0) && (a->dk == 1 || p.st_sk % 4 == 0);
+    cudaError_t e = launch_linattn_update(p, a->dtype == SSM_BF16, vec, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "linear attention update launch");
+    return SSM_OK;
+}
+
+// ---- layer norm --------------------------------------------------------------------------------
+static int ln_common(const char* name, const ssm_layer_norm_args* a) {
+    if (!a) return fail(SSM_ERR_INVALID, "%s: args is NULL", name);
+    if (a->rows < 1 || a->dim < 1) return fail(SSM_ERR_INVALID, "%s: sizes must be positive", name);
+    if (a->rows > ((int64_t)1 << 31) - 1 || a->dim > (1 << 24))
+        return fail(SSM_ERR_INVALID, "%s: rows must be < 2^31 and dim <= 2^24", name);
+    if (!valid_dtype(a->dtype)) return fail(SSM_ERR_INVALID, "%s: dtype must be SSM_F32 or SSM_BF16", name);
+    if (!a->x) return fail(SSM_ERR_INVALID, "%s: x is required", name);
+    return SSM_OK;
+}
+
+static LnParams ln_params(const ssm_layer_norm_args* a) {
+    LnParams p;
+    memset(&p, 0, sizeof(p));
+    p.rows = a->rows; p.dim = (int)a->dim; p.eps = a->eps; p.inv_dim = 1.f / (float)a->dim;
+    p.x = a->x; p.x_s = a->x_row_stride;
+    p.weight = a->weight; p.bias = a->bias;
+    p.mean = a->mean; p.rstd = a->rstd;
+    return p;
+}
+
+// 16-byte vectors: every row of each tensor and the weights start on 16 bytes, no partial vector
+static int ln_vec(const ssm_layer_norm_args* a, bool backward) {
+    const int64_t es = a->dtype == SSM_BF16 ? 2 : 4;
+    auto ok = [&](const void* p, int64_t s) { return aligned16(p) && (a->rows == 1 || ((s * es) & 15) == 0); };
+    return (a->dim * es) % 16 == 0 && ok(a->x, a->x_row_stride) && aligned16(a->weight) && aligned16(a->bias) &&
+           (backward ? ok(a->dy, a->dy_row_stride) && ok(a->dx, a->dx_row_stride) : ok(a->y, a->y_row_stride));
+}
+
+int ssm_layer_norm_fwd(const ssm_layer_norm_args* a, void* stream) {
+    NvtxRange r_("ssm_layer_norm_fwd");
+    int rc = ln_common("ssm_layer_norm_fwd", a);
+    if (rc) return rc;
+    if (!a->y) return fail(SSM_ERR_INVALID, "ssm_layer_norm_fwd: y is required");
+    if (!a->mean != !a->rstd) return fail(SSM_ERR_INVALID, "ssm_layer_norm_fwd: mean and rstd go together");
+    LnParams p = ln_params(a);
+    p.y = a->y; p.y_s = a->y_row_stride;
+    cudaError_t e = launch_layer_norm(p, a->dtype == SSM_BF16, ln_vec(a, false), 0, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "layer norm launch");
+    return SSM_OK;
+}
+
+size_t ssm_layer_norm_bwd_workspace_size(const ssm_layer_norm_args* a) {
+    if (ln_common("ssm_layer_norm_bwd", a)) return 0;
+    DevInfo* di = nullptr;
+    if (device_info(&di)) return 0;
+    return (size_t)layer_norm_parts(a->rows, (int)a->dim, di->sms) * 2 * a->dim * sizeof(float);
+}
+
+int ssm_layer_norm_bwd(const ssm_layer_norm_args* a, void* workspace, size_t ws_bytes, void* stream) {
+    NvtxRange r_("ssm_layer_norm_bwd");
+    int rc = ln_common("ssm_layer_norm_bwd", a);
+    if (rc) return rc;
+    if (!a->dy || !a->dx || !a->mean || !a->rstd)
+        return fail(SSM_ERR_INVALID, "ssm_layer_norm_bwd: dy, dx, mean and rstd are required");
+    DevInfo* di = nullptr;
+    if ((rc = device_info(&di))) return rc;
+    LnParams p = ln_params(a);
+    p.dy = a->dy; p.dy_s = a->dy_row_stride; p.dx = a->dx; p.dx_s = a->dx_row_stride;
+    p.dweight = a->dweight; p.dbias = a->dbias;
+    p.nparts = layer_norm_parts(a->rows, p.dim, di->sms);
+    const size_t need = (size_t)p.nparts * 2 * a->dim * sizeof(float);
+    if (!workspace || ws_bytes < need || !aligned16(workspace))
+        return fail(SSM_ERR_WORKSPACE, "ssm_layer_norm_bwd: workspace needs %zu bytes, 16-byte aligned", need);
+    p.part = static_cast<float*>(workspace);
+    cudaError_t e = launch_layer_norm(p, a->dtype == SSM_BF16, ln_vec(a, true), 1, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "layer norm backward launch");
+    return SSM_OK;
 }
 
 int ssm_exp2_compare(const float* x, float* y_fma, float* y_mufu, int64_t n, void* stream) {

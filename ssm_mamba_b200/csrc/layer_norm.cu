@@ -1,0 +1,379 @@
+// Layer norm over the last dimension, forward and backward, for sm_100a.
+//     mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r, y = h w + b
+//     c = dy w:  dx = r (c - mean(c) - h mean(c h)),   dw = sum_rows dy h,   db = sum_rows dy
+// Bound by HBM: x in and y out, or x and dy in and dx out, once.  TPR threads own a row and keep
+// it in registers (E elements each), so the second pass of the variance and the output need no
+// second reading.  All sums are float32.
+//
+// Backward: a thread owns the same columns of every row it meets, so the sums of dw and db
+// stay in its registers over all rows of a CTA; each CTA leaves one partial row, and a second
+// kernel adds the partial rows in a fixed order (deterministic, no floating-point atomics).
+//
+// Rows of more than 8192 elements do not fit the registers: they are read again for each pass
+// (from L2), and dw and db get a pass of their own.
+#include "common.cuh"
+#include "params.h"
+
+namespace ssm {
+
+namespace {
+
+// VT elements from p as raw bits, widened when used
+template <typename T, int VT> struct Raw;
+template <> struct Raw<float, 4> { float4 r; __device__ void load(const float* p) { r = *reinterpret_cast<const float4*>(p); }
+    __device__ float get(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; } };
+template <> struct Raw<float, 1> { float r; __device__ void load(const float* p) { r = *p; } __device__ float get(int) const { return r; } };
+template <> struct Raw<__nv_bfloat16, 8> { uint4 r; __device__ void load(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint4*>(p); }
+    __device__ float get(int i) const {
+        const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+        return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+    } };
+template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 r; __device__ void load(const __nv_bfloat16* p) { r = *p; }
+    __device__ float get(int) const { return __bfloat162float(r); } };
+
+template <int VT>
+__device__ __forceinline__ void load_f32(const float* p, float (&v)[VT]) {
+    if constexpr (VT == 1) v[0] = *p;
+    else
+#pragma unroll
+        for (int i = 0; i < VT; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p + i);
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+        }
+}
+
+template <typename T, int VT>
+__device__ __forceinline__ void store_elems(T* p, const float (&v)[VT]) {
+    if constexpr (VT == 1) {
+        *p = from_f<T>(v[0]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Sums of N values over the TPR threads of a row; every thread gets them.  Rows of one warp need
+// no barrier; wider rows are the CTA's only row, and `slot` alternates so that one barrier
+// per sum is enough.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* slot) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (lane == 0) slot[i * W + warp] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; w++) s += slot[i * W + w];
+            v[i] = s;
+        }
+    }
+}
+
+template <int TPR> constexpr int kRowsPerCta = TPR >= 128 ? 1 : 4;
+
+template <typename T, int VT, int E, int TPR>
+__global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_fwd_kernel(const __grid_constant__ LnParams p) {
+    constexpr int NV = E / VT, RPC = kRowsPerCta<TPR>;
+    __shared__ float slots[2][TPR / 32];
+    const int64_t row = (int64_t)blockIdx.x * RPC + threadIdx.x / TPR;
+    const int tid = threadIdx.x % TPR;
+    if (row >= p.rows) return;                    // whole warps; with TPR > 32 whole CTAs
+    const T* x = static_cast<const T*>(p.x) + row * p.x_s;
+    Raw<T, VT> xr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (tid + i * TPR) * VT;
+        if (c < p.dim) xr[i].load(x + c);
+    }
+    float v[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if ((tid + i * TPR) * VT < p.dim)
+#pragma unroll
+            for (int j = 0; j < VT; j++) v[0] += xr[i].get(j);
+    row_sum<TPR>(v, slots[0]);
+    const float mean = v[0] / (float)p.dim;    // a division: exact for a constant row's exact sum
+    v[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if ((tid + i * TPR) * VT < p.dim)
+#pragma unroll
+            for (int j = 0; j < VT; j++) {
+                const float d = xr[i].get(j) - mean;
+                v[0] = fmaf(d, d, v[0]);
+            }
+    row_sum<TPR>(v, slots[1]);
+    const float rstd = rsqrtf(fmaf(v[0], p.inv_dim, p.eps));
+    if (tid == 0 && p.mean) {
+        p.mean[row] = mean;
+        p.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(p.y) + row * p.y_s;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (tid + i * TPR) * VT;
+        if (c >= p.dim) continue;
+        float o[VT], t[VT];
+#pragma unroll
+        for (int j = 0; j < VT; j++) o[j] = (xr[i].get(j) - mean) * rstd;
+        if (p.weight) {
+            load_f32<VT>(p.weight + c, t);
+#pragma unroll
+            for (int j = 0; j < VT; j++) o[j] *= t[j];
+        }
+        if (p.bias) {
+            load_f32<VT>(p.bias + c, t);
+#pragma unroll
+            for (int j = 0; j < VT; j++) o[j] += t[j];
+        }
+        store_elems<T, VT>(y + c, o);
+    }
+}
+
+template <typename T, int VT, int E, int TPR>
+__global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(const __grid_constant__ LnParams p) {
+    constexpr int NV = E / VT, RPC = kRowsPerCta<TPR>;
+    __shared__ float slots[2][2 * (TPR / 32)];
+    __shared__ float fold[RPC > 1 ? RPC * TPR * VT : 1];
+    const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    float dw[NV][VT] = {}, db[NV][VT] = {};
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * RPC + sub; row < p.rows; row += (int64_t)gridDim.x * RPC, turn ^= 1) {
+        const T* x = static_cast<const T*>(p.x) + row * p.x_s;
+        const T* dy = static_cast<const T*>(p.dy) + row * p.dy_s;
+        Raw<T, VT> xr[NV], gr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (tid + i * TPR) * VT;
+            if (c < p.dim) {
+                xr[i].load(x + c);
+                gr[i].load(dy + c);
+            }
+        }
+        const float mean = p.mean[row], rstd = p.rstd[row];
+        float v[2] = {0.f, 0.f};                  // sum of c, sum of c h
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (tid + i * TPR) * VT;
+            if (c >= p.dim) continue;
+            float w[VT];
+            if (p.weight) load_f32<VT>(p.weight + c, w);
+#pragma unroll
+            for (int j = 0; j < VT; j++) {
+                const float g = gr[i].get(j), h = (xr[i].get(j) - mean) * rstd;
+                const float e = p.weight ? g * w[j] : g;
+                v[0] += e;
+                v[1] = fmaf(e, h, v[1]);
+                dw[i][j] = fmaf(g, h, dw[i][j]);
+                db[i][j] += g;
+            }
+        }
+        row_sum<TPR>(v, slots[turn]);
+        const float m0 = v[0] * p.inv_dim, m1 = v[1] * p.inv_dim;
+        T* dx = static_cast<T*>(p.dx) + row * p.dx_s;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (tid + i * TPR) * VT;
+            if (c >= p.dim) continue;
+            float o[VT], w[VT];
+            if (p.weight) load_f32<VT>(p.weight + c, w);
+#pragma unroll
+            for (int j = 0; j < VT; j++) {
+                const float g = gr[i].get(j), h = (xr[i].get(j) - mean) * rstd;
+                const float e = p.weight ? g * w[j] : g;
+                o[j] = rstd * (e - m0 - h * m1);
+            }
+            store_elems<T, VT>(dx + c, o);
+        }
+    }
+    // one partial row per CTA: [cta][0] dw, [cta][1] db
+    float* out = p.part + (int64_t)blockIdx.x * 2 * p.dim;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        if (which ? !p.dbias : !p.dweight) continue;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (tid + i * TPR) * VT;
+            if constexpr (RPC > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < VT; j++) fold[sub * TPR * VT + j * TPR + tid] = which ? db[i][j] : dw[i][j];
+                __syncthreads();
+                if (sub == 0 && c < p.dim)
+#pragma unroll
+                    for (int j = 0; j < VT; j++) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int q = 0; q < RPC; q++) s += fold[q * TPR * VT + j * TPR + tid];
+                        out[which * p.dim + c + j] = s;
+                    }
+            } else if (c < p.dim) {
+#pragma unroll
+                for (int j = 0; j < VT; j++) out[which * p.dim + c + j] = which ? db[i][j] : dw[i][j];
+            }
+        }
+    }
+}
+
+// ---- rows too long for the registers ----------------------------------------------------------
+constexpr int kWide = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(kWide) layer_norm_wide_fwd_kernel(const __grid_constant__ LnParams p) {
+    __shared__ float slots[2][kWide / 32];
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_s;
+    float v[1] = {0.f};
+    for (int c = threadIdx.x; c < p.dim; c += kWide) v[0] += to_f(x[c]);
+    row_sum<kWide>(v, slots[0]);
+    const float mean = v[0] / (float)p.dim;    // a division: exact for a constant row's exact sum
+    v[0] = 0.f;
+    for (int c = threadIdx.x; c < p.dim; c += kWide) {
+        const float d = to_f(x[c]) - mean;
+        v[0] = fmaf(d, d, v[0]);
+    }
+    row_sum<kWide>(v, slots[1]);
+    const float rstd = rsqrtf(fmaf(v[0], p.inv_dim, p.eps));
+    if (threadIdx.x == 0 && p.mean) {
+        p.mean[row] = mean;
+        p.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(p.y) + row * p.y_s;
+    for (int c = threadIdx.x; c < p.dim; c += kWide) {
+        const float h = (to_f(x[c]) - mean) * rstd;
+        y[c] = from_f<T>((p.weight ? h * p.weight[c] : h) + (p.bias ? p.bias[c] : 0.f));
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWide) layer_norm_wide_dx_kernel(const __grid_constant__ LnParams p) {
+    __shared__ float slots[2 * (kWide / 32)];
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_s;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.dy_s;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float v[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < p.dim; c += kWide) {
+        const float e = p.weight ? to_f(dy[c]) * p.weight[c] : to_f(dy[c]);
+        v[0] += e;
+        v[1] = fmaf(e, (to_f(x[c]) - mean) * rstd, v[1]);
+    }
+    row_sum<kWide>(v, slots);
+    const float m0 = v[0] * p.inv_dim, m1 = v[1] * p.inv_dim;
+    T* dx = static_cast<T*>(p.dx) + row * p.dx_s;
+    for (int c = threadIdx.x; c < p.dim; c += kWide) {
+        const float e = p.weight ? to_f(dy[c]) * p.weight[c] : to_f(dy[c]);
+        dx[c] = from_f<T>(rstd * (e - m0 - (to_f(x[c]) - mean) * rstd * m1));
+    }
+}
+
+// thread = column, blockIdx.y = slice of the rows
+template <typename T>
+__global__ void __launch_bounds__(256) layer_norm_wide_dw_kernel(const __grid_constant__ LnParams p) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.dim) return;
+    float dw = 0.f, db = 0.f;
+    for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const float g = to_f(static_cast<const T*>(p.dy)[row * p.dy_s + c]);
+        dw = fmaf(g, (to_f(static_cast<const T*>(p.x)[row * p.x_s + c]) - p.mean[row]) * p.rstd[row], dw);
+        db += g;
+    }
+    float* out = p.part + (int64_t)blockIdx.y * 2 * p.dim + c;
+    out[0] = dw;
+    out[p.dim] = db;
+}
+
+// dweight / dbias = sums of the nparts partial rows: 32 columns x 8 threads per CTA, each
+// thread every 8th row, then the 8 sums in order
+__global__ void __launch_bounds__(256) layer_norm_dw_kernel(const float* part, int nparts, int dim, float* dweight,
+                                                            float* dbias) {
+    __shared__ float s[8][32];
+    const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float* out = blockIdx.y ? dbias : dweight;
+    if (!out) return;
+    float sum = 0.f;
+    if (c < dim)
+        for (int i = y; i < nparts; i += 8) sum += part[((int64_t)i * 2 + blockIdx.y) * dim + c];
+    s[y][lane] = sum;
+    __syncthreads();
+    if (y == 0 && c < dim) {
+#pragma unroll
+        for (int i = 1; i < 8; i++) sum += s[i][lane];
+        out[c] = sum;
+    }
+}
+
+template <typename T, int VT, int E, int TPR>
+cudaError_t launch_rows(const LnParams& p, int backward, cudaStream_t stream) {
+    constexpr int RPC = kRowsPerCta<TPR>;
+    if (!backward) layer_norm_fwd_kernel<T, VT, E, TPR><<<(unsigned)((p.rows + RPC - 1) / RPC), TPR * RPC, 0, stream>>>(p);
+    else layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T, int VT>
+cudaError_t dispatch(const LnParams& p, int backward, cudaStream_t stream) {
+    if (p.dim <= 256) return launch_rows<T, VT, 8, 32>(p, backward, stream);
+    if (p.dim <= 512) return launch_rows<T, VT, 16, 32>(p, backward, stream);
+    if (p.dim <= 768) return launch_rows<T, VT, 24, 32>(p, backward, stream);
+    if (p.dim <= 1024) return launch_rows<T, VT, 32, 32>(p, backward, stream);
+    if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
+    if (p.dim <= 128 * 24) return launch_rows<T, VT, 24, 128>(p, backward, stream);
+    if (p.dim <= 4096) return launch_rows<T, VT, 32, 128>(p, backward, stream);
+    return launch_rows<T, VT, 16, 512>(p, backward, stream);
+}
+
+template <typename T>
+cudaError_t dispatch_wide(const LnParams& p, int backward, cudaStream_t stream) {
+    if (!backward) {
+        layer_norm_wide_fwd_kernel<T><<<(unsigned)p.rows, kWide, 0, stream>>>(p);
+    } else {
+        layer_norm_wide_dx_kernel<T><<<(unsigned)p.rows, kWide, 0, stream>>>(p);
+        if (p.dweight || p.dbias)
+            layer_norm_wide_dw_kernel<T><<<dim3((p.dim + 255) / 256, p.nparts), 256, 0, stream>>>(p);
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+// Partial rows of dw and db: one per CTA of the backward, at most two CTAs per SM, none
+// without a row; for wide rows 64 slices of the rows.
+int layer_norm_parts(int64_t rows, int dim, int sms) {
+    if (dim > kLnMaxDim) return (int)(rows < 64 ? rows : 64);
+    const int rpc = dim <= 1024 ? 4 : 1;
+    const int64_t ctas = (rows + rpc - 1) / rpc, most = (int64_t)sms * 4;
+    return (int)(ctas < most ? ctas : most);
+}
+
+cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream) {
+    cudaError_t e;
+    if (p.dim > kLnMaxDim) {
+        e = is_bf16 ? dispatch_wide<__nv_bfloat16>(p, backward, stream) : dispatch_wide<float>(p, backward, stream);
+    } else if (is_bf16) {
+        e = vec ? dispatch<__nv_bfloat16, 8>(p, backward, stream) : dispatch<__nv_bfloat16, 1>(p, backward, stream);
+    } else {
+        e = vec ? dispatch<float, 4>(p, backward, stream) : dispatch<float, 1>(p, backward, stream);
+    }
+    if (e != cudaSuccess || !backward || (!p.dweight && !p.dbias)) return e;
+    layer_norm_dw_kernel<<<dim3((p.dim + 31) / 32, 2), 256, 0, stream>>>(p.part, p.nparts, p.dim, p.dweight, p.dbias);
+    return cudaGetLastError();
+}
+
+}  // namespace ssm

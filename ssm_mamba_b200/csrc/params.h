@@ -142,4 +142,22 @@ struct UpdParams {
     int* err;            // device error word (streamed kernel's bounded waits)
 };
 
+// Layer norm over the last dimension (layer_norm.cu).
+constexpr int kLnMaxDim = 8192;          // longest row kept in registers
+struct LnParams {
+    int64_t rows;
+    int dim;
+    float eps, inv_dim;
+    const void* x; int64_t x_s;          // row strides
+    const float* weight; const float* bias;   // (dim) or null
+    void* y; int64_t y_s;
+    float* mean; float* rstd;            // (rows); forward outputs (may be null), backward inputs
+    // backward only
+    const void* dy; int64_t dy_s;
+    void* dx; int64_t dx_s;
+    float* dweight; float* dbias;        // may be null
+    float* part;                         // (nparts, 2, dim) partial sums of dweight and dbias
+    int nparts;
+};
+
 }  // namespace ssm

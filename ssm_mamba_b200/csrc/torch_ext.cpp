@@ -628,6 +628,121 @@ std::vector<at::Tensor> linear_attn_bwd(const at::Tensor& q, const at::Tensor& k
     return {dq, dk, dv, di};
 }
 
+// One decode step; `state` (batch, heads, dk, dv) is updated in place.  Returns out (batch, heads, dv).
+at::Tensor linear_attn_update(const at::Tensor& state, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                              const at::Tensor& log_decay, double scale) {
+    check_cuda(state, "state");
+    TORCH_CHECK(state.dim() == 4 && state.scalar_type() == at::kFloat && (state.stride(3) == 1 || state.size(3) == 1),
+                "state must be float32 of shape (batch, heads, dk, dv) with unit dv stride");
+    const int64_t B = state.size(0), H = state.size(1), K = state.size(2), V = state.size(3);
+    TORCH_CHECK(log_decay.is_cuda() && log_decay.dim() == 1 && log_decay.size(0) == H &&
+                    log_decay.scalar_type() == at::kFloat && log_decay.is_contiguous(),
+                "log_decay must be a contiguous float32 CUDA tensor of shape (heads,)");
+    struct Item { const at::Tensor* t; const char* name; int64_t d; };
+    for (const Item& it : {Item{&q, "q", K}, Item{&k, "k", K}, Item{&v, "v", V}}) {
+        check_cuda(*it.t, it.name);
+        TORCH_CHECK(it.t->dim() == 3 && it.t->size(0) == B && it.t->size(1) > 0 && H % it.t->size(1) == 0 &&
+                        it.t->size(2) == it.d && (it.t->stride(2) == 1 || it.d == 1),
+                    it.name, " must have shape (", B, ", n, ", it.d, ") with n dividing ", H, " and unit channel stride");
+        TORCH_CHECK(it.t->scalar_type() == q.scalar_type(), "q, k and v must share a dtype");
+        TORCH_CHECK(it.t->device() == state.device(), "state, q, k, v and log_decay must be on one device");
+    }
+    TORCH_CHECK(log_decay.device() == state.device(), "state, q, k, v and log_decay must be on one device");
+    ssm_linear_attn_update_args a;
+    memset(&a, 0, sizeof(a));
+    a.dtype = dtype_code(q);
+    c10::cuda::CUDAGuard guard(state.device());
+    at::Tensor out = at::empty({B, H, V}, q.options());
+    if (B == 0) return out;
+    a.batch = B; a.heads = H; a.dk = K; a.dv = V; a.scale = (float)scale;
+    a.q_heads = q.size(1); a.k_heads = k.size(1); a.v_heads = v.size(1);
+    a.q = q.data_ptr(); a.q_batch_stride = q.stride(0); a.q_head_stride = q.stride(1);
+    a.k = k.data_ptr(); a.k_batch_stride = k.stride(0); a.k_head_stride = k.stride(1);
+    a.v = v.data_ptr(); a.v_batch_stride = v.stride(0); a.v_head_stride = v.stride(1);
+    a.log_decay = log_decay.data_ptr<float>();
+    a.state = state.data_ptr<float>(); a.state_batch_stride = state.stride(0); a.state_head_stride = state.stride(1);
+    a.state_k_stride = state.stride(2);
+    a.out = out.data_ptr(); a.out_batch_stride = out.stride(0); a.out_head_stride = out.stride(1);
+    ok(ssm_linear_attn_update(&a, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+// ---- layer norm --------------------------------------------------------------------------------
+void check_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t dim, at::ScalarType st) {
+    check_cuda(t, name);
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == dim && (t.stride(1) == 1 || dim == 1), name,
+                " must have shape (", rows, ", ", dim, ") with unit element stride");
+    TORCH_CHECK(t.scalar_type() == st, name, " must have dtype ", st);
+}
+
+ssm_layer_norm_args ln_args(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                            const std::optional<at::Tensor>& bias, double eps) {
+    TORCH_CHECK(x.dim() == 2, "x must be a 2D tensor");
+    ssm_layer_norm_args a;
+    memset(&a, 0, sizeof(a));
+    a.dtype = dtype_code(x);
+    a.rows = x.size(0); a.dim = x.size(1); a.eps = (float)eps;
+    TORCH_CHECK(a.dim > 0, "layer norm needs at least one element per row");
+    check_rows(x, "x", a.rows, a.dim, x.scalar_type());
+    for (auto* t : {&weight, &bias}) {
+        if (!t->has_value()) continue;
+        check_f32(**t, t == &weight ? "weight" : "bias", {a.dim});
+        TORCH_CHECK((*t)->is_contiguous() && (*t)->device() == x.device(),
+                    "weight and bias must be contiguous, on the device of x");
+    }
+    a.x = x.data_ptr(); a.x_row_stride = x.stride(0);
+    a.weight = ptr<const float>(weight);
+    a.bias = ptr<const float>(bias);
+    return a;
+}
+
+// Returns [y, mean or undefined, rstd or undefined].
+std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                                       const std::optional<at::Tensor>& bias, double eps, bool want_stats) {
+    ssm_layer_norm_args a = ln_args(x, weight, bias, eps);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor y = at::empty({a.rows, a.dim}, x.options()), mean, rstd;
+    if (want_stats) {
+        mean = at::empty({a.rows}, x.options().dtype(at::kFloat));
+        rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
+        a.mean = mean.data_ptr<float>(); a.rstd = rstd.data_ptr<float>();
+    }
+    if (a.rows == 0) return {y, mean, rstd};
+    a.y = y.data_ptr(); a.y_row_stride = y.stride(0);
+    ok(ssm_layer_norm_fwd(&a, at::cuda::getCurrentCUDAStream().stream()));
+    return {y, mean, rstd};
+}
+
+// Returns [dx, dweight or undefined, dbias or undefined].
+std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                                       const at::Tensor& mean, const at::Tensor& rstd, const at::Tensor& dy,
+                                       bool want_dweight, bool want_dbias) {
+    ssm_layer_norm_args a = ln_args(x, weight, std::nullopt, 0.0);
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rows(dy, "dy", a.rows, a.dim, x.scalar_type());
+    check_f32(mean, "mean", {a.rows});
+    check_f32(rstd, "rstd", {a.rows});
+    const auto f32 = x.options().dtype(at::kFloat);
+    at::Tensor dx = at::empty({a.rows, a.dim}, x.options());
+    at::Tensor dw = want_dweight ? at::empty({a.dim}, f32) : at::Tensor();
+    at::Tensor db = want_dbias ? at::empty({a.dim}, f32) : at::Tensor();
+    if (a.rows == 0) {
+        if (want_dweight) dw.zero_();
+        if (want_dbias) db.zero_();
+        return {dx, dw, db};
+    }
+    a.mean = mean.data_ptr<float>(); a.rstd = rstd.data_ptr<float>();
+    a.dy = dy.data_ptr(); a.dy_row_stride = dy.stride(0);
+    a.dx = dx.data_ptr(); a.dx_row_stride = dx.stride(0);
+    a.dweight = want_dweight ? dw.data_ptr<float>() : nullptr;
+    a.dbias = want_dbias ? db.data_ptr<float>() : nullptr;
+    const size_t n = ssm_layer_norm_bwd_workspace_size(&a);
+    TORCH_CHECK(n > 0, ssm_last_error());
+    at::Tensor ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
+    ok(ssm_layer_norm_bwd(&a, ws.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()));
+    return {dx, dw, db};
+}
+
 int64_t check_device_error() {
     int code = 0;
     ssm_check_device_error(&code, at::cuda::getCurrentCUDAStream().stream());
@@ -650,6 +765,9 @@ PYBIND11_MODULE(_C, m) {
     m.def("conv1d_update", &conv1d_update, "causal depthwise conv1d (+ SiLU) decode step");
     m.def("linear_attn_fwd", &linear_attn_fwd, "linear attention with a decay for each head, forward");
     m.def("linear_attn_bwd", &linear_attn_bwd, "linear attention with a decay for each head, backward");
+    m.def("linear_attn_update", &linear_attn_update, "linear attention with a decay for each head, one decode step");
+    m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward");
+    m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward");
     m.def("ckpt_from_reference", &ckpt_from_reference, "compact checkpoints from reference chunk states");
     m.def("state_update", &state_update, "one decode step");
     m.def("ckpt_len", [](int64_t n) { return ssm_scan_ckpt_len(n); });

@@ -79,4 +79,16 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
                                    ensure_contiguous(initial_state), lengths, bool(return_last_state))
 
 
-__all__ = ["LinearAttentionFn", "linear_attention_fn"]
+def linear_attention_update(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            log_decay: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """One decode step; `state` (batch, heads, dk, dv) float32 is updated in place.
+
+    q, k: (batch, heads, dk); v: (batch, heads, dv), fewer heads as in linear_attention_fn.
+    Returns out (batch, heads, dv) in q's dtype.  Not differentiable."""
+    _check("linear_attention_update", q, k, v, log_decay)
+    q, k, v = map(_unit_channel_stride, (q, k, v))
+    return _C.linear_attn_update(state, q, k, v, log_decay.float().contiguous(),
+                                 float(q.shape[-1] ** -0.5 if scale is None else scale))
+
+
+__all__ = ["LinearAttentionFn", "linear_attention_fn", "linear_attention_update"]
