@@ -49,6 +49,7 @@ cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width
                                  float* dbias, int sms, cudaStream_t stream);
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
+cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, cudaStream_t stream);
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_update(const LaUpdParams& p, int is_bf16, int vec, cudaStream_t stream);
 cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream);
@@ -171,7 +172,14 @@ int device_info(DevInfo** out) {
 // ---- TMA tensor maps ---------------------------------------------------------------------------
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
+// The encoder, with the calling thread bound to the device's primary context: the driver call
+// needs a current context, and a thread that has made no runtime call that needs one (the one
+// that runs a framework's backward) has none.
 int get_encoder() {
+    int dev = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce == cudaSuccess) ce = cudaSetDevice(dev);
+    if (ce != cudaSuccess) return cuda_fail(ce, "cudaSetDevice");
     if (g_encode) return SSM_OK;
     std::lock_guard<std::mutex> lk(g_mu);
     if (g_encode) return SSM_OK;
@@ -988,6 +996,28 @@ static int la_plan_segments(const ssm_linear_attn_args* a, int sms, int* seglen)
     return (int)((a->seqlen + len - 1) / len);
 }
 
+// Map of a bfloat16 (batch, token, head, channel) tensor; box of 64 channels x 128 tokens, 128-byte
+// swizzle, zeros outside.
+static int la_encode(CUtensorMap* map, const void* ptr, int64_t d, int64_t L, int64_t heads, int64_t batch, int64_t st,
+                     int64_t sh, int64_t sb) {
+    cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)L, (cuuint64_t)heads, (cuuint64_t)batch};
+    // a dimension of size 1 may have any stride; give TMA a valid one
+    cuuint64_t strides[3] = {(cuuint64_t)(L == 1 ? 256 : st * 2), (cuuint64_t)(heads == 1 ? 256 : sh * 2),
+                             (cuuint64_t)(batch == 1 ? 256 : sb * 2)};
+    cuuint32_t box[4] = {64u, 128u, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SSM_ERR_CUDA, "cuTensorMapEncodeTiled (linear attention) failed (%d)", (int)r);
+    return SSM_OK;
+}
+
+// Can a TMA fetch this tensor: aligned, and no dimension repeated with a stride of zero?
+static bool la_tma_ok(const LaTensor& t, int64_t L, int64_t heads, int64_t batch) {
+    auto ok = [](int64_t n, int64_t s) { return n == 1 || (s > 0 && s * 2 < ((int64_t)1 << 40)); };
+    return t.vec && ok(L, t.st) && ok(heads, t.sh) && ok(batch, t.sb);
+}
+
 namespace {
 // Workspace: per role the segment states, then the per-head gradients of shared heads.
 struct LaPlan {
@@ -1101,7 +1131,33 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.role[2].state0 = a->dlast_state;
     }
     const int is_bf16 = a->dtype == SSM_BF16;
-    cudaError_t e = launch_linattn_simt(p, is_bf16, stream);
+    bool tc = is_bf16 != 0;
+    for (int i = 0; i < p.nroles; i++) {
+        const LaRole& r = p.role[i];
+        for (const LaTensor* t : {&r.a, &r.b, &r.c}) tc = tc && la_tma_ok(*t, a->seqlen, H / t->share, a->batch);
+    }
+    cudaError_t e;
+    if (tc) {
+        if ((rc = get_encoder())) return rc;
+        LaMaps maps;
+        memset(&maps, 0, sizeof(maps));
+        for (int i = 0; i < p.nroles; i++) {
+            const LaRole& r = p.role[i];
+            auto in = [&](CUtensorMap* m, const LaTensor& t, int d) {
+                return la_encode(m, t.p, d, a->seqlen, H / t.share, a->batch, t.st, t.sh, t.sb);
+            };
+            if ((rc = in(&maps.a[i], r.a, r.db)) || (rc = in(&maps.b[i], r.b, r.db)) || (rc = in(&maps.c[i], r.c, r.dc)))
+                return rc;
+            if (!r.out_f32 && r.out_vec &&
+                (rc = la_encode(&maps.o[i], r.out, r.dc, a->seqlen, H, a->batch, r.o_st, r.o_sh, r.o_sb)))
+                return rc;
+        }
+        const int kmax = dk > dv ? dk : dv;
+        const int kb = backward ? kmax : dk, kc = backward ? kmax : dv;
+        e = launch_linattn_tc(p, maps, kb <= 64 ? 64 : 128, kc <= 64 ? 64 : 128, stream);
+    } else {
+        e = launch_linattn_simt(p, is_bf16, stream);
+    }
     if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
     for (int i = 0; backward && i < 3; i++) {
         if (!p.role[i].out_f32) continue;

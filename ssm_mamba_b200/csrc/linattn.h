@@ -2,6 +2,7 @@
 // Built by capi.cu from the C-ABI argument struct after validation; strides are in elements.
 #pragma once
 
+#include <cuda.h>
 #include <stdint.h>
 
 namespace ssm {
@@ -49,6 +50,11 @@ struct LaParams {
     const int64_t* length;  // may be null
     int* err;             // device error word
     LaRole role[3];
+};
+
+// TMA maps of every role's tensors: (channel, token, head, batch), boxes of 64 channels x 128 tokens
+struct LaMaps {
+    CUtensorMap a[3], b[3], c[3], o[3];
 };
 
 // out[b, t, g, :] = sum of the share heads of src (batch, seqlen, heads, d) float32
