@@ -46,16 +46,16 @@ constexpr uint32_t kColC = 384;            // 64 + 64: second and first plane of
 // Decay tables in shared memory, filled once per CTA.
 struct Decays {
     float pow[kT + 1];                     // w^0 .. w^128
-    alignas(16) float block[32];           // within a 32-column block of P: w^(31 - k), reverse w^k
+    float score[kT];                       // alpha w^d: weights of P by distance
     alignas(16) float full[kT];            // weights of C' for a chunk of 128 tokens
     alignas(16) float part[kT];            // and for the row's one shorter chunk, zero past its end
 };
 
-__device__ __forceinline__ void fill_decays(Decays& d, float g2, float sigma, int reverse, int n_part) {
+__device__ __forceinline__ void fill_decays(Decays& d, float g2, float alpha, float sigma, int reverse, int n_part) {
     for (int i = threadIdx.x; i <= kT; i += kThreads) {
         d.pow[i] = exp2f(g2 * (float)i);
-        if (i < 32) d.block[i] = exp2f(g2 * (float)(reverse ? i : 31 - i));
         if (i < kT) {
+            d.score[i] = alpha * exp2f(g2 * (float)i);
             d.full[i] = sigma * exp2f(g2 * (float)(reverse ? i + 1 : kT - 1 - i));
             d.part[i] = i < n_part ? sigma * exp2f(g2 * (float)(reverse ? i + 1 : n_part - 1 - i)) : 0.f;
         }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         *abort = 0;
         fence_mbar_init();
     }
-    fill_decays(dec, g2, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
+    fill_decays(dec, g2, r.alpha, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -259,11 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             tma_store_wait_all();
             if (*abort)      // copies in flight still write to this CTA's shared memory
                 for (int c = max(0, issued - 2); c < issued; c++) mbar_wait_bounded(bars + kFull + (c & 1), (c >> 1) & 1);
-        } else if (warp == 8 && lane == 0) {
+        } else if (warp == 8 && elect_one()) {
             // ---- products -----------------------------------------------------------------------
             constexpr uint32_t id_scores = umma_idesc(128, 128, false), id_as = umma_idesc(128, KC, false),
                                id_pc = umma_idesc(128, KC, true), id_upd = umma_idesc(128, KB, true);
-            const uint64_t s_desc = umma_desc(smem_u32(smem + L::OFF_S), 16);
+            const uint32_t s_desc = umma_desc_lo(smem_u32(smem + L::OFF_S), 16);
             for (int c = 0; c < nchunk; c++) {
                 const uint32_t st = smem_u32(smem + (c & 1) * L::STAGE), par = c & 1;
                 if (!wait(kFull + (c & 1), (c >> 1) & 1)) break;
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 if (c > 0 && !(wait(kPC, par ^ 1) && wait(kUpd, par ^ 1))) break;
                 tc_fence_after();
                 // K-major panels of 64 channels: 16 channels are 32 bytes
-                const uint64_t a_desc = umma_desc(st, 16), b_desc = umma_desc(st + L::A, 16);
+                const uint32_t a_desc = umma_desc_lo(st, 16), b_desc = umma_desc_lo(st + L::A, 16);
 #pragma unroll
                 for (int i = 0; i < KB / 16; i++) {
                     const uint32_t off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 if (!wait(kCReady, par)) break;
                 tc_fence_after();
                 // N-major panels of 64 channels: 16 tokens are 2048 bytes
-                const uint64_t bn_desc = umma_desc(st + L::A, kPanel), cn_desc = umma_desc(st + 2 * L::A, kPanel);
+                const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
 #pragma unroll
                 for (int i = 0; i < 2 * kT / 16; i++)      // second plane, then first
                     umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, i > 0);
@@ -329,21 +329,33 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         };
         auto ok = [&](bool v) { return __all_sync(0xffffffffu, v); };
 
-        // S^T of the first chunk: the initial state and the segments before this one
+        // S^T of the first chunk: the initial state, then the segments before this one.  Through TMEM,
+        // so that the loop over columns stays a loop (registers have no index).
         float s[NS];
+        if (s_on) {
+            const float* src0 = r.state0 && row < r.dc ? r.state0 + k.bh * r.db * r.dc + row * r.s_j : nullptr;
+            const float* src = r.seg + k.bh * p.nseg * r.db * r.dc + row;
+#pragma unroll 1
+            for (int i = 0; i < NS; i += 8) {
+                float x[8];
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const int ii = i0 + i;
-            s[i] = s_on && r.state0 && row < r.dc && ii < r.db
-                       ? r.state0[k.bh * r.db * r.dc + (int64_t)ii * r.s_i + row * r.s_j] : 0.f;
-        }
-        for (int e = 0; e < k.slot; e++) {
-            const int sg = reverse ? p.nseg - 1 - e : e;
-            const float f = exp2f(g2 * (float)la_segment_tokens(p, k.row_len, sg));
-            const float* src = r.seg + (k.bh * p.nseg + sg) * r.db * r.dc;
+                for (int e = 0; e < 8; e++) x[e] = src0 && i0 + i + e < r.db ? src0[(i0 + i + e) * r.s_i] : 0.f;
+#pragma unroll 1
+                for (int g = 0; g < k.slot; g++) {
+                    const int sg = reverse ? p.nseg - 1 - g : g;
+                    const float f = exp2f(g2 * (float)la_segment_tokens(p, k.row_len, sg));
 #pragma unroll
-            for (int i = 0; i < NS; i++)
-                if (s_on && row < r.dc && i0 + i < r.db) s[i] = fmaf(f, s[i], src[(i0 + i) * r.dc + row]);
+                    for (int e = 0; e < 8; e++)
+                        x[e] = fmaf(f, x[e], row < r.dc && i0 + i + e < r.db ? src[(sg * r.db + i0 + i + e) * r.dc] : 0.f);
+                }
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = __float_as_uint(x[e]);
+                tmem_st8(tm + kColU + i0 + i, v);
+            }
+            tmem_wait_st();
+#pragma unroll
+            for (int i = 0; i < NS; i++) s[i] = 0.f;
         }
         // bfloat16(S^T) to shared memory for A S
         auto put_state = [&]() {
@@ -371,7 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 for (int e = 0; e < 32; e++) s[i + e] = fmaf(fn, s[i + e], __uint_as_float(v[e]));
             }
         };
-        if (nchunk > 0) put_state();
+        add_update(0);
+        if (nchunk > 0) {
+            tc_fence_before();
+            put_state();
+        }
 
         bool fine = true;
         for (int c = 0; c < nchunk; c++) {
@@ -397,38 +413,29 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             tc_fence_before();
             arrive(kCReady);
 
-            // P: 32 x 32 blocks are whole, on the diagonal or empty for the whole warp
+            // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
             if (!(fine = ok(wait(kScores, par)))) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int blk = 0; blk < 2; blk++) {
                 const int sb = half * 2 + blk;
-                uint32_t v[32], o[16];
-                const bool whole = reverse ? sb > q : sb < q;
-                if (whole || sb == q) {
+                uint32_t o[16];
+                if (reverse ? sb >= q : sb <= q) {
+                    uint32_t v[32];
                     tmem_ld32(tm + kColScores + sb * 32, v);
                     tmem_wait_ld();
-                }
-                if (whole) {
-                    // w^|t - s| as two factors, neither above one: up to the block's edge and inside it
-                    const float f = r.alpha * dec.pow[reverse ? sb * 32 - row : row - (sb * 32 + 31)];
+                    const int d0 = reverse ? sb * 32 - row : row - sb * 32;   // distance to the block's first column
+                    const float* wt = dec.score + d0;
+                    if (reverse) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float4 wb = lds128(dec.block + 2 * e);
-                        o[e] = pack_bf16(__uint_as_float(v[2 * e]) * (f * wb.x), __uint_as_float(v[2 * e + 1]) * (f * wb.y));
-                        o[e + 1] = pack_bf16(__uint_as_float(v[2 * e + 2]) * (f * wb.z),
-                                             __uint_as_float(v[2 * e + 3]) * (f * wb.w));
-                    }
-                } else if (sb == q) {
+                        for (int e = 0; e < 16; e++)
+                            o[e] = pack_bf16(d0 + 2 * e >= 0 ? __uint_as_float(v[2 * e]) * wt[2 * e] : 0.f,
+                                             d0 + 2 * e + 1 >= 0 ? __uint_as_float(v[2 * e + 1]) * wt[2 * e + 1] : 0.f);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float x[2];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int d = reverse ? e + u - lane : lane - (e + u);
-                            x[u] = d >= 0 ? __uint_as_float(v[e + u]) * (r.alpha * dec.pow[max(d, 0)]) : 0.f;
-                        }
-                        o[e / 2] = pack_bf16(x[0], x[1]);
+                        for (int e = 0; e < 16; e++)
+                            o[e] = pack_bf16(d0 >= 2 * e ? __uint_as_float(v[2 * e]) * wt[-2 * e] : 0.f,
+                                             d0 >= 2 * e + 1 ? __uint_as_float(v[2 * e + 1]) * wt[-2 * e - 1] : 0.f);
                     }
                 } else {
 #pragma unroll
@@ -487,20 +494,26 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     *reinterpret_cast<uint4*>(st + (oc >> 6) * kPanel + swz128(row, (oc & 63) * 2)) = v;
                 }
                 fence_proxy_async_smem();
-            } else if (row < n) {
-                const int64_t at = k.b * r.o_sb + (int64_t)(first(c) + row) * r.o_st + k.h * r.o_sh + o0;
-                const int cols = min(NO, r.dc - o0);
-                if (r.out_f32) {
-                    float* op = static_cast<float*>(r.out) + at;
+            } else {
+                // float32 partials and rows a TMA cannot store: through the warp's own piece of the stage,
+                // 16-byte pieces swizzled by the row, then row by row
+                float* own = reinterpret_cast<float*>(st) + warp * 32 * NO;
 #pragma unroll
-                    for (int i = 0; i < NO; i++)
-                        if (i < cols) op[i] = acc[i];
-                } else {
-                    __nv_bfloat16* op = static_cast<__nv_bfloat16*>(r.out) + at;
-#pragma unroll
-                    for (int i = 0; i < NO; i++)
-                        if (i < cols) op[i] = __float2bfloat16_rn(acc[i]);
+                for (int i = 0; i < NO; i += 4)
+                    *reinterpret_cast<float4*>(own + lane * NO + (((i >> 2) ^ (lane & 7)) << 2)) =
+                        make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                __syncwarp();
+                const int64_t at = k.b * r.o_sb + (int64_t)(first(c) + q * 32) * r.o_st + k.h * r.o_sh + o0;
+                const int cols = min(NO, r.dc - o0), rows = min(32, n - q * 32);
+#pragma unroll 1
+                for (int i = lane; i < rows * NO; i += 32) {
+                    const int rw = i / NO, col = i % NO;
+                    const float x = own[rw * NO + (((col >> 2) ^ (rw & 7)) << 2) + (col & 3)];
+                    if (col >= cols) continue;
+                    if (r.out_f32) static_cast<float*>(r.out)[at + rw * r.o_st + col] = x;
+                    else static_cast<__nv_bfloat16*>(r.out)[at + rw * r.o_st + col] = __float2bfloat16_rn(x);
                 }
+                fence_proxy_async_smem();
             }
             tc_fence_before();
             arrive(kStaged + (c & 1));
@@ -509,9 +522,23 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         if (fine) {
             if (k.slot == p.nseg - 1 && r.state_out && s_on) {
 #pragma unroll
-                for (int i = 0; i < NS; i++)
-                    if (row < r.dc && i0 + i < r.db)
-                        r.state_out[k.bh * r.db * r.dc + (int64_t)(i0 + i) * r.s_i + row * r.s_j] = s[i];
+                for (int i = 0; i < NS; i += 32) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(s[i + e]);
+                    tmem_st32(tm + kColU + i0 + i, v);
+                }
+                tmem_wait_st();
+                float* dst = r.state_out + k.bh * r.db * r.dc + row * r.s_j;
+#pragma unroll 1
+                for (int i = 0; i < NS; i += 8) {
+                    uint32_t v[8];
+                    tmem_ld8(tm + kColU + i0 + i, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (row < r.dc && i0 + i + e < r.db) dst[(i0 + i + e) * r.s_i] = __uint_as_float(v[e]);
+                }
             }
             // tokens past the row's length
             const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * KC;
@@ -584,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
         *abort = 0;
         fence_mbar_init();
     }
-    fill_decays(dec, g2, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
+    fill_decays(dec, g2, r.alpha, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -615,15 +642,15 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
         }
         __syncwarp();
     } else if (warp == 8) {
-        if (lane == 0) {
+        if (elect_one()) {
             constexpr uint32_t id_upd = umma_idesc(128, KB, true);
             for (int c = 0; c < nchunk; c++) {
                 if (!wait(kSbFull + c % kStages, (c / kStages) & 1)) break;
                 if (!wait(kSbReady + (c & 1), (c >> 1) & 1)) break;
                 tc_fence_after();
-                const uint64_t bn_desc = umma_desc(smem_u32(smem + (c % kStages) * L::STAGE), kPanel);
+                const uint32_t bn_desc = umma_desc_lo(smem_u32(smem + (c % kStages) * L::STAGE), kPanel);
                 const uint32_t cp = tmem + 128 + (c & 1) * 192;
-#pragma unroll 8
+#pragma unroll
                 for (int i = 0; i < 3 * kT / 16; i++)
                     umma_ts(tmem, cp + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, c > 0 || i > 0);
                 umma_commit(bars + kSbFree + c % kStages);
@@ -675,18 +702,16 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
         if (fine && s_on) {
             constexpr int NS = KB / 2;
             float* e = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc;
-#pragma unroll
-            for (int i = 0; i < NS; i += 32) {
-                uint32_t v[32];
+#pragma unroll 1
+            for (int i = half * NS; i < half * NS + NS; i += 8) {
+                uint32_t v[8] = {};
                 if (nchunk > 0) {
-                    tmem_ld32(tm + half * NS + i, v);
+                    tmem_ld8(tm + i, v);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int u = 0; u < 32; u++) {
-                    const int ii = half * NS + i + u;
-                    if (row < r.dc && ii < r.db) e[ii * r.dc + row] = nchunk > 0 ? __uint_as_float(v[u]) : 0.f;
-                }
+                for (int u = 0; u < 8; u++)
+                    if (row < r.dc && i + u < r.db) e[(i + u) * r.dc + row] = __uint_as_float(v[u]);
             }
         }
     }
