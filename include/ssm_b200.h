@@ -329,8 +329,8 @@ typedef struct ssm_linear_attn_args {
 } ssm_linear_attn_args;
 
 /* Bytes of device workspace of the forward (backward = 0) or the backward (backward = 1): the
- * states of the segments that a long row is cut into, and per-head gradients of shared heads.
- * May be 0 (also on an error: ssm_last_error() is then non-empty and the call itself fails). */
+ * states of the segments that a long row is cut into, the states of rows that two CTAs share,
+ * and per-head gradients of shared heads.  May be 0 (also on an error: ssm_last_error() is then non-empty and the call itself fails). */
 SSM_API size_t ssm_linear_attn_workspace_size(const ssm_linear_attn_args* args, int backward);
 /* Forward in chunks.  The workspace is 256-byte aligned. */
 SSM_API int ssm_linear_attn_fwd(const ssm_linear_attn_args* args, void* workspace, size_t workspace_bytes,

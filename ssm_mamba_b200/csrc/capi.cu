@@ -49,7 +49,7 @@ cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width
                                  float* dbias, int sms, cudaStream_t stream);
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
-cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, cudaStream_t stream);
+cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_update(const LaUpdParams& p, int is_bf16, int vec, cudaStream_t stream);
 cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream);
@@ -980,20 +980,26 @@ static int la_common(const char* name, const ssm_linear_attn_args* a) {
     return SSM_OK;
 }
 
-// Tokens per segment: a multiple of the longest chunk.  Cutting a row in n segments costs
-// another reading of b and c, so it is done only where the (batch, head) pairs alone give the
-// SMs less than two CTAs each.
-static int la_plan_segments(const ssm_linear_attn_args* a, int sms, int* seglen) {
-    const int64_t rows = a->batch * a->heads;
-    int64_t want = (2 * (int64_t)sms + rows - 1) / rows;
-    const int64_t most = a->seqlen / 512;      // at least 512 tokens each
-    if (want > most) want = most;
-    if (want > 16) want = 16;                  // every CTA folds the states of those before it
-    if (want < 1) want = 1;
-    int64_t len = (a->seqlen + want - 1) / want;
-    len = (len + 127) / 128 * 128;
+// Segments of a row, for `rows` independent (batch row, head, role) triples.  More segments fill more
+// SMs but cost a second reading of b and c (the state pass, about 0.45 of a chunk's time per chunk)
+// and a launch (about two chunks' time); measured on B200 at 40 rows of 1024 chunks.  The SMs share
+// the chunks evenly once there are more rows than SMs.
+static int la_plan_segments(int64_t rows, int64_t seqlen, int sms, int* seglen) {
+    const int64_t chunks = (seqlen + 127) / 128;
+    int best = 1;
+    double best_t = 0;
+    for (int n = 1; n <= 16 && (n == 1 || chunks >= 4 * n); n++) {   // at least 512 tokens each
+        const int64_t len = (chunks + n - 1) / n, all = rows * n;
+        double t = all <= sms ? (double)len : (double)(rows * chunks) / sms + 1;
+        if (n > 1) t += 0.45 * (double)(len * ((rows * (n - 1) + sms - 1) / sms)) + 2;
+        if (n == 1 || t < best_t) {
+            best = n;
+            best_t = t;
+        }
+    }
+    const int64_t len = (chunks + best - 1) / best * 128;
     *seglen = (int)len;
-    return (int)((a->seqlen + len - 1) / len);
+    return (int)((seqlen + len - 1) / len);
 }
 
 // Map of a bfloat16 (batch, token, head, channel) tensor; box of 64 channels x 128 tokens, 128-byte
@@ -1021,16 +1027,27 @@ static bool la_tma_ok(const LaTensor& t, int64_t L, int64_t heads, int64_t batch
 namespace {
 // Workspace: per role the segment states, then the per-head gradients of shared heads.
 struct LaPlan {
-    int nseg, seglen;
-    size_t seg[3], part[3], bytes;             // byte offsets
+    int nseg, seglen, split;
+    size_t seg[3], part[3], flags, handoff, bytes;   // byte offsets
 };
 }  // namespace
 
 static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     LaPlan pl;
     memset(&pl, 0, sizeof(pl));
-    pl.nseg = la_plan_segments(a, sms, &pl.seglen);
     const int nroles = backward ? 3 : 1;
+    const int64_t rows = a->batch * a->heads * nroles;
+    if (a->dtype == SSM_BF16) {
+        pl.nseg = la_plan_segments(rows, a->seqlen, sms, &pl.seglen);
+    } else {
+        // the float32 kernel runs two or more smaller CTAs per SM: two per SM, of 512 tokens or more
+        int64_t n = (2 * (int64_t)sms + rows - 1) / rows;
+        n = n < a->seqlen / 512 ? n : a->seqlen / 512;
+        n = n < 1 ? 1 : n > 16 ? 16 : n;
+        pl.seglen = (int)(((a->seqlen + n - 1) / n + 127) / 128 * 128);
+        pl.nseg = (int)((a->seqlen + pl.seglen - 1) / pl.seglen);
+    }
+    pl.split = rows * pl.nseg > sms;
     auto take = [&](size_t n) {
         const size_t at = pl.bytes;
         pl.bytes += (n + 255) / 256 * 256;
@@ -1039,6 +1056,10 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     if (pl.nseg > 1)
         for (int i = 0; i < nroles; i++)
             pl.seg[i] = take((size_t)a->batch * a->heads * pl.nseg * a->dk * a->dv * sizeof(float));
+    if (pl.split && a->dtype == SSM_BF16) {
+        pl.flags = take((size_t)(sms + 1) * sizeof(int));
+        pl.handoff = take((size_t)(sms + 1) * 128 * 128 * sizeof(float));
+    }
     if (backward) {
         const int64_t heads[3] = {a->q_heads, a->v_heads, a->k_heads}, d[3] = {a->dk, a->dv, a->dk};
         for (int i = 0; i < 3; i++)
@@ -1085,6 +1106,11 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
     memset(&p, 0, sizeof(p));
     p.batch = (int)a->batch; p.seqlen = (int)a->seqlen; p.heads = (int)a->heads;
     p.nseg = pl.nseg; p.seglen = pl.seglen;
+    p.split = pl.split;
+    if (pl.split && a->dtype == SSM_BF16) {
+        p.flags = reinterpret_cast<int*>(ws + pl.flags);
+        p.handoff = reinterpret_cast<float*>(ws + pl.handoff);
+    }
     p.log_decay = a->log_decay; p.length = a->length; p.err = di->err;
     const LaTensor q = la_tensor(a, a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads);
     const LaTensor k = la_tensor(a, a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads);
@@ -1154,7 +1180,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         }
         const int kmax = dk > dv ? dk : dv;
         const int kb = backward ? kmax : dk, kc = backward ? kmax : dv;
-        e = launch_linattn_tc(p, maps, kb <= 64 ? 64 : 128, kc <= 64 ? 64 : 128, stream);
+        e = launch_linattn_tc(p, maps, kb <= 64 ? 64 : 128, kc <= 64 ? 64 : 128, di->sms, stream);
     } else {
         e = launch_linattn_simt(p, is_bf16, stream);
     }

@@ -1,8 +1,8 @@
 // Linear attention with a decay for each head on the fifth-generation tensor cores: bfloat16
 // streams whose rows a TMA can fetch (the recurrence and its four uses are in linattn.h).
 //
-// A CTA walks one (batch row, head, segment) in chunks of 128 tokens.  Per chunk, with
-// w = exp(log_decay[h]) and the float32 state S^T (row = channel of c) in registers:
+// A row is one (batch row, head, role, segment); it is walked in chunks of 128 tokens.  Per chunk,
+// with w = exp(log_decay[h]) and the float32 state S^T (row = channel of c) in registers:
 //     scores = A B^T                         128 x 128, then P = alpha scores o W as bfloat16
 //     O      = P C + beta diag(w^.) (A S)    two products; the second is taken out of TMEM and
 //                                            scaled per row before the first uses its columns
@@ -13,12 +13,20 @@
 //
 // Roundings below float32: P and the copy of S that A multiplies are bfloat16, each on its own
 // part of O, whose result is rounded to bfloat16 anyway.  The state itself is float32: C' is
-// carried as a sum of three bfloat16 planes (24 bits) with the smallest terms added first where the
-// TMEM has room, and U is added to the decayed state in float32.
+// carried as a sum of three bfloat16 planes (24 bits) and U is added to the decayed state in
+// float32.
 //
-// Warps 0-7 (two warpgroups, each with half of the columns) do the work between products;
-// warp 8 issues the products, warp 9 the copies.  The order of the phases lets each run beside a
-// product:  C'(c) | scores, A S;   P(c) | U;   S(c + 1) | P C;   O(c) | scores(c + 1).
+// One CTA per SM.  Warps 0-15 do the work between products, four for each quarter of the TMEM
+// lanes, each with a quarter of the columns; warp 16 issues the products, warp 17 the loads, warp
+// 18 the stores.  The order of the phases lets each run beside a product:
+//     C'(c) | scores, A S;   P(c) | U;   S(c + 1) | P C;   O(c) | scores(c + 1).
+//
+// With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
+// range, so its first row may have been begun by the CTA before it and its last may be finished
+// by the next.  It does the beginning of its last row first and publishes the state it reaches, and
+// the end of its first row last: by then the state it needs is there, since the two parts of a
+// row together are no longer than a CTA's range.
+//
 // Every wait is bounded: the first that runs out sets the device error word and a flag that
 // ends all others.
 #include "common.cuh"
@@ -31,19 +39,21 @@ namespace {
 
 constexpr int kT = 128;                    // tokens per chunk
 constexpr int kPanel = kT * 128;           // bytes of 128 rows x 64 channels
-constexpr int kCompute = 256;
-constexpr int kThreads = kCompute + 128;   // the third warpgroup issues copies and products
-// Registers: launched with 168 each (384 * 168 = 64512 = 256 * 224 + 128 * 56)
-constexpr int kRegsCompute = 224, kRegsControl = 56;
+constexpr int kWarps = 16;                 // compute warps
+constexpr int kCompute = kWarps * 32;
+constexpr int kThreads = kCompute + 128;   // the last warpgroup issues copies and products
+// Registers: launched with 96 each (640 * 96 = 512 * 104 + 128 * 64)
+constexpr int kRegsCompute = 104, kRegsControl = 64;
 constexpr uint32_t kTmemCols = 512;
 // TMEM columns
-constexpr uint32_t kColScores = 0;         // 128: scores, then P in [0, 32) and [64, 96), the
-                                           //      third plane of C' in [32, 64) and [96, 128)
+constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P then takes the first 16
+                                           //      and the third plane of C' the last 16
 constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
 constexpr uint32_t kColC = 384;            // 64 + 64: second and first plane of C'^T
+constexpr float kZeroLog2 = -151.f;        // exp2 of anything below is zero in float32
 
-// Decay tables in shared memory, filled once per CTA.
+// Decay tables in shared memory, filled once per row.
 struct Decays {
     float pow[kT + 1];                     // w^0 .. w^128
     float score[kT];                       // alpha w^d: weights of P by distance
@@ -52,15 +62,20 @@ struct Decays {
 };
 
 __device__ __forceinline__ void fill_decays(Decays& d, float g2, float alpha, float sigma, int reverse, int n_part) {
-    for (int i = threadIdx.x; i <= kT; i += kThreads) {
-        d.pow[i] = exp2f(g2 * (float)i);
-        if (i < kT) {
-            d.score[i] = alpha * exp2f(g2 * (float)i);
-            d.full[i] = sigma * exp2f(g2 * (float)(reverse ? i + 1 : kT - 1 - i));
-            d.part[i] = i < n_part ? sigma * exp2f(g2 * (float)(reverse ? i + 1 : n_part - 1 - i)) : 0.f;
-        }
+    const int i = threadIdx.x;
+    if (i <= kT) d.pow[i] = exp2f(g2 * (float)i);
+    if (i < kT) {
+        d.score[i] = alpha * exp2f(g2 * (float)i);
+        d.full[i] = sigma * exp2f(g2 * (float)(reverse ? i + 1 : kT - 1 - i));
+        d.part[i] = i < n_part ? sigma * exp2f(g2 * (float)(reverse ? i + 1 : n_part - 1 - i)) : 0.f;
     }
 }
+
+// The chunks [c0, c1) that a CTA does of rows [row0, row1]: from chunk c0 of the first row up to
+// chunk c1 of the last.
+struct Range {
+    int row0, row1, c0, c1;
+};
 
 // KB: channels of a and b, KC: channels of c and out, padded to 64 or 128
 template <int KB, int KC>
@@ -71,14 +86,14 @@ struct TcSmem {
     static constexpr int OFF_S = 2 * STAGE;
     static constexpr int OFF_W = OFF_S + S;
     static constexpr int OFF_BAR = OFF_W + (int)sizeof(Decays);
-    static constexpr int NBAR = 16;
+    static constexpr int NBAR = 18;
     static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-    static constexpr int USED = OFF_MISC + 16;
+    static constexpr int USED = OFF_MISC + 16 + (int)sizeof(Range);
     // more than half an SM, so that two CTAs never share one SM's TMEM
     static constexpr int BYTES = USED > 120 * 1024 ? USED : 120 * 1024;
 };
 
-enum Bar { kFull = 0, kStaged = 2, kScores = 4, kAS, kUpd, kPC, kSReady, kCReady, kPReady, kFixed, kDrain };
+enum Bar { kFull = 0, kStaged = 2, kFree = 4, kScores = 6, kAS, kUpd, kPC, kSReady, kCReady, kPReady, kFixed, kItem, kDrain };
 
 struct Waiter {
     uint64_t* bars;
@@ -87,18 +102,17 @@ struct Waiter {
     // false once any wait of the CTA has run out
     __device__ __forceinline__ bool operator()(int bar, uint32_t parity) const {
         if (mbar_try_wait(bars + bar, parity)) return true;
-        return slow(bar, parity);
-    }
-    __device__ __forceinline__ bool slow(int bar, uint32_t parity) const {
         const long long start = clock64();
-        while (!mbar_try_wait(bars + bar, parity)) {
-            if (*abort) return false;
-            if (clock64() - start > 2000000000LL) {
-                *abort = 1;
-                *err = kDevErrTmaTimeout;
-                return false;
-            }
-        }
+        while (!mbar_try_wait(bars + bar, parity))
+            if (gone(start)) return false;
+        return true;
+    }
+    // has any wait run out, this one included?
+    __device__ __forceinline__ bool gone(long long start) const {
+        if (*abort) return true;
+        if (clock64() - start <= 2000000000LL) return false;
+        *abort = 1;
+        *err = kDevErrTmaTimeout;
         return true;
     }
 };
@@ -110,11 +124,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// Cuts the leading bfloat16 (by truncation: what is left is exact) off both values and packs them.
+__device__ __forceinline__ uint32_t cut_plane(float2& x) {
+    const uint32_t hx = __float_as_uint(x.x) & 0xffff0000u, hy = __float_as_uint(x.y) & 0xffff0000u;
+    x = __fadd2_rn(x, make_float2(-__uint_as_float(hx), -__uint_as_float(hy)));
+    return __byte_perm(hx, hy, 0x7632);
+}
+
 // The three bfloat16 planes of the decayed, transposed C' for the 32 channels j0 .. of the warp and
-// the 64 tokens s0 .., as TMEM fragments: plane[lanes 0-15, 16-31][two registers per 8 tokens].
-// weights points at the weight of token s0.
+// the 32 tokens s0 .., as TMEM fragments: plane[lanes 0-15, 16-31][two registers per 8 tokens].
+// weights points at the weight of token s0.  An infinite product leaves NaN in the later planes.
 struct Planes {
-    uint32_t p[3][2][16];
+    uint32_t p[3][2][8];
 };
 __device__ __forceinline__ void decayed_planes(uint32_t tile, int j0, int s0, const float* weights, float factor,
                                                Planes& o) {
@@ -123,33 +144,28 @@ __device__ __forceinline__ void decayed_planes(uint32_t tile, int j0, int s0, co
                           (((((j0 & 63) >> 3) + (lane >> 3)) ^ rr) << 4);
     const float* wp = weights + 2 * (lane & 3);
 #pragma unroll
-    for (int blk = 0; blk < 8; blk++) {
+    for (int blk = 0; blk < 4; blk++) {
         uint32_t m[4];
         ldmatrix_x4_trans(addr + blk * 1024, m[0], m[1], m[2], m[3]);
-        float2 wt = *reinterpret_cast<const float2*>(wp + blk * 8);
-        wt.x *= factor;
-        wt.y *= factor;
+        const float2 wt = __fmul2_rn(*reinterpret_cast<const float2*>(wp + blk * 8), make_float2(factor, factor));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float x = bf16_lo(m[i]) * wt.x, y = bf16_hi(m[i]) * wt.y;
+            float2 x = __fmul2_rn(make_float2(bf16_lo(m[i]), bf16_hi(m[i])), wt);
             const int at = 2 * blk + (i & 1);
-            const uint32_t h = pack_bf16(x, y);
-            o.p[0][i >> 1][at] = h;
-            x -= bf16_lo(h);
-            y -= bf16_hi(h);
-            const uint32_t l = pack_bf16(x, y);
-            o.p[1][i >> 1][at] = l;
-            o.p[2][i >> 1][at] = pack_bf16(x - bf16_lo(l), y - bf16_hi(l));
+            o.p[0][i >> 1][at] = cut_plane(x);
+            o.p[1][i >> 1][at] = cut_plane(x);
+            o.p[2][i >> 1][at] = pack_bf16(x.x, x.y);
         }
     }
 }
-__device__ __forceinline__ void store_plane(uint32_t addr, const uint32_t (&p)[2][16]) {
-    tmem_st_16x128b_x8(addr, p[0]);
-    tmem_st_16x128b_x8(addr + (16u << 16), p[1]);
+__device__ __forceinline__ void store_plane(uint32_t addr, const uint32_t (&p)[2][8]) {
+    tmem_st_16x128b_x4(addr, p[0]);
+    tmem_st_16x128b_x4(addr + (16u << 16), p[1]);
 }
 
 // zeros into rows [n, 128) of `panels` panels of a stage
 __device__ __forceinline__ void zero_rows(unsigned char* st, int panels, int n, int tid) {
+#pragma unroll 1
     for (int i = tid; i < panels * (kT - n) * 8; i += kCompute) {
         const int piece = i % 8, rw = n + (i / 8) % (kT - n), pn = i / 8 / (kT - n);
         *reinterpret_cast<uint4*>(st + pn * kPanel + rw * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
@@ -157,28 +173,112 @@ __device__ __forceinline__ void zero_rows(unsigned char* st, int panels, int n, 
     fence_proxy_async_smem();
 }
 
-// What a CTA works on.
-struct Work {
-    int ri, h, b, slot, seg, row_len, ntok, tok0, nchunk;
+// A row: role fastest (the roles of one head read the same tensors), then head, batch row and
+// segment; `slot` is the segment's place in the order of walking.
+struct Row {
+    int ri, h, b, seg, slot, row_len, ntok, tok0, nchunk;
     int64_t bh;
 };
-__device__ __forceinline__ Work locate(const LaParams& p) {
-    Work k;
-    // the roles of one (batch row, head) run side by side: they read the same tensors
-    int64_t id = blockIdx.x;
-    k.ri = (int)(id % p.nroles);
+__device__ __forceinline__ Row locate(const LaParams& p, int id) {
+    Row k;
+    k.ri = id % p.nroles;
     id /= p.nroles;
-    k.h = (int)(id % p.heads);
+    k.h = id % p.heads;
     id /= p.heads;
-    k.b = (int)(id % p.batch);
-    k.slot = (int)(id / p.batch);
-    k.seg = p.role[k.ri].reverse ? p.nseg - 1 - k.slot : k.slot;
+    k.b = id % p.batch;
+    k.seg = id / p.batch;
+    k.slot = p.role[k.ri].reverse ? p.nseg - 1 - k.seg : k.seg;
     k.bh = (int64_t)k.b * p.heads + k.h;
     k.row_len = la_row_length(p, k.b);
     k.ntok = la_segment_tokens(p, k.row_len, k.seg);
     k.tok0 = k.seg * p.seglen;
     k.nchunk = (k.ntok + kT - 1) / kT;
     return k;
+}
+
+// One warp finds the range of this CTA: every row counts its chunks, at least one.
+__device__ __forceinline__ Range find_range(const LaParams& p) {
+    if (!p.split) {
+        const int id = blockIdx.x;
+        return Range{id, id, 0, 1 << 30};
+    }
+    const int lane = threadIdx.x & 31;
+    const int pairs = p.nseg * p.batch, per = p.heads * p.nroles;   // rows of one (segment, batch row)
+    auto units = [&](int i) {
+        const int n = la_segment_tokens(p, la_row_length(p, i % p.batch), i / p.batch);
+        return max(1, (n + kT - 1) / kT);
+    };
+    int64_t total = 0;
+    for (int i = lane; i < pairs; i += 32) total += (int64_t)units(i) * per;
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
+    const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x - 1;
+    Range r{0, 0, 0, 0};
+    int64_t base = 0;
+    for (int i0 = 0; i0 < pairs; i0 += 32) {
+        const int i = i0 + lane;
+        const int u = i < pairs ? units(i) : 1;
+        const int64_t mine = i < pairs ? (int64_t)u * per : 0;
+        int64_t end = mine;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, end, m);
+            if (lane >= m) end += o;
+        }
+        const int64_t at = base + end - mine;
+        const bool a = u0 >= at && u0 < at + mine, z = u1 >= at && u1 < at + mine;
+        const unsigned ma = __ballot_sync(0xffffffffu, a), mz = __ballot_sync(0xffffffffu, z);
+        const int ra = i * per + (int)((u0 - at) / u), ca = (int)((u0 - at) % u);
+        const int rz = i * per + (int)((u1 - at) / u), cz = (int)((u1 - at) % u) + 1;
+        if (ma) {
+            r.row0 = __shfl_sync(0xffffffffu, ra, __ffs(ma) - 1);
+            r.c0 = __shfl_sync(0xffffffffu, ca, __ffs(ma) - 1);
+        }
+        if (mz) {
+            r.row1 = __shfl_sync(0xffffffffu, rz, __ffs(mz) - 1);
+            r.c1 = __shfl_sync(0xffffffffu, cz, __ffs(mz) - 1);
+        }
+        base += __shfl_sync(0xffffffffu, end, 31);
+    }
+    return r;
+}
+
+// The rows of a range in the order of work: the last (which the next CTA may wait for), those
+// between, the first.
+struct Items {
+    const LaParams& p;
+    Range r;
+    __device__ __forceinline__ int count() const { return r.row1 - r.row0 + 1; }
+    __device__ __forceinline__ Row row(int i, int& c0, int& c1) const {
+        const int n = count();
+        const int id = i == 0 ? r.row1 : i == n - 1 ? r.row0 : r.row0 + i;
+        const Row k = locate(p, id);
+        c0 = id == r.row0 ? min(r.c0, k.nchunk) : 0;
+        c1 = id == r.row1 ? min(r.c1, k.nchunk) : k.nchunk;
+        return k;
+    }
+};
+
+// first token of the chunk of step c, and its tokens
+__device__ __forceinline__ int chunk_first(const Row& k, int reverse, int c) {
+    return k.tok0 + (reverse ? k.nchunk - 1 - c : c) * kT;
+}
+__device__ __forceinline__ int chunk_count(const Row& k, int reverse, int c) {
+    return min(kT, k.tok0 + k.ntok - chunk_first(k, reverse, c));
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&v)[N]) {
+    static_assert(N == 16 || N == 32);
+    if constexpr (N == 16) tmem_ld16(addr, v);
+    else tmem_ld32(addr, v);
+    tmem_wait_ld();
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[N]) {
+    if constexpr (N == 16) tmem_st16(addr, v);
+    else tmem_st32(addr, v);
+    tmem_wait_st();
 }
 
 template <int KB, int KC>
@@ -190,124 +290,146 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
     Decays& dec = *reinterpret_cast<Decays*>(smem + L::OFF_W);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
+    Range* range_slot = reinterpret_cast<Range*>(smem + L::OFF_MISC + 16);
     const Waiter wait{bars, abort, p.err};
-
-    const Work k = locate(p);
-    const LaRole& r = p.role[k.ri];
-    const int reverse = r.reverse, nchunk = k.nchunk;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float g2 = la_log2_decay(p.log_decay[k.h]);
-    const bool tma_out = !r.out_f32 && r.out_vec;
-    // chunk of step c, its first token and its tokens
-    auto first = [&](int c) { return k.tok0 + (reverse ? nchunk - 1 - c : c) * kT; };
-    auto count = [&](int c) { return min(kT, k.tok0 + k.ntok - first(c)); };
 
     if ((smem_u32(smem) & 1023u) != 0) {
         if (tid == 0) *p.err = kDevErrSmemAlign;
         return;
     }
-    if (warp == 8) tmem_alloc(tmem_slot, kTmemCols);
-    if (tid == 0) {
+    if (warp == kWarps) tmem_alloc(tmem_slot, kTmemCols);
+    if (warp == 0) {
+        const Range r = find_range(p);
+        if (lane == 0) *range_slot = r;
+    }
+    if (tid == 32) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bars + kFull + i, 1);
-            mbar_init(bars + kStaged + i, 8);
+            mbar_init(bars + kStaged + i, kWarps);
+            mbar_init(bars + kFree + i, 1);
         }
         for (int i : {kScores, kAS, kUpd, kPC, kDrain}) mbar_init(bars + i, 1);
-        for (int i : {kSReady, kCReady, kPReady, kFixed}) mbar_init(bars + i, 8);
+        for (int i : {kSReady, kCReady, kPReady, kFixed, kItem}) mbar_init(bars + i, kWarps);
         *abort = 0;
         fence_mbar_init();
     }
-    fill_decays(dec, g2, r.alpha, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const Items items{p, *range_slot};
+    const int nitems = items.count();
 
-    if (warp >= 8) {
+    if (warp >= kWarps) {
         regs_release<kRegsControl>();
-        if (warp == 9 && lane == 0) {
-            // ---- copies -------------------------------------------------------------------------
-            auto load = [&](int c) {
-                unsigned char* st = smem + (c & 1) * L::STAGE;
-                uint64_t* bar = bars + kFull + (c & 1);
-                const int t = first(c);
-                mbar_arrive_expect_tx(bar, L::STAGE);
+        if (warp == kWarps + 1 && elect_one()) {
+            // ---- loads --------------------------------------------------------------------------
+            int it = 0;
+            bool fine = true;
+            for (int n = 0; n < nitems && fine; n++) {
+                int c0, c1;
+                const Row k = items.row(n, c0, c1);
+                const LaRole& r = p.role[k.ri];
+                const int ha = k.h / r.a.share, hb = k.h / r.b.share, hc = k.h / r.c.share;
+                for (int c = c0; c < c1; c++, it++) {
+                    if (it >= 2 && !(fine = wait(kFree + (it & 1), ((it >> 1) - 1) & 1))) break;
+                    unsigned char* st = smem + (it & 1) * L::STAGE;
+                    uint64_t* bar = bars + kFull + (it & 1);
+                    const int t = chunk_first(k, r.reverse, c);
+                    mbar_arrive_expect_tx(bar, L::STAGE);
 #pragma unroll
-                for (int i = 0; i < KB / 64; i++) {
-                    tma_load_4d(st + i * kPanel, &maps.a[k.ri], bar, i * 64, t, k.h / r.a.share, k.b);
-                    tma_load_4d(st + L::A + i * kPanel, &maps.b[k.ri], bar, i * 64, t, k.h / r.b.share, k.b);
-                }
-#pragma unroll
-                for (int i = 0; i < KC / 64; i++)
-                    tma_load_4d(st + 2 * L::A + i * kPanel, &maps.c[k.ri], bar, i * 64, t, k.h / r.c.share, k.b);
-            };
-            int issued = 0;
-            for (; issued < 2 && issued < nchunk; issued++) load(issued);
-            for (int c = 0; c < nchunk; c++) {
-                // the chunk's output is staged over its a (and b) tile, and nobody uses its stage any more
-                if (!wait(kStaged + (c & 1), (c >> 1) & 1)) break;
-                if (tma_out) {
+                    for (int i = 0; i < KB / 64; i++) {
+                        tma_load_4d(st + i * kPanel, &maps.a[k.ri], bar, i * 64, t, ha, k.b);
+                        tma_load_4d(st + L::A + i * kPanel, &maps.b[k.ri], bar, i * 64, t, hb, k.b);
+                    }
 #pragma unroll
                     for (int i = 0; i < KC / 64; i++)
-                        if (i * 64 < r.dc)
-                            tma_store_4d(&maps.o[k.ri], smem + (c & 1) * L::STAGE + i * kPanel, i * 64, first(c), k.h, k.b);
-                    tma_store_commit();
-                    tma_store_wait_read_all();
+                        tma_load_4d(st + 2 * L::A + i * kPanel, &maps.c[k.ri], bar, i * 64, t, hc, k.b);
                 }
-                if (issued < nchunk) load(issued++);
+            }
+            if (!fine)       // copies in flight still write to this CTA's shared memory
+                for (int i = max(0, it - 2); i < it; i++) mbar_wait_bounded(bars + kFull + (i & 1), (i >> 1) & 1);
+        } else if (warp == kWarps + 2 && elect_one()) {
+            // ---- stores -------------------------------------------------------------------------
+            int it = 0;
+            bool fine = true;
+            for (int n = 0; n < nitems && fine; n++) {
+                int c0, c1;
+                const Row k = items.row(n, c0, c1);
+                const LaRole& r = p.role[k.ri];
+                for (int c = c0; c < c1; c++, it++) {
+                    // the chunk's output is staged over its a (and b) tile, and nobody uses its stage any more
+                    if (!(fine = wait(kStaged + (it & 1), (it >> 1) & 1))) break;
+                    if (!r.out_f32 && r.out_vec) {
+                        const int t = chunk_first(k, r.reverse, c);
+#pragma unroll
+                        for (int i = 0; i < KC / 64; i++)
+                            if (i * 64 < r.dc)
+                                tma_store_4d(&maps.o[k.ri], smem + (it & 1) * L::STAGE + i * kPanel, i * 64, t, k.h, k.b);
+                        tma_store_commit();
+                        tma_store_wait_read_all();
+                    }
+                    mbar_arrive(bars + kFree + (it & 1));
+                }
             }
             tma_store_wait_all();
-            if (*abort)      // copies in flight still write to this CTA's shared memory
-                for (int c = max(0, issued - 2); c < issued; c++) mbar_wait_bounded(bars + kFull + (c & 1), (c >> 1) & 1);
-        } else if (warp == 8 && elect_one()) {
+        } else if (warp == kWarps && elect_one()) {
             // ---- products -----------------------------------------------------------------------
             constexpr uint32_t id_scores = umma_idesc(128, 128, false), id_as = umma_idesc(128, KC, false),
                                id_pc = umma_idesc(128, KC, true), id_upd = umma_idesc(128, KB, true);
             const uint32_t s_desc = umma_desc_lo(smem_u32(smem + L::OFF_S), 16);
-            for (int c = 0; c < nchunk; c++) {
-                const uint32_t st = smem_u32(smem + (c & 1) * L::STAGE), par = c & 1;
-                if (!wait(kFull + (c & 1), (c >> 1) & 1)) break;
-                if (count(c) < kT && !wait(kFixed, 0)) break;
-                // P and the third plane of the previous chunk are still read until these two
-                if (c > 0 && !(wait(kPC, par ^ 1) && wait(kUpd, par ^ 1))) break;
-                tc_fence_after();
-                // K-major panels of 64 channels: 16 channels are 32 bytes
-                const uint32_t a_desc = umma_desc_lo(st, 16), b_desc = umma_desc_lo(st + L::A, 16);
+            int it = 0, fixed = 0;
+            bool fine = true;
+            for (int n = 0; n < nitems && fine; n++) {
+                int c0, c1;
+                const Row k = items.row(n, c0, c1);
+                const int reverse = p.role[k.ri].reverse;
+                for (int c = c0; c < c1; c++, it++) {
+                    const uint32_t st = smem_u32(smem + (it & 1) * L::STAGE), par = it & 1;
+                    if (!(fine = wait(kFull + (it & 1), (it >> 1) & 1))) break;
+                    if (chunk_count(k, reverse, c) < kT && !(fine = wait(kFixed, fixed++ & 1))) break;
+                    // P and the third plane of the previous chunk are still read until these two
+                    if (it > 0 && !(fine = wait(kPC, par ^ 1) && wait(kUpd, par ^ 1))) break;
+                    tc_fence_after();
+                    // K-major panels of 64 channels: 16 channels are 32 bytes
+                    const uint32_t a_desc = umma_desc_lo(st, 16), b_desc = umma_desc_lo(st + L::A, 16);
 #pragma unroll
-                for (int i = 0; i < KB / 16; i++) {
-                    const uint32_t off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
-                    umma_ss(tmem + kColScores, a_desc + off, b_desc + off, id_scores, i > 0);
+                    for (int i = 0; i < KB / 16; i++) {
+                        const uint32_t off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
+                        umma_ss(tmem + kColScores, a_desc + off, b_desc + off, id_scores, i > 0);
+                    }
+                    umma_commit(bars + kScores);
+                    if (!(fine = wait(kSReady, par))) break;
+                    if (it > 0 && !(fine = wait(kStaged + (par ^ 1), ((it - 1) >> 1) & 1))) break;   // O has been read
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < KB / 16; i++)
+                        umma_ss(tmem + kColO, a_desc + (((i >> 2) * kPanel + (i & 3) * 32) >> 4),
+                                s_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, i > 0);
+                    umma_commit(bars + kAS);
+                    if (!(fine = wait(kCReady, par))) break;
+                    tc_fence_after();
+                    // N-major panels of 64 channels: 16 tokens are 2048 bytes
+                    const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
+#pragma unroll
+                    for (int i = 0; i < 2 * kT / 16; i++)      // second plane, then first
+                        umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, i > 0);
+                    if (!(fine = wait(kPReady, par))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < kT / 16; i++)
+                        umma_ts(tmem + kColU, tmem + kColScores + (i >> 1) * 32 + 16 + (i & 1) * 8,
+                                bn_desc + i * (2048 >> 4), id_upd, true);
+                    umma_commit(bars + kUpd);
+#pragma unroll
+                    for (int i = 0; i < kT / 16; i++)
+                        umma_ts(tmem + kColO, tmem + kColScores + (i >> 1) * 32 + (i & 1) * 8, cn_desc + i * (2048 >> 4),
+                                id_pc, i > 0);
+                    umma_commit(bars + kPC);
                 }
-                umma_commit(bars + kScores);
-                if (!wait(kSReady, par)) break;
-                if (c > 0 && !wait(kStaged + (par ^ 1), ((c - 1) >> 1) & 1)) break;   // O has been read
-                tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < KB / 16; i++)
-                    umma_ss(tmem + kColO, a_desc + (((i >> 2) * kPanel + (i & 3) * 32) >> 4),
-                            s_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, i > 0);
-                umma_commit(bars + kAS);
-                if (!wait(kCReady, par)) break;
-                tc_fence_after();
-                // N-major panels of 64 channels: 16 tokens are 2048 bytes
-                const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
-#pragma unroll
-                for (int i = 0; i < 2 * kT / 16; i++)      // second plane, then first
-                    umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, i > 0);
-                if (!wait(kPReady, par)) break;
-                tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < kT / 16; i++)
-                    umma_ts(tmem + kColU, tmem + kColScores + (i >> 2) * 64 + 32 + (i & 3) * 8,
-                            bn_desc + i * (2048 >> 4), id_upd, 1);
-                umma_commit(bars + kUpd);
-#pragma unroll
-                for (int i = 0; i < kT / 16; i++)
-                    umma_ts(tmem + kColO, tmem + kColScores + (i >> 2) * 64 + (i & 3) * 8, cn_desc + i * (2048 >> 4),
-                            id_pc, i > 0);
-                umma_commit(bars + kPC);
             }
-            if (*abort) {
+            if (!fine) {
                 umma_commit(bars + kDrain);
                 mbar_wait_bounded(bars + kDrain, 0);
             }
@@ -316,250 +438,282 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
     } else {
         // ---- the work between products ----------------------------------------------------------
         regs_claim<kRegsCompute>();
-        const int q = warp & 3, half = warp >> 2;     // TMEM lanes 32 q .. + 32; half of the columns
+        const int q = warp & 3, part = warp >> 2;     // TMEM lanes 32 q .. + 32; quarter of the columns
         const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16);
         const int row = q * 32 + lane;                // token of P and O, channel of c (row j of S^T)
-        constexpr int NS = KB / 2;                    // columns of S^T per thread
-        constexpr int NO = KC / 2;                    // columns of O per thread
+        constexpr int NS = KB / 4;                    // columns of S^T per thread
+        constexpr int NO = KC / 4;                    // columns of O per thread
         const bool s_on = q * 32 < KC;                // S^T has KC rows
-        const int i0 = half * NS, o0 = half * NO;
+        const int i0 = part * NS, o0 = part * NO;
         auto arrive = [&](int bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + bar);
         };
         auto ok = [&](bool v) { return __all_sync(0xffffffffu, v); };
-
-        // S^T of the first chunk: the initial state, then the segments before this one.  Through TMEM,
-        // so that the loop over columns stays a loop (registers have no index).
-        float s[NS];
-        if (s_on) {
-            const float* src0 = r.state0 && row < r.dc ? r.state0 + k.bh * r.db * r.dc + row * r.s_j : nullptr;
-            const float* src = r.seg + k.bh * p.nseg * r.db * r.dc + row;
-#pragma unroll 1
-            for (int i = 0; i < NS; i += 8) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = src0 && i0 + i + e < r.db ? src0[(i0 + i + e) * r.s_i] : 0.f;
-#pragma unroll 1
-                for (int g = 0; g < k.slot; g++) {
-                    const int sg = reverse ? p.nseg - 1 - g : g;
-                    const float f = exp2f(g2 * (float)la_segment_tokens(p, k.row_len, sg));
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        x[e] = fmaf(f, x[e], row < r.dc && i0 + i + e < r.db ? src[(sg * r.db + i0 + i + e) * r.dc] : 0.f);
-                }
-                uint32_t v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = __float_as_uint(x[e]);
-                tmem_st8(tm + kColU + i0 + i, v);
-            }
-            tmem_wait_st();
-#pragma unroll
-            for (int i = 0; i < NS; i++) s[i] = 0.f;
-        }
-        // bfloat16(S^T) to shared memory for A S
-        auto put_state = [&]() {
-            if (s_on) {
-#pragma unroll
-                for (int i = 0; i < NS; i += 8) {
-                    const uint4 v = make_uint4(pack_bf16(s[i], s[i + 1]), pack_bf16(s[i + 2], s[i + 3]),
-                                               pack_bf16(s[i + 4], s[i + 5]), pack_bf16(s[i + 6], s[i + 7]));
-                    const int ii = i0 + i;
-                    *reinterpret_cast<uint4*>(smem + L::OFF_S + (ii >> 6) * (KC * 128) + swz128(row, (ii & 63) * 2)) = v;
-                }
-            }
-            fence_proxy_async_smem();
-            arrive(kSReady);
+        int it = 0, fixed = 0, meets = 0;
+        // every compute warp has come this far
+        auto meet = [&]() {
+            arrive(kItem);
+            return ok(wait(kItem, meets++ & 1));
         };
-        auto add_update = [&](int n) {
-            if (!s_on) return;
-            const float fn = dec.pow[n];
-#pragma unroll
-            for (int i = 0; i < NS; i += 32) {
-                uint32_t v[32];
-                tmem_ld32(tm + kColU + i0 + i, v);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; e++) s[i + e] = fmaf(fn, s[i + e], __uint_as_float(v[e]));
-            }
-        };
-        add_update(0);
-        if (nchunk > 0) {
-            tc_fence_before();
-            put_state();
-        }
-
         bool fine = true;
-        for (int c = 0; c < nchunk; c++) {
-            const uint32_t par = c & 1;
-            const int n = count(c);
-            unsigned char* st = smem + (c & 1) * L::STAGE;
-            if (!(fine = ok(wait(kFull + (c & 1), (c >> 1) & 1)))) break;
-            if (n < kT) {
-                // rows past the length hold whatever the caller's padding holds
-                zero_rows(st, L::STAGE / kPanel, n, tid);
-                arrive(kFixed);
-                if (!(fine = ok(wait(kFixed, 0)))) break;
-            }
-            // planes of C'^T for this half's 64 tokens; the third waits for its columns
-            Planes pl;
-            if (s_on) {
-                decayed_planes(smem_u32(st + 2 * L::A), q * 32, half * 64, (n < kT ? dec.part : dec.full) + half * 64,
-                               1.f, pl);
-                store_plane(tm + kColC + half * 32, pl.p[1]);
-                store_plane(tm + kColC + 64 + half * 32, pl.p[0]);
-                tmem_wait_st();
-            }
-            tc_fence_before();
-            arrive(kCReady);
 
-            // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
-            if (!(fine = ok(wait(kScores, par)))) break;
-            tc_fence_after();
+        for (int item = 0; item < nitems; item++) {
+            int c0, c1;
+            const Row k = items.row(item, c0, c1);
+            const LaRole& r = p.role[k.ri];
+            const int reverse = r.reverse;
+            const float g2 = la_log2_decay(p.log_decay[k.h]);
+            if (!(fine = meet())) break;              // nobody reads the last row's tables any more
+            fill_decays(dec, g2, r.alpha, r.sigma, reverse, k.nchunk > 0 ? k.ntok - (k.nchunk - 1) * kT : 0);
+
+            // S^T before chunk c0: the state that the CTA before this one has published, or the initial state
+            // and then the segments before this one.  Through TMEM, so that the loop over columns stays a
+            // loop (registers have no index).
+            if (c0 > 0) {
+                const int* flag = p.flags + blockIdx.x;
+                int there = 0;
+                const long long start = clock64();
+                while (true) {
+                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(flag) : "memory");
+                    if (there || wait.gone(start)) break;
+                }
+                if (!(fine = ok(there != 0))) break;
+            }
+            float s[NS];
+            if (s_on) {
+                const float* src0 = nullptr;
+                int64_t step = r.s_i;
+                if (c0 > 0) {
+                    src0 = p.handoff + (int64_t)blockIdx.x * KB * KC + row;
+                    step = KC;
+                } else if (r.state0 && row < r.dc) {
+                    src0 = r.state0 + k.bh * r.db * r.dc + row * r.s_j;
+                }
+                const int cols = c0 > 0 ? KB : r.db, folds = c0 > 0 ? 0 : k.slot;
+                const float* src = r.seg + k.bh * p.nseg * r.db * r.dc + row;
 #pragma unroll 1
-            for (int blk = 0; blk < 2; blk++) {
-                const int sb = half * 2 + blk;
-                uint32_t o[16];
-                if (reverse ? sb >= q : sb <= q) {
-                    uint32_t v[32];
-                    tmem_ld32(tm + kColScores + sb * 32, v);
-                    tmem_wait_ld();
-                    const int d0 = reverse ? sb * 32 - row : row - sb * 32;   // distance to the block's first column
-                    const float* wt = dec.score + d0;
-                    if (reverse) {
+                for (int i = 0; i < NS; i += 8) {
+                    float x[8];
 #pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            o[e] = pack_bf16(d0 + 2 * e >= 0 ? __uint_as_float(v[2 * e]) * wt[2 * e] : 0.f,
-                                             d0 + 2 * e + 1 >= 0 ? __uint_as_float(v[2 * e + 1]) * wt[2 * e + 1] : 0.f);
+                    for (int e = 0; e < 8; e++) x[e] = src0 && i0 + i + e < cols ? __ldcg(src0 + (i0 + i + e) * step) : 0.f;
+#pragma unroll 1
+                    for (int g = 0; g < folds; g++) {
+                        const int sg = reverse ? p.nseg - 1 - g : g;
+                        const float f = exp2f(g2 * (float)la_segment_tokens(p, k.row_len, sg));
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            x[e] = fmaf(f, x[e], row < r.dc && i0 + i + e < r.db ? src[(sg * r.db + i0 + i + e) * r.dc] : 0.f);
+                    }
+                    uint32_t v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = __float_as_uint(x[e]);
+                    tmem_st8(tm + kColU + i0 + i, v);
+                }
+                tmem_wait_st();
+                uint32_t v[NS];
+                tmem_ld<NS>(tm + kColU + i0, v);
+#pragma unroll
+                for (int e = 0; e < NS; e++) s[e] = __uint_as_float(v[e]);
+            }
+            // bfloat16(S^T) to shared memory for A S
+            auto put_state = [&]() {
+                if (s_on) {
+#pragma unroll
+                    for (int i = 0; i < NS; i += 8) {
+                        const uint4 v = make_uint4(pack_bf16(s[i], s[i + 1]), pack_bf16(s[i + 2], s[i + 3]),
+                                                   pack_bf16(s[i + 4], s[i + 5]), pack_bf16(s[i + 6], s[i + 7]));
+                        const int ii = i0 + i;
+                        *reinterpret_cast<uint4*>(smem + L::OFF_S + (ii >> 6) * (KC * 128) + swz128(row, (ii & 63) * 2)) = v;
+                    }
+                }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                arrive(kSReady);
+            };
+            if (c0 < c1) put_state();
+            if (!(fine = meet())) break;              // the tables are there
+
+            for (int c = c0; c < c1; c++, it++) {
+                const uint32_t par = it & 1;
+                const int n = chunk_count(k, reverse, c);
+                unsigned char* st = smem + (it & 1) * L::STAGE;
+                if (!(fine = ok(wait(kFull + (it & 1), (it >> 1) & 1)))) break;
+                if (n < kT) {
+                    // rows past the length hold whatever the caller's padding holds
+                    zero_rows(st, L::STAGE / kPanel, n, tid);
+                    arrive(kFixed);
+                    if (!(fine = ok(wait(kFixed, fixed++ & 1)))) break;
+                }
+                // planes of C'^T for this quarter's 32 tokens; the third waits for its columns
+                Planes pl;
+                if (s_on) {
+                    decayed_planes(smem_u32(st + 2 * L::A), q * 32, part * 32, (n < kT ? dec.part : dec.full) + part * 32,
+                                   1.f, pl);
+                    store_plane(tm + kColC + part * 16, pl.p[1]);
+                    store_plane(tm + kColC + 64 + part * 16, pl.p[0]);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                arrive(kCReady);
+
+                // P: this warp's 32 x 32 block, which the mask empties, halves or leaves whole
+                if (!(fine = ok(wait(kScores, par)))) break;
+                tc_fence_after();
+                {
+                    uint32_t o[16];
+                    if (reverse ? part >= q : part <= q) {
+                        uint32_t v[32];
+                        tmem_ld<32>(tm + kColScores + part * 32, v);
+                        const int d0 = reverse ? part * 32 - row : row - part * 32;   // distance to the block's first column
+                        const float* wt = dec.score + d0;
+                        if (reverse) {
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                o[e] = pack_bf16(d0 + 2 * e >= 0 ? __uint_as_float(v[2 * e]) * wt[2 * e] : 0.f,
+                                                 d0 + 2 * e + 1 >= 0 ? __uint_as_float(v[2 * e + 1]) * wt[2 * e + 1] : 0.f);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                o[e] = pack_bf16(d0 >= 2 * e ? __uint_as_float(v[2 * e]) * wt[-2 * e] : 0.f,
+                                                 d0 >= 2 * e + 1 ? __uint_as_float(v[2 * e + 1]) * wt[-2 * e - 1] : 0.f);
+                        }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            o[e] = pack_bf16(d0 >= 2 * e ? __uint_as_float(v[2 * e]) * wt[-2 * e] : 0.f,
-                                             d0 >= 2 * e + 1 ? __uint_as_float(v[2 * e + 1]) * wt[-2 * e - 1] : 0.f);
+                        for (int e = 0; e < 16; e++) o[e] = 0;
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[e] = 0;
+                    // over scores that this thread alone reads, and has read
+                    tmem_st16(tm + kColScores + part * 32, o);
+                    if (s_on) store_plane(tm + kColScores + part * 32 + 16, pl.p[2]);
                 }
-                // over scores that this thread has read: 16 of the half's first 32 columns per block
-                tmem_st16(tm + kColScores + half * 64 + blk * 16, o);
-            }
-            // every warp of this half that shares the lanes is this warp: its scores are read
-            if (s_on) store_plane(tm + kColScores + half * 64 + 32, pl.p[2]);
-            // A S leaves TMEM, scaled per row
-            if (!(fine = ok(wait(kAS, par)))) break;
-            tc_fence_after();
-            float acc[NO];
-            {
-                const float f = r.beta * dec.pow[reverse ? max(n - 1 - row, 0) : row + 1];
+                // A S leaves TMEM, scaled per row
+                if (!(fine = ok(wait(kAS, par)))) break;
+                tc_fence_after();
+                float acc[NO];
+                {
+                    const float f = r.beta * dec.pow[reverse ? max(n - 1 - row, 0) : row + 1];
+                    uint32_t v[NO];
+                    tmem_ld<NO>(tm + kColO + o0, v);
 #pragma unroll
-                for (int i = 0; i < NO; i += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(tm + kColO + o0 + i, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; e++) acc[i + e] = __uint_as_float(v[e]) * f;
-                }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            arrive(kPReady);
-
-            // the state after this chunk; the stage's b is also free after the update
-            if (!(fine = ok(wait(kUpd, par)))) break;
-            tc_fence_after();
-            add_update(n);
-            if (c + 1 < nchunk) {
-                tc_fence_before();
-                put_state();
-            }
-
-            // O
-            if (!(fine = ok(wait(kPC, par)))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < NO; i += 32) {
-                uint32_t v[32];
-                tmem_ld32(tm + kColO + o0 + i, v);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; e++) acc[i + e] = row < n ? acc[i + e] + __uint_as_float(v[e]) : 0.f;
-            }
-            if (tma_out) {
-#pragma unroll
-                for (int i = 0; i < NO; i += 8) {
-                    const uint4 v = make_uint4(pack_bf16(acc[i], acc[i + 1]), pack_bf16(acc[i + 2], acc[i + 3]),
-                                               pack_bf16(acc[i + 4], acc[i + 5]), pack_bf16(acc[i + 6], acc[i + 7]));
-                    const int oc = o0 + i;
-                    *reinterpret_cast<uint4*>(st + (oc >> 6) * kPanel + swz128(row, (oc & 63) * 2)) = v;
-                }
-                fence_proxy_async_smem();
-            } else {
-                // float32 partials and rows a TMA cannot store: through the warp's own piece of the stage,
-                // 16-byte pieces swizzled by the row, then row by row
-                float* own = reinterpret_cast<float*>(st) + warp * 32 * NO;
-#pragma unroll
-                for (int i = 0; i < NO; i += 4)
-                    *reinterpret_cast<float4*>(own + lane * NO + (((i >> 2) ^ (lane & 7)) << 2)) =
-                        make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-                __syncwarp();
-                const int64_t at = k.b * r.o_sb + (int64_t)(first(c) + q * 32) * r.o_st + k.h * r.o_sh + o0;
-                const int cols = min(NO, r.dc - o0), rows = min(32, n - q * 32);
-#pragma unroll 1
-                for (int i = lane; i < rows * NO; i += 32) {
-                    const int rw = i / NO, col = i % NO;
-                    const float x = own[rw * NO + (((col >> 2) ^ (rw & 7)) << 2) + (col & 3)];
-                    if (col >= cols) continue;
-                    if (r.out_f32) static_cast<float*>(r.out)[at + rw * r.o_st + col] = x;
-                    else static_cast<__nv_bfloat16*>(r.out)[at + rw * r.o_st + col] = __float2bfloat16_rn(x);
-                }
-                fence_proxy_async_smem();
-            }
-            tc_fence_before();
-            arrive(kStaged + (c & 1));
-        }
-
-        if (fine) {
-            if (k.slot == p.nseg - 1 && r.state_out && s_on) {
-#pragma unroll
-                for (int i = 0; i < NS; i += 32) {
-                    uint32_t v[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(s[i + e]);
-                    tmem_st32(tm + kColU + i0 + i, v);
+                    for (int e = 0; e < NO; e++) acc[e] = __uint_as_float(v[e]) * f;
                 }
                 tmem_wait_st();
-                float* dst = r.state_out + k.bh * r.db * r.dc + row * r.s_j;
-#pragma unroll 1
-                for (int i = 0; i < NS; i += 8) {
-                    uint32_t v[8];
-                    tmem_ld8(tm + kColU + i0 + i, v);
-                    tmem_wait_ld();
+                tc_fence_before();
+                arrive(kPReady);
+
+                // the state after this chunk; the stage's b is also free after the update
+                if (!(fine = ok(wait(kUpd, par)))) break;
+                tc_fence_after();
+                if (s_on) {
+                    const float fn = dec.pow[n];
+                    uint32_t v[NS];
+                    tmem_ld<NS>(tm + kColU + i0, v);
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (row < r.dc && i0 + i + e < r.db) dst[(i0 + i + e) * r.s_i] = __uint_as_float(v[e]);
+                    for (int e = 0; e < NS; e++) s[e] = fmaf(fn, s[e], __uint_as_float(v[e]));
+                }
+                if (c + 1 < c1) put_state();
+
+                // O
+                if (!(fine = ok(wait(kPC, par)))) break;
+                tc_fence_after();
+                {
+                    uint32_t v[NO];
+                    tmem_ld<NO>(tm + kColO + o0, v);
+#pragma unroll
+                    for (int e = 0; e < NO; e++) acc[e] = row < n ? acc[e] + __uint_as_float(v[e]) : 0.f;
+                }
+                if (!r.out_f32 && r.out_vec) {
+#pragma unroll
+                    for (int i = 0; i < NO; i += 8) {
+                        const uint4 v = make_uint4(pack_bf16(acc[i], acc[i + 1]), pack_bf16(acc[i + 2], acc[i + 3]),
+                                                   pack_bf16(acc[i + 4], acc[i + 5]), pack_bf16(acc[i + 6], acc[i + 7]));
+                        const int oc = o0 + i;
+                        *reinterpret_cast<uint4*>(st + (oc >> 6) * kPanel + swz128(row, (oc & 63) * 2)) = v;
+                    }
+                    fence_proxy_async_smem();
+                } else {
+                    // float32 partials and rows a TMA cannot store: through the warp's own piece of the stage,
+                    // 16-byte pieces swizzled by the row, then row by row
+                    float* own = reinterpret_cast<float*>(st) + warp * 32 * NO;
+                    constexpr int M = NO / 4 - 1;
+#pragma unroll
+                    for (int i = 0; i < NO; i += 4)
+                        *reinterpret_cast<float4*>(own + lane * NO + (((i >> 2) ^ (lane & M)) << 2)) =
+                            make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                    __syncwarp();
+                    const int64_t at = k.b * r.o_sb + (int64_t)(chunk_first(k, reverse, c) + q * 32) * r.o_st +
+                                       k.h * r.o_sh + o0;
+                    const int cols = min(NO, r.dc - o0), rows = min(32, n - q * 32);
+#pragma unroll 1
+                    for (int i = lane; i < rows * NO; i += 32) {
+                        const int rw = i / NO, col = i % NO;
+                        const float x = own[rw * NO + (((col >> 2) ^ (rw & M)) << 2) + (col & 3)];
+                        if (col >= cols) continue;
+                        if (r.out_f32) static_cast<float*>(r.out)[at + rw * r.o_st + col] = x;
+                        else static_cast<__nv_bfloat16*>(r.out)[at + rw * r.o_st + col] = __float2bfloat16_rn(x);
+                    }
+                    fence_proxy_async_smem();
+                }
+                tc_fence_before();
+                arrive(kStaged + (it & 1));
+            }
+            if (!fine) break;
+
+            // the state goes to the CTA that continues the row, or out
+            const bool ends = c1 == k.nchunk;
+            const bool out = ends && k.slot == p.nseg - 1 && r.state_out;
+            if (!ends || out) {
+                if (s_on) {
+                    uint32_t v[NS];
+#pragma unroll
+                    for (int e = 0; e < NS; e++) v[e] = __float_as_uint(s[e]);
+                    tmem_st<NS>(tm + kColU + i0, v);
+                    float* dst = ends ? r.state_out + k.bh * r.db * r.dc + row * r.s_j
+                                      : p.handoff + (int64_t)(blockIdx.x + 1) * KB * KC + row;
+                    const int64_t step = ends ? r.s_i : KC;
+                    const int rows = ends ? r.dc : KC, cols = ends ? r.db : KB;
+#pragma unroll 1
+                    for (int i = 0; i < NS; i += 8) {
+                        uint32_t u[8];
+                        tmem_ld8(tm + kColU + i0 + i, u);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (row < rows && i0 + i + e < cols) dst[(i0 + i + e) * step] = __uint_as_float(u[e]);
+                    }
+                }
+                if (!ends) {
+                    __threadfence();
+                    if (!(fine = meet())) break;
+                    if (tid == 0)
+                        asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(p.flags + blockIdx.x + 1), "r"(1)
+                                     : "memory");
                 }
             }
-            // tokens past the row's length
-            const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * KC;
-            for (int i = tid; i < total; i += kCompute) {
-                const int t = k.ntok + i / KC, cc = i % KC;
-                if (cc >= r.dc) continue;
-                const int64_t at = k.b * r.o_sb + (int64_t)(k.tok0 + t) * r.o_st + k.h * r.o_sh + cc;
-                if (r.out_f32) static_cast<float*>(r.out)[at] = 0.f;
-                else static_cast<__nv_bfloat16*>(r.out)[at] = __float2bfloat16_rn(0.f);
+            if (ends) {
+                // tokens past the row's length
+                const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * KC;
+#pragma unroll 1
+                for (int i = tid; i < total; i += kCompute) {
+                    const int t = k.ntok + i / KC, cc = i % KC;
+                    if (cc >= r.dc) continue;
+                    const int64_t at = k.b * r.o_sb + (int64_t)(k.tok0 + t) * r.o_st + k.h * r.o_sh + cc;
+                    if (r.out_f32) static_cast<float*>(r.out)[at] = 0.f;
+                    else static_cast<__nv_bfloat16*>(r.out)[at] = __float2bfloat16_rn(0.f);
+                }
             }
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tmem_dealloc(tmem, kTmemCols);
+    if (warp == kWarps) tmem_dealloc(tmem, kTmemCols);
 }
 
 // The state a segment reaches from a zero start: only U, with every token weighted towards the
-// segment's end, so that the sum needs no rescaling between chunks.  C'^T has two buffers of
-// three planes; the threads fill one while the product reads the other.
+// segment's end, so that the sum needs no rescaling between chunks, and chunks whose every weight
+// is zero in float32 are not read.  C'^T has two buffers of three planes; the threads fill one
+// while the product reads the other.
 constexpr int kStages = 3;
 template <int KB, int KC>
 struct StateSmem {
@@ -584,86 +738,93 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
     const Waiter wait{bars, abort, p.err};
 
-    const Work k = locate(p);
+    // the last segment in the order of walking feeds nobody: segments 0 .. nseg - 2, or 1 .. reversed
+    Row k = locate(p, blockIdx.x);
     const LaRole& r = p.role[k.ri];
-    const int reverse = r.reverse, nchunk = k.nchunk;
+    const int reverse = r.reverse;
+    if (reverse) k = locate(p, blockIdx.x + p.nroles * p.heads * p.batch);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float g2 = la_log2_decay(p.log_decay[k.h]);
     auto first = [&](int c) { return k.tok0 + c * kT; };
-    auto count = [&](int c) { return min(kT, k.tok0 + k.ntok - first(c)); };
+    auto count = [&](int c) { return min(kT, k.ntok - c * kT); };
+    // tokens between a chunk and the end of the walk: later ones, or earlier ones in reverse
+    auto far = [&](int c) { return reverse ? c * kT : k.ntok - c * kT - count(c); };
+    int cb = 0, ce = k.nchunk;                // chunks with a weight that is not zero
+    while (cb < ce && !reverse && g2 * (float)far(cb) < kZeroLog2) cb++;
+    while (cb < ce && reverse && g2 * (float)far(ce - 1) < kZeroLog2) ce--;
+    const int nchunk = ce - cb;
 
     if ((smem_u32(smem) & 1023u) != 0) {
         if (tid == 0) *p.err = kDevErrSmemAlign;
         return;
     }
-    if (warp == 8) tmem_alloc(tmem_slot, kTmemCols);
+    if (warp == kWarps) tmem_alloc(tmem_slot, kTmemCols);
     if (tid == 0) {
         for (int i = 0; i < kStages; i++) {
             mbar_init(bars + kSbFull + i, 1);
             mbar_init(bars + kSbFree + i, 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(bars + kSbReady + i, 8);
+            mbar_init(bars + kSbReady + i, kWarps);
             mbar_init(bars + kSbDone + i, 1);
         }
-        mbar_init(bars + kSbFixed, 8);
+        mbar_init(bars + kSbFixed, kWarps);
         mbar_init(bars + kSbDrain, 1);
         *abort = 0;
         fence_mbar_init();
     }
-    fill_decays(dec, g2, r.alpha, r.sigma, reverse, nchunk > 0 ? k.ntok - (nchunk - 1) * kT : 0);
+    fill_decays(dec, g2, r.alpha, r.sigma, reverse, k.nchunk > 0 ? k.ntok - (k.nchunk - 1) * kT : 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 9) {
-        if (lane == 0) {
-            auto load = [&](int c) {
-                unsigned char* st = smem + (c % kStages) * L::STAGE;
-                uint64_t* bar = bars + kSbFull + c % kStages;
+    if (warp == kWarps + 1) {
+        if (elect_one()) {
+            const int hb = k.h / r.b.share, hc = k.h / r.c.share;
+            bool fine = true;
+            int i = 0;
+            for (; i < nchunk; i++) {
+                if (i >= kStages && !(fine = wait(kSbFree + i % kStages, (i / kStages - 1) & 1))) break;
+                unsigned char* st = smem + (i % kStages) * L::STAGE;
+                uint64_t* bar = bars + kSbFull + i % kStages;
                 mbar_arrive_expect_tx(bar, L::STAGE);
 #pragma unroll
-                for (int i = 0; i < KB / 64; i++)
-                    tma_load_4d(st + i * kPanel, &maps.b[k.ri], bar, i * 64, first(c), k.h / r.b.share, k.b);
+                for (int n = 0; n < KB / 64; n++)
+                    tma_load_4d(st + n * kPanel, &maps.b[k.ri], bar, n * 64, first(cb + i), hb, k.b);
 #pragma unroll
-                for (int i = 0; i < KC / 64; i++)
-                    tma_load_4d(st + L::B + i * kPanel, &maps.c[k.ri], bar, i * 64, first(c), k.h / r.c.share, k.b);
-            };
-            int issued = 0;
-            for (; issued < kStages && issued < nchunk; issued++) load(issued);
-            for (int c = 0; issued < nchunk; c++) {
-                if (!wait(kSbFree + c % kStages, (c / kStages) & 1)) break;
-                load(issued++);
+                for (int n = 0; n < KC / 64; n++)
+                    tma_load_4d(st + L::B + n * kPanel, &maps.c[k.ri], bar, n * 64, first(cb + i), hc, k.b);
             }
-            if (*abort)
-                for (int c = max(0, issued - kStages); c < issued; c++)
-                    mbar_wait_bounded(bars + kSbFull + c % kStages, (c / kStages) & 1);
+            if (!fine)
+                for (int n = max(0, i - kStages); n < i; n++)
+                    mbar_wait_bounded(bars + kSbFull + n % kStages, (n / kStages) & 1);
         }
         __syncwarp();
-    } else if (warp == 8) {
+    } else if (warp == kWarps) {
         if (elect_one()) {
             constexpr uint32_t id_upd = umma_idesc(128, KB, true);
-            for (int c = 0; c < nchunk; c++) {
-                if (!wait(kSbFull + c % kStages, (c / kStages) & 1)) break;
-                if (!wait(kSbReady + (c & 1), (c >> 1) & 1)) break;
+            bool fine = true;
+            for (int i = 0; i < nchunk; i++) {
+                if (!(fine = wait(kSbFull + i % kStages, (i / kStages) & 1))) break;
+                if (!(fine = wait(kSbReady + (i & 1), (i >> 1) & 1))) break;
                 tc_fence_after();
-                const uint32_t bn_desc = umma_desc_lo(smem_u32(smem + (c % kStages) * L::STAGE), kPanel);
-                const uint32_t cp = tmem + 128 + (c & 1) * 192;
+                const uint32_t bn_desc = umma_desc_lo(smem_u32(smem + (i % kStages) * L::STAGE), kPanel);
+                const uint32_t cp = tmem + 128 + (i & 1) * 192;
 #pragma unroll
-                for (int i = 0; i < 3 * kT / 16; i++)
-                    umma_ts(tmem, cp + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, c > 0 || i > 0);
-                umma_commit(bars + kSbFree + c % kStages);
-                umma_commit(bars + kSbDone + (c & 1));
+                for (int e = 0; e < 3 * kT / 16; e++)
+                    umma_ts(tmem, cp + e * 8, bn_desc + (e & 7) * (2048 >> 4), id_upd, i > 0 || e > 0);
+                umma_commit(bars + kSbFree + i % kStages);
+                umma_commit(bars + kSbDone + (i & 1));
             }
-            if (*abort) {
+            if (!fine) {
                 umma_commit(bars + kSbDrain);
                 mbar_wait_bounded(bars + kSbDrain, 0);
             }
         }
         __syncwarp();
-    } else if (warp < 8) {
-        const int q = warp & 3, half = warp >> 2;
+    } else if (warp < kWarps) {
+        const int q = warp & 3, part = warp >> 2;
         const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16);
         const int row = q * 32 + lane;
         const bool s_on = q * 32 < KC;
@@ -673,37 +834,35 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
         };
         auto ok = [&](bool v) { return __all_sync(0xffffffffu, v); };
         bool fine = true;
-        for (int c = 0; c < nchunk; c++) {
-            const int n = count(c);
-            unsigned char* st = smem + (c % kStages) * L::STAGE;
-            if (!(fine = ok(wait(kSbFull + c % kStages, (c / kStages) & 1)))) break;
-            if (c >= 2 && !(fine = ok(wait(kSbDone + (c & 1), ((c - 2) >> 1) & 1)))) break;   // the buffer is free
+        for (int i = 0; i < nchunk; i++) {
+            const int c = cb + i, n = count(c);
+            unsigned char* st = smem + (i % kStages) * L::STAGE;
+            if (!(fine = ok(wait(kSbFull + i % kStages, (i / kStages) & 1)))) break;
+            if (i >= 2 && !(fine = ok(wait(kSbDone + (i & 1), ((i - 2) >> 1) & 1)))) break;   // the buffer is free
             if (n < kT) {
                 zero_rows(st, L::STAGE / kPanel, n, tid);
                 arrive(kSbFixed);
                 if (!(fine = ok(wait(kSbFixed, 0)))) break;
             }
             if (s_on) {
-                // tokens after this chunk (forward) or before it (reverse)
-                const int far = reverse ? c * kT : k.ntok - c * kT - n;
                 Planes pl;
-                decayed_planes(smem_u32(st + L::B), q * 32, half * 64, (n < kT ? dec.part : dec.full) + half * 64,
-                               exp2f(g2 * (float)far), pl);
-                const uint32_t cp = tm + 128 + (c & 1) * 192 + half * 32;
+                decayed_planes(smem_u32(st + L::B), q * 32, part * 32, (n < kT ? dec.part : dec.full) + part * 32,
+                               exp2f(g2 * (float)far(c)), pl);
+                const uint32_t cp = tm + 128 + (i & 1) * 192 + part * 16;
 #pragma unroll
-                for (int i = 0; i < 3; i++) store_plane(cp + i * 64, pl.p[2 - i]);   // smallest first
+                for (int e = 0; e < 3; e++) store_plane(cp + e * 64, pl.p[2 - e]);   // smallest first
                 tmem_wait_st();
             }
             tc_fence_before();
-            arrive(kSbReady + (c & 1));
+            arrive(kSbReady + (i & 1));
         }
         if (fine && nchunk > 0) fine = ok(wait(kSbDone + ((nchunk - 1) & 1), ((nchunk - 1) >> 1) & 1));
         tc_fence_after();
         if (fine && s_on) {
-            constexpr int NS = KB / 2;
+            constexpr int NS = KB / 4;
             float* e = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc;
 #pragma unroll 1
-            for (int i = half * NS; i < half * NS + NS; i += 8) {
+            for (int i = part * NS; i < part * NS + NS; i += 8) {
                 uint32_t v[8] = {};
                 if (nchunk > 0) {
                     tmem_ld8(tm + i, v);
@@ -718,15 +877,13 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tmem_dealloc(tmem, kTmemCols);
+    if (warp == kWarps) tmem_dealloc(tmem, kTmemCols);
 }
 
 template <int KB, int KC>
-cudaError_t launch_tc(const LaParams& p, const LaMaps& maps, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(linattn_tc_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         TcSmem<KB, KC>::BYTES);
-    if (e != cudaSuccess) return e;
+cudaError_t launch_tc(const LaParams& p, const LaMaps& maps, int sms, cudaStream_t stream) {
     const int64_t rows = (int64_t)p.batch * p.heads * p.nroles;
+    cudaError_t e;
     if (p.nseg > 1) {
         e = cudaFuncSetAttribute(linattn_tc_state_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  StateSmem<KB, KC>::BYTES);
@@ -734,16 +891,30 @@ cudaError_t launch_tc(const LaParams& p, const LaMaps& maps, cudaStream_t stream
         linattn_tc_state_kernel<KB, KC><<<(unsigned)(rows * (p.nseg - 1)), kThreads, StateSmem<KB, KC>::BYTES, stream>>>(p, maps);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    linattn_tc_kernel<KB, KC><<<(unsigned)(rows * p.nseg), kThreads, TcSmem<KB, KC>::BYTES, stream>>>(p, maps);
-    return cudaGetLastError();
+    e = cudaFuncSetAttribute(linattn_tc_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             TcSmem<KB, KC>::BYTES);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.split ? sms : rows * p.nseg));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = TcSmem<KB, KC>::BYTES;
+    cfg.stream = stream;
+    // a CTA may wait for the one before it: all of them are resident at once
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.split ? 1 : 0;
+    if (p.split && (e = cudaMemsetAsync(p.flags, 0, (size_t)(sms + 1) * sizeof(int), stream)) != cudaSuccess) return e;
+    return cudaLaunchKernelEx(&cfg, linattn_tc_kernel<KB, KC>, p, maps);
 }
 
 }  // namespace
 
 // Every role of p has db <= kb and dc <= kc (64 or 128).
-cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, cudaStream_t stream) {
-    if (kb == 64) return kc == 64 ? launch_tc<64, 64>(p, maps, stream) : launch_tc<64, 128>(p, maps, stream);
-    return kc == 64 ? launch_tc<128, 64>(p, maps, stream) : launch_tc<128, 128>(p, maps, stream);
+cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, int sms, cudaStream_t stream) {
+    if (kb == 64) return kc == 64 ? launch_tc<64, 64>(p, maps, sms, stream) : launch_tc<64, 128>(p, maps, sms, stream);
+    return kc == 64 ? launch_tc<128, 64>(p, maps, sms, stream) : launch_tc<128, 128>(p, maps, sms, stream);
 }
 
 }  // namespace ssm
