@@ -16,9 +16,9 @@
 // carried as a sum of three bfloat16 planes (24 bits) and U is added to the decayed state in
 // float32.
 //
-// One CTA per SM.  Warps 0-15 do the work between products, four for each quarter of the TMEM
-// lanes, each with a quarter of the columns; warp 16 issues the products, warp 17 the loads, warp
-// 18 the stores.  The order of the phases lets each run beside a product:
+// One CTA per SM.  Warps 0-7 do the work between products, two for each quarter of the TMEM
+// lanes, each with half of the columns; warp 8 issues the products, warp 9 the loads, warp 10
+// the stores.  The order of the phases lets each run beside a product:
 //     C'(c) | scores, A S;   P(c) | U;   S(c + 1) | P C;   O(c) | scores(c + 1).
 //
 // With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
@@ -39,11 +39,11 @@ namespace {
 
 constexpr int kT = 128;                    // tokens per chunk
 constexpr int kPanel = kT * 128;           // bytes of 128 rows x 64 channels
-constexpr int kWarps = 16;                 // compute warps
+constexpr int kWarps = 8;                  // compute warps
 constexpr int kCompute = kWarps * 32;
 constexpr int kThreads = kCompute + 128;   // the last warpgroup issues copies and products
-// Registers: launched with 96 each (640 * 96 = 512 * 104 + 128 * 64)
-constexpr int kRegsCompute = 104, kRegsControl = 64;
+// Registers: launched with 168 each (384 * 168 = 256 * 224 + 128 * 56)
+constexpr int kRegsCompute = 224, kRegsControl = 56;
 constexpr uint32_t kTmemCols = 512;
 // TMEM columns
 constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P then takes the first 16
@@ -51,23 +51,43 @@ constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P 
 constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
 constexpr uint32_t kColC = 384;            // 64 + 64: second and first plane of C'^T
+// Tries before a wait has run out: each lasts 30 cycles or more (a try may suspend for longer), so
+// 0.06 s or more, against the microseconds of the longest wait that ends
+constexpr int kTries = 1 << 22;
 constexpr float kZeroLog2 = -151.f;        // exp2 of anything below is zero in float32
+
+// A weight as a sum of three bfloat16 of 8 bits each.
+__device__ __forceinline__ void split_weight(float x, __nv_bfloat16& u, __nv_bfloat16& v, __nv_bfloat16& z) {
+    u = __float2bfloat16_rn(x);
+    x -= __bfloat162float(u);
+    v = __float2bfloat16_rn(x);
+    z = __float2bfloat16_rn(x - __bfloat162float(v));
+}
 
 // Decay tables in shared memory, filled once per row.
 struct Decays {
     float pow[kT + 1];                     // w^0 .. w^128
-    float score[kT];                       // alpha w^d: weights of P by distance
-    alignas(16) float full[kT];            // weights of C' for a chunk of 128 tokens
-    alignas(16) float part[kT];            // and for the row's one shorter chunk, zero past its end
+    float score[kT];                       // weights of P: alpha w^d at d, or at 127 - d (forward); up to 31
+                                           // entries before and after it are read for masked columns, unused
+    alignas(16) float block[32];           // within a whole block of P: w^(31 - column), reverse w^column
+    // weights of C' by token, split: [0] for a chunk of 128 tokens, [1] for the row's one shorter chunk
+    // (zero past its end)
+    alignas(16) __nv_bfloat16 plane[2][3][kT];
 };
 
+__device__ __forceinline__ float plane_weight(float g2, float sigma, int reverse, int i, int n) {
+    return i < n ? sigma * exp2f(g2 * (float)(reverse ? i + 1 : n - 1 - i)) : 0.f;
+}
 __device__ __forceinline__ void fill_decays(Decays& d, float g2, float alpha, float sigma, int reverse, int n_part) {
     const int i = threadIdx.x;
     if (i <= kT) d.pow[i] = exp2f(g2 * (float)i);
+    if (i < 32) d.block[i] = exp2f(g2 * (float)(reverse ? i : 31 - i));
     if (i < kT) {
-        d.score[i] = alpha * exp2f(g2 * (float)i);
-        d.full[i] = sigma * exp2f(g2 * (float)(reverse ? i + 1 : kT - 1 - i));
-        d.part[i] = i < n_part ? sigma * exp2f(g2 * (float)(reverse ? i + 1 : n_part - 1 - i)) : 0.f;
+        d.score[i] = alpha * exp2f(g2 * (float)(reverse ? i : kT - 1 - i));
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            split_weight(plane_weight(g2, sigma, reverse, i, e ? n_part : kT), d.plane[e][0][i], d.plane[e][1][i],
+                         d.plane[e][2][i]);
     }
 }
 
@@ -101,13 +121,16 @@ struct Waiter {
     int* err;
     // false once any wait of the CTA has run out
     __device__ __forceinline__ bool operator()(int bar, uint32_t parity) const {
-        if (mbar_try_wait(bars + bar, parity)) return true;
-        const long long start = clock64();
+        int tries = 0;
         while (!mbar_try_wait(bars + bar, parity))
-            if (gone(start)) return false;
+            if (*abort || ++tries == kTries) {
+                *abort = 1;
+                *err = kDevErrTmaTimeout;
+                return false;
+            }
         return true;
     }
-    // has any wait run out, this one included?
+    // has any wait run out, or this one, of a flag in global memory, begun at `start`?
     __device__ __forceinline__ bool gone(long long start) const {
         if (*abort) return true;
         if (clock64() - start <= 2000000000LL) return false;
@@ -124,37 +147,47 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// Cuts the leading bfloat16 (by truncation: what is left is exact) off both values and packs them.
-__device__ __forceinline__ uint32_t cut_plane(float2& x) {
-    const uint32_t hx = __float_as_uint(x.x) & 0xffff0000u, hy = __float_as_uint(x.y) & 0xffff0000u;
-    x = __fadd2_rn(x, make_float2(-__uint_as_float(hx), -__uint_as_float(hy)));
-    return __byte_perm(hx, hy, 0x7632);
-}
-
 // The three bfloat16 planes of the decayed, transposed C' for the 32 channels j0 .. of the warp and
 // the 32 tokens s0 .., as TMEM fragments: plane[lanes 0-15, 16-31][two registers per 8 tokens].
-// weights points at the weight of token s0.  An infinite product leaves NaN in the later planes.
+// weights(i) gives the split weights of the lane's token pair of the 8 tokens s0 + 8 i ...
+//
+// In packed bfloat16 arithmetic (the FMA pipe; splitting float32 products takes more instructions,
+// most of them on the slower ALU pipe).  The weight is u + v + z, 8 bits each, and c has 8 bits, so
+// the rounding error of a product is itself a bfloat16, which one fused multiply-add yields:
+//     c u = p0 + e,   c v = q + d,   e + q = p1 + t      all exactly (the last is Knuth's two-sum)
+// and what is left, c z + d + t, is 2^-16 of the whole and needs only p2's 8 bits.  (Without the
+// two-sum, p2 = rn(c z + rn(c v + rn(e - p1))): half the instructions and a state error of 1.7e-6
+// instead of 4e-7.)
 struct Planes {
     uint32_t p[3][2][8];
 };
-__device__ __forceinline__ void decayed_planes(uint32_t tile, int j0, int s0, const float* weights, float factor,
-                                               Planes& o) {
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+struct SplitPair {
+    __nv_bfloat162 u, v, z;
+};
+template <typename W>
+__device__ __forceinline__ void decayed_planes(uint32_t tile, int j0, int s0, W weights, Planes& o) {
     const int lane = threadIdx.x & 31, rr = lane & 7;
     const uint32_t addr = tile + (j0 >> 6) * kPanel + (s0 + rr) * 128 +
                           (((((j0 & 63) >> 3) + (lane >> 3)) ^ rr) << 4);
-    const float* wp = weights + 2 * (lane & 3);
 #pragma unroll
     for (int blk = 0; blk < 4; blk++) {
         uint32_t m[4];
         ldmatrix_x4_trans(addr + blk * 1024, m[0], m[1], m[2], m[3]);
-        const float2 wt = __fmul2_rn(*reinterpret_cast<const float2*>(wp + blk * 8), make_float2(factor, factor));
+        const SplitPair w = weights(blk);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float2 x = __fmul2_rn(make_float2(bf16_lo(m[i]), bf16_hi(m[i])), wt);
+            const __nv_bfloat162 c = as_bf162(m[i]);
+            const __nv_bfloat162 p0 = __hmul2_rn(c, w.u), e = __hfma2(c, w.u, __hneg2(p0));
+            const __nv_bfloat162 f = __hmul2_rn(c, w.v), d = __hfma2(c, w.v, __hneg2(f));
+            const __nv_bfloat162 p1 = __hadd2_rn(e, f), b = __hsub2_rn(p1, e);
+            const __nv_bfloat162 t = __hadd2_rn(__hsub2_rn(e, __hsub2_rn(p1, b)), __hsub2_rn(f, b));
             const int at = 2 * blk + (i & 1);
-            o.p[0][i >> 1][at] = cut_plane(x);
-            o.p[1][i >> 1][at] = cut_plane(x);
-            o.p[2][i >> 1][at] = pack_bf16(x.x, x.y);
+            o.p[0][i >> 1][at] = as_u32(p0);
+            o.p[1][i >> 1][at] = as_u32(p1);
+            o.p[2][i >> 1][at] = as_u32(__hadd2_rn(__hfma2(c, w.z, d), t));
         }
     }
 }
@@ -269,18 +302,11 @@ __device__ __forceinline__ int chunk_count(const Row& k, int reverse, int c) {
 
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&v)[N]) {
-    static_assert(N == 16 || N == 32);
-    if constexpr (N == 16) tmem_ld16(addr, v);
-    else tmem_ld32(addr, v);
+    static_assert(N == 32 || N == 64);
+    tmem_ld32(addr, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+    if constexpr (N == 64) tmem_ld32(addr + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
     tmem_wait_ld();
 }
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[N]) {
-    if constexpr (N == 16) tmem_st16(addr, v);
-    else tmem_st32(addr, v);
-    tmem_wait_st();
-}
-
 template <int KB, int KC>
 __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_constant__ LaParams p,
                                                                  const __grid_constant__ LaMaps maps) {
@@ -438,13 +464,13 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
     } else {
         // ---- the work between products ----------------------------------------------------------
         regs_claim<kRegsCompute>();
-        const int q = warp & 3, part = warp >> 2;     // TMEM lanes 32 q .. + 32; quarter of the columns
+        const int q = warp & 3, half = warp >> 2;     // TMEM lanes 32 q .. + 32; half of the columns
         const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16);
         const int row = q * 32 + lane;                // token of P and O, channel of c (row j of S^T)
-        constexpr int NS = KB / 4;                    // columns of S^T per thread
-        constexpr int NO = KC / 4;                    // columns of O per thread
+        constexpr int NS = KB / 2;                    // columns of S^T per thread
+        constexpr int NO = KC / 2;                    // columns of O per thread
         const bool s_on = q * 32 < KC;                // S^T has KC rows
-        const int i0 = part * NS, o0 = part * NO;
+        const int i0 = half * NS, o0 = half * NO;
         auto arrive = [&](int bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + bar);
@@ -545,58 +571,74 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     arrive(kFixed);
                     if (!(fine = ok(wait(kFixed, fixed++ & 1)))) break;
                 }
-                // planes of C'^T for this quarter's 32 tokens; the third waits for its columns
-                Planes pl;
+                // planes of C'^T for this half's 64 tokens; the third waits for its columns
+                Planes pl[2];
                 if (s_on) {
-                    decayed_planes(smem_u32(st + 2 * L::A), q * 32, part * 32, (n < kT ? dec.part : dec.full) + part * 32,
-                                   1.f, pl);
-                    store_plane(tm + kColC + part * 16, pl.p[1]);
-                    store_plane(tm + kColC + 64 + part * 16, pl.p[0]);
+                    const __nv_bfloat16(*wt)[kT] = dec.plane[n < kT];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int s0 = half * 64 + i * 32;
+                        decayed_planes(smem_u32(st + 2 * L::A), q * 32, s0, [&](int e) {
+                            const int at = s0 + 8 * e + 2 * (lane & 3);
+                            return SplitPair{*reinterpret_cast<const __nv_bfloat162*>(&wt[0][at]),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&wt[1][at]),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&wt[2][at])};
+                        }, pl[i]);
+                        store_plane(tm + kColC + half * 32 + i * 16, pl[i].p[1]);
+                        store_plane(tm + kColC + 64 + half * 32 + i * 16, pl[i].p[0]);
+                    }
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 arrive(kCReady);
 
-                // P: this warp's 32 x 32 block, which the mask empties, halves or leaves whole
+                // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
                 if (!(fine = ok(wait(kScores, par)))) break;
                 tc_fence_after();
-                {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int sb = half * 2 + i;
                     uint32_t o[16];
-                    if (reverse ? part >= q : part <= q) {
+                    if (reverse ? sb >= q : sb <= q) {
                         uint32_t v[32];
-                        tmem_ld<32>(tm + kColScores + part * 32, v);
-                        const int d0 = reverse ? part * 32 - row : row - part * 32;   // distance to the block's first column
-                        const float* wt = dec.score + d0;
-                        if (reverse) {
+                        tmem_ld<32>(tm + kColScores + sb * 32, v);
+                        if (sb != q) {
+                            // w^|t - s| as two factors, neither above one: up to the block's edge and inside it
+                            const float f = dec.score[reverse ? sb * 32 - row : kT - 1 - row + sb * 32 + 31];
+                            const float2 f2 = make_float2(f, f);
 #pragma unroll
-                            for (int e = 0; e < 16; e++)
-                                o[e] = pack_bf16(d0 + 2 * e >= 0 ? __uint_as_float(v[2 * e]) * wt[2 * e] : 0.f,
-                                                 d0 + 2 * e + 1 >= 0 ? __uint_as_float(v[2 * e + 1]) * wt[2 * e + 1] : 0.f);
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 wb = lds128(dec.block + e);
+                                const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])),
+                                                            __fmul2_rn(f2, make_float2(wb.x, wb.y)));
+                                const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])),
+                                                            __fmul2_rn(f2, make_float2(wb.z, wb.w)));
+                                o[e / 2] = pack_bf16(x.x, x.y);
+                                o[e / 2 + 1] = pack_bf16(y.x, y.y);
+                            }
                         } else {
+                            // the table runs with the columns: its entry for column e of the block is wt[e]
+                            const float* wt = dec.score + (reverse ? sb * 32 - row : kT - 1 - row + sb * 32);
+                            const uint32_t live = reverse ? ~0u << lane : ~0u >> (31 - lane);
 #pragma unroll
-                            for (int e = 0; e < 16; e++)
-                                o[e] = pack_bf16(d0 >= 2 * e ? __uint_as_float(v[2 * e]) * wt[-2 * e] : 0.f,
-                                                 d0 >= 2 * e + 1 ? __uint_as_float(v[2 * e + 1]) * wt[-2 * e - 1] : 0.f);
+                            for (int e = 0; e < 32; e += 2) {
+                                const float x = __uint_as_float(v[e]) * wt[e], y = __uint_as_float(v[e + 1]) * wt[e + 1];
+                                o[e / 2] = pack_bf16(live & (1u << e) ? x : 0.f, live & (2u << e) ? y : 0.f);
+                            }
                         }
                     } else {
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[e] = 0;
                     }
                     // over scores that this thread alone reads, and has read
-                    tmem_st16(tm + kColScores + part * 32, o);
-                    if (s_on) store_plane(tm + kColScores + part * 32 + 16, pl.p[2]);
+                    tmem_st16(tm + kColScores + sb * 32, o);
+                    if (s_on) store_plane(tm + kColScores + sb * 32 + 16, pl[i].p[2]);
                 }
-                // A S leaves TMEM, scaled per row
+                // A S leaves TMEM
                 if (!(fine = ok(wait(kAS, par)))) break;
                 tc_fence_after();
-                float acc[NO];
-                {
-                    const float f = r.beta * dec.pow[reverse ? max(n - 1 - row, 0) : row + 1];
-                    uint32_t v[NO];
-                    tmem_ld<NO>(tm + kColO + o0, v);
-#pragma unroll
-                    for (int e = 0; e < NO; e++) acc[e] = __uint_as_float(v[e]) * f;
-                }
+                uint32_t as[NO];
+                tmem_ld<NO>(tm + kColO + o0, as);
                 tmem_wait_st();
                 tc_fence_before();
                 arrive(kPReady);
@@ -609,18 +651,33 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     uint32_t v[NS];
                     tmem_ld<NS>(tm + kColU + i0, v);
 #pragma unroll
-                    for (int e = 0; e < NS; e++) s[e] = fmaf(fn, s[e], __uint_as_float(v[e]));
+                    for (int e = 0; e < NS; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(fn, fn), make_float2(s[e], s[e + 1]),
+                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                        s[e] = x.x;
+                        s[e + 1] = x.y;
+                    }
                 }
                 if (c + 1 < c1) put_state();
 
                 // O
                 if (!(fine = ok(wait(kPC, par)))) break;
                 tc_fence_after();
+                float acc[NO];
                 {
+                    const float f = r.beta * dec.pow[reverse ? max(n - 1 - row, 0) : row + 1];
                     uint32_t v[NO];
                     tmem_ld<NO>(tm + kColO + o0, v);
 #pragma unroll
-                    for (int e = 0; e < NO; e++) acc[e] = row < n ? acc[e] + __uint_as_float(v[e]) : 0.f;
+                    for (int e = 0; e < NO; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(f, f), make_float2(__uint_as_float(as[e]), __uint_as_float(as[e + 1])),
+                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                        acc[e] = x.x;
+                        acc[e + 1] = x.y;
+                    }
+                    if (n < kT && row >= n)
+#pragma unroll
+                        for (int e = 0; e < NO; e++) acc[e] = 0.f;
                 }
                 if (!r.out_f32 && r.out_vec) {
 #pragma unroll
@@ -635,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     // float32 partials and rows a TMA cannot store: through the warp's own piece of the stage,
                     // 16-byte pieces swizzled by the row, then row by row
                     float* own = reinterpret_cast<float*>(st) + warp * 32 * NO;
-                    constexpr int M = NO / 4 - 1;
+                    constexpr int M = 7;
 #pragma unroll
                     for (int i = 0; i < NO; i += 4)
                         *reinterpret_cast<float4*>(own + lane * NO + (((i >> 2) ^ (lane & M)) << 2)) =
@@ -664,10 +721,14 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             const bool out = ends && k.slot == p.nseg - 1 && r.state_out;
             if (!ends || out) {
                 if (s_on) {
-                    uint32_t v[NS];
 #pragma unroll
-                    for (int e = 0; e < NS; e++) v[e] = __float_as_uint(s[e]);
-                    tmem_st<NS>(tm + kColU + i0, v);
+                    for (int i = 0; i < NS; i += 32) {
+                        uint32_t v[32];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(s[i + e]);
+                        tmem_st32(tm + kColU + i0 + i, v);
+                    }
+                    tmem_wait_st();
                     float* dst = ends ? r.state_out + k.bh * r.db * r.dc + row * r.s_j
                                       : p.handoff + (int64_t)(blockIdx.x + 1) * KB * KC + row;
                     const int64_t step = ends ? r.s_i : KC;
@@ -715,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 // is zero in float32 are not read.  C'^T has two buffers of three planes; the threads fill one
 // while the product reads the other.
 constexpr int kStages = 3;
+constexpr int kStateThreads = (kWarps + 2) * 32;
 template <int KB, int KC>
 struct StateSmem {
     static constexpr int B = KB / 64 * kPanel, C = KC / 64 * kPanel;
@@ -728,8 +790,8 @@ struct StateSmem {
 enum StateBar { kSbFull = 0, kSbFree = 3, kSbReady = 6, kSbDone = 8, kSbFixed = 10, kSbDrain = 11 };
 
 template <int KB, int KC>
-__global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __grid_constant__ LaParams p,
-                                                                       const __grid_constant__ LaMaps maps) {
+__global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(const __grid_constant__ LaParams p,
+                                                                            const __grid_constant__ LaMaps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
     using L = StateSmem<KB, KC>;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -823,8 +885,8 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
             }
         }
         __syncwarp();
-    } else if (warp < kWarps) {
-        const int q = warp & 3, part = warp >> 2;
+    } else {
+        const int q = warp & 3, half = warp >> 2;
         const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16);
         const int row = q * 32 + lane;
         const bool s_on = q * 32 < KC;
@@ -838,31 +900,51 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_state_kernel(const __g
             const int c = cb + i, n = count(c);
             unsigned char* st = smem + (i % kStages) * L::STAGE;
             if (!(fine = ok(wait(kSbFull + i % kStages, (i / kStages) & 1)))) break;
-            if (i >= 2 && !(fine = ok(wait(kSbDone + (i & 1), ((i - 2) >> 1) & 1)))) break;   // the buffer is free
             if (n < kT) {
                 zero_rows(st, L::STAGE / kPanel, n, tid);
                 arrive(kSbFixed);
                 if (!(fine = ok(wait(kSbFixed, 0)))) break;
             }
-            if (s_on) {
+            const float f = r.sigma * exp2f(g2 * (float)far(c));
+#pragma unroll 1
+            for (int e = 0; e < 2; e++) {
+                const int s0 = half * 64 + e * 32;
                 Planes pl;
-                decayed_planes(smem_u32(st + L::B), q * 32, part * 32, (n < kT ? dec.part : dec.full) + part * 32,
-                               exp2f(g2 * (float)far(c)), pl);
-                const uint32_t cp = tm + 128 + (i & 1) * 192 + part * 16;
+                if (s_on)
+                    decayed_planes(smem_u32(st + L::B), q * 32, s0, [&](int b) {
+                        const int at = s0 + 8 * b + 2 * (lane & 3);
+                        float x = f * dec.pow[reverse ? at + 1 : max(n - 1 - at, 0)];
+                        float y = f * dec.pow[reverse ? at + 2 : max(n - 2 - at, 0)];
+                        x = at < n ? x : 0.f;
+                        y = at + 1 < n ? y : 0.f;
+                        SplitPair w;
+                        w.u = __floats2bfloat162_rn(x, y);
+                        x -= __low2float(w.u);
+                        y -= __high2float(w.u);
+                        w.v = __floats2bfloat162_rn(x, y);
+                        w.z = __floats2bfloat162_rn(x - __low2float(w.v), y - __high2float(w.v));
+                        return w;
+                    }, pl);
+                if (e == 0 && i >= 2 && !(fine = ok(wait(kSbDone + (i & 1), ((i - 2) >> 1) & 1)))) break;   // the buffer is free
+                tc_fence_after();
+                if (s_on) {
+                    const uint32_t cp = tm + 128 + (i & 1) * 192 + s0 / 2;
 #pragma unroll
-                for (int e = 0; e < 3; e++) store_plane(cp + e * 64, pl.p[2 - e]);   // smallest first
-                tmem_wait_st();
+                    for (int u = 0; u < 3; u++) store_plane(cp + u * 64, pl.p[2 - u]);   // smallest first
+                    tmem_wait_st();
+                }
             }
+            if (!fine) break;
             tc_fence_before();
             arrive(kSbReady + (i & 1));
         }
         if (fine && nchunk > 0) fine = ok(wait(kSbDone + ((nchunk - 1) & 1), ((nchunk - 1) >> 1) & 1));
         tc_fence_after();
         if (fine && s_on) {
-            constexpr int NS = KB / 4;
+            constexpr int NS = KB / 2;
             float* e = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc;
 #pragma unroll 1
-            for (int i = part * NS; i < part * NS + NS; i += 8) {
+            for (int i = half * NS; i < half * NS + NS; i += 8) {
                 uint32_t v[8] = {};
                 if (nchunk > 0) {
                     tmem_ld8(tm + i, v);
@@ -888,7 +970,7 @@ cudaError_t launch_tc(const LaParams& p, const LaMaps& maps, int sms, cudaStream
         e = cudaFuncSetAttribute(linattn_tc_state_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  StateSmem<KB, KC>::BYTES);
         if (e != cudaSuccess) return e;
-        linattn_tc_state_kernel<KB, KC><<<(unsigned)(rows * (p.nseg - 1)), kThreads, StateSmem<KB, KC>::BYTES, stream>>>(p, maps);
+        linattn_tc_state_kernel<KB, KC><<<(unsigned)(rows * (p.nseg - 1)), kStateThreads, StateSmem<KB, KC>::BYTES, stream>>>(p, maps);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     e = cudaFuncSetAttribute(linattn_tc_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
