@@ -13,13 +13,14 @@
 //
 // Roundings below float32: P and the copy of S that A multiplies are bfloat16, each on its own
 // part of O, whose result is rounded to bfloat16 anyway.  The state itself is float32: C' is
-// carried as a sum of three bfloat16 planes (24 bits) and U is added to the decayed state in
-// float32.
+// carried as a sum of four bfloat16 planes (24 bits of the weight) and U is added to the decayed
+// state in float32.
 //
 // One CTA per SM.  Warps 0-7 do the work between products, two for each quarter of the TMEM
 // lanes, each with half of the columns; warp 8 issues the products, warp 9 the loads, warp 10
 // the stores.  The order of the phases lets each run beside a product:
-//     C'(c) | scores, A S;   P(c) | U;   S(c + 1) | P C;   O(c) | scores(c + 1).
+//     C'(c), first 64 tokens | scores, A S;   P(c) | U, first half;   C'(c), last 64 | P C;
+//     O(c) | U, last half;   S(c + 1) | scores(c + 1).
 //
 // With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
 // range, so its first row may have been begun by the CTA before it and its last may be finished
@@ -47,10 +48,9 @@ constexpr int kRegsCompute = 224, kRegsControl = 56;
 constexpr uint32_t kTmemCols = 512;
 // TMEM columns
 constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P then takes the first 16
-                                           //      and the third plane of C' the last 16
 constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
-constexpr uint32_t kColC = 384;            // 64 + 64: second and first plane of C'^T
+constexpr uint32_t kColC = 384;            // 4 x 32: planes of C'^T for 64 tokens
 // Tries before a wait has run out: each lasts 30 cycles or more (a try may suspend for longer), so
 // 0.06 s or more, against the microseconds of the longest wait that ends
 constexpr int kTries = 1 << 22;
@@ -113,7 +113,16 @@ struct TcSmem {
     static constexpr int BYTES = USED > 120 * 1024 ? USED : 120 * 1024;
 };
 
-enum Bar { kFull = 0, kStaged = 2, kFree = 4, kScores = 6, kAS, kUpd, kPC, kSReady, kCReady, kPReady, kFixed, kItem, kDrain };
+// mbarriers.  Those of a pair belong to one stage, whose next use nobody can reach before everybody
+// has seen this one: a waiter never falls two phases behind.
+enum Bar {
+    kFull = 0,       // [2] a stage's tiles are there
+    kStaged = 2,     // [2] O is staged over them
+    kFree = 4,       // [2] and stored, and every product has read them
+    kUpd = 6,        // [2] U is complete
+    kScores = 8, kAS, kPC, kCFree,      // products complete; kCFree: those of the first 64 tokens' planes
+    kSReady, kCReady, kPReady, kFixed, kItem, kDrain
+};
 
 struct Waiter {
     uint64_t* bars;
@@ -147,19 +156,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// The three bfloat16 planes of the decayed, transposed C' for the 32 channels j0 .. of the warp and
+// The four bfloat16 planes of the decayed, transposed C' for the 32 channels j0 .. of the warp and
 // the 32 tokens s0 .., as TMEM fragments: plane[lanes 0-15, 16-31][two registers per 8 tokens].
 // weights(i) gives the split weights of the lane's token pair of the 8 tokens s0 + 8 i ...
 //
-// In packed bfloat16 arithmetic (the FMA pipe; splitting float32 products takes more instructions,
-// most of them on the slower ALU pipe).  The weight is u + v + z, 8 bits each, and c has 8 bits, so
-// the rounding error of a product is itself a bfloat16, which one fused multiply-add yields:
-//     c u = p0 + e,   c v = q + d,   e + q = p1 + t      all exactly (the last is Knuth's two-sum)
-// and what is left, c z + d + t, is 2^-16 of the whole and needs only p2's 8 bits.  (Without the
-// two-sum, p2 = rn(c z + rn(c v + rn(e - p1))): half the instructions and a state error of 1.7e-6
-// instead of 4e-7.)
+// In packed bfloat16 arithmetic: the weight is u + v + z, 8 bits each, and c has 8 bits, so the
+// rounding error of a product is itself a bfloat16, which one fused multiply-add yields:
+//     c u = p0 + p1,   c v = p2 + d      both exactly,     p3 = rn(c z + d), 2^-16 of the whole
+// Five operations for two elements.  Three planes (p1 + p2 joined by a two-sum, the rest in the
+// third) took twelve and 1500 cycles of a chunk more, three planes cut from float32 products took
+// as many on the half-rate ALU pipe, and two planes leave a state error of 2.7e-6 instead of 4e-7.
 struct Planes {
-    uint32_t p[3][2][8];
+    uint32_t p[4][2][8];
 };
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -180,14 +188,12 @@ __device__ __forceinline__ void decayed_planes(uint32_t tile, int j0, int s0, W 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const __nv_bfloat162 c = as_bf162(m[i]);
-            const __nv_bfloat162 p0 = __hmul2_rn(c, w.u), e = __hfma2(c, w.u, __hneg2(p0));
-            const __nv_bfloat162 f = __hmul2_rn(c, w.v), d = __hfma2(c, w.v, __hneg2(f));
-            const __nv_bfloat162 p1 = __hadd2_rn(e, f), b = __hsub2_rn(p1, e);
-            const __nv_bfloat162 t = __hadd2_rn(__hsub2_rn(e, __hsub2_rn(p1, b)), __hsub2_rn(f, b));
+            const __nv_bfloat162 p0 = __hmul2_rn(c, w.u), p2 = __hmul2_rn(c, w.v);
             const int at = 2 * blk + (i & 1);
             o.p[0][i >> 1][at] = as_u32(p0);
-            o.p[1][i >> 1][at] = as_u32(p1);
-            o.p[2][i >> 1][at] = as_u32(__hadd2_rn(__hfma2(c, w.z, d), t));
+            o.p[1][i >> 1][at] = as_u32(__hfma2(c, w.u, __hneg2(p0)));
+            o.p[2][i >> 1][at] = as_u32(p2);
+            o.p[3][i >> 1][at] = as_u32(__hfma2(c, w.z, __hfma2(c, w.v, __hneg2(p2))));
         }
     }
 }
@@ -334,8 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             mbar_init(bars + kFull + i, 1);
             mbar_init(bars + kStaged + i, kWarps);
             mbar_init(bars + kFree + i, 1);
+            mbar_init(bars + kUpd + i, 1);
         }
-        for (int i : {kScores, kAS, kUpd, kPC, kDrain}) mbar_init(bars + i, 1);
+        for (int i : {kScores, kAS, kPC, kCFree, kDrain}) mbar_init(bars + i, 1);
         for (int i : {kSReady, kCReady, kPReady, kFixed, kItem}) mbar_init(bars + i, kWarps);
         *abort = 0;
         fence_mbar_init();
@@ -385,7 +392,6 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const Row k = items.row(n, c0, c1);
                 const LaRole& r = p.role[k.ri];
                 for (int c = c0; c < c1; c++, it++) {
-                    // the chunk's output is staged over its a (and b) tile, and nobody uses its stage any more
                     if (!(fine = wait(kStaged + (it & 1), (it >> 1) & 1))) break;
                     if (!r.out_f32 && r.out_vec) {
                         const int t = chunk_first(k, r.reverse, c);
@@ -396,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         tma_store_commit();
                         tma_store_wait_read_all();
                     }
+                    if (!(fine = wait(kUpd + (it & 1), (it >> 1) & 1))) break;    // the last product to read the stage
                     mbar_arrive(bars + kFree + (it & 1));
                 }
             }
@@ -415,8 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     const uint32_t st = smem_u32(smem + (it & 1) * L::STAGE), par = it & 1;
                     if (!(fine = wait(kFull + (it & 1), (it >> 1) & 1))) break;
                     if (chunk_count(k, reverse, c) < kT && !(fine = wait(kFixed, fixed++ & 1))) break;
-                    // P and the third plane of the previous chunk are still read until these two
-                    if (it > 0 && !(fine = wait(kPC, par ^ 1) && wait(kUpd, par ^ 1))) break;
+                    if (it > 0 && !(fine = wait(kPC, par ^ 1))) break;       // the last P has been read
                     tc_fence_after();
                     // K-major panels of 64 channels: 16 channels are 32 bytes
                     const uint32_t a_desc = umma_desc_lo(st, 16), b_desc = umma_desc_lo(st + L::A, 16);
@@ -434,25 +440,27 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         umma_ss(tmem + kColO, a_desc + (((i >> 2) * kPanel + (i & 3) * 32) >> 4),
                                 s_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, i > 0);
                     umma_commit(bars + kAS);
-                    if (!(fine = wait(kCReady, par))) break;
-                    tc_fence_after();
                     // N-major panels of 64 channels: 16 tokens are 2048 bytes
                     const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
-#pragma unroll
-                    for (int i = 0; i < 2 * kT / 16; i++)      // second plane, then first
-                        umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 7) * (2048 >> 4), id_upd, i > 0);
-                    if (!(fine = wait(kPReady, par))) break;
+                    if (!(fine = wait(kCReady, 0))) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < kT / 16; i++)
-                        umma_ts(tmem + kColU, tmem + kColScores + (i >> 1) * 32 + 16 + (i & 1) * 8,
-                                bn_desc + i * (2048 >> 4), id_upd, true);
-                    umma_commit(bars + kUpd);
+                    for (int i = 0; i < 16; i++)               // the smallest plane first
+                        umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 3) * (2048 >> 4), id_upd, i > 0);
+                    umma_commit(bars + kCFree);
+                    if (!(fine = wait(kPReady, par))) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < kT / 16; i++)
                         umma_ts(tmem + kColO, tmem + kColScores + (i >> 1) * 32 + (i & 1) * 8, cn_desc + i * (2048 >> 4),
                                 id_pc, i > 0);
                     umma_commit(bars + kPC);
+                    if (!(fine = wait(kCReady, 1))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd, true);
+                    umma_commit(bars + kUpd + par);
                 }
             }
             if (!fine) {
@@ -571,26 +579,26 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     arrive(kFixed);
                     if (!(fine = ok(wait(kFixed, fixed++ & 1)))) break;
                 }
-                // planes of C'^T for this half's 64 tokens; the third waits for its columns
-                Planes pl[2];
-                if (s_on) {
-                    const __nv_bfloat16(*wt)[kT] = dec.plane[n < kT];
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int s0 = half * 64 + i * 32;
+                // planes of C'^T, 64 tokens at a time, of which this warp does 32
+                auto put_planes = [&](int sub) {
+                    if (s_on) {
+                        const __nv_bfloat16(*wt)[kT] = dec.plane[n < kT];
+                        const int s0 = sub * 64 + half * 32;
+                        Planes pl;
                         decayed_planes(smem_u32(st + 2 * L::A), q * 32, s0, [&](int e) {
                             const int at = s0 + 8 * e + 2 * (lane & 3);
                             return SplitPair{*reinterpret_cast<const __nv_bfloat162*>(&wt[0][at]),
                                              *reinterpret_cast<const __nv_bfloat162*>(&wt[1][at]),
                                              *reinterpret_cast<const __nv_bfloat162*>(&wt[2][at])};
-                        }, pl[i]);
-                        store_plane(tm + kColC + half * 32 + i * 16, pl[i].p[1]);
-                        store_plane(tm + kColC + 64 + half * 32 + i * 16, pl[i].p[0]);
+                        }, pl);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) store_plane(tm + kColC + e * 32 + half * 16, pl.p[3 - e]);
+                        tmem_wait_st();
                     }
-                    tmem_wait_st();
-                }
-                tc_fence_before();
-                arrive(kCReady);
+                    tc_fence_before();
+                    arrive(kCReady);
+                };
+                put_planes(0);
 
                 // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
                 if (!(fine = ok(wait(kScores, par)))) break;
@@ -632,7 +640,6 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     }
                     // over scores that this thread alone reads, and has read
                     tmem_st16(tm + kColScores + sb * 32, o);
-                    if (s_on) store_plane(tm + kColScores + sb * 32 + 16, pl[i].p[2]);
                 }
                 // A S leaves TMEM
                 if (!(fine = ok(wait(kAS, par)))) break;
@@ -643,22 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 tc_fence_before();
                 arrive(kPReady);
 
-                // the state after this chunk; the stage's b is also free after the update
-                if (!(fine = ok(wait(kUpd, par)))) break;
+                if (!(fine = ok(wait(kCFree, par)))) break;
                 tc_fence_after();
-                if (s_on) {
-                    const float fn = dec.pow[n];
-                    uint32_t v[NS];
-                    tmem_ld<NS>(tm + kColU + i0, v);
-#pragma unroll
-                    for (int e = 0; e < NS; e += 2) {
-                        const float2 x = __ffma2_rn(make_float2(fn, fn), make_float2(s[e], s[e + 1]),
-                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                        s[e] = x.x;
-                        s[e + 1] = x.y;
-                    }
-                }
-                if (c + 1 < c1) put_state();
+                put_planes(1);
 
                 // O
                 if (!(fine = ok(wait(kPC, par)))) break;
@@ -679,7 +673,10 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                         for (int e = 0; e < NO; e++) acc[e] = 0.f;
                 }
-                if (!r.out_f32 && r.out_vec) {
+                const bool tma = !r.out_f32 && r.out_vec;
+                // the tile is staged over a, and where that is not enough over b, which the update reads
+                if ((!tma || KC > KB) && !(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
+                if (tma) {
 #pragma unroll
                     for (int i = 0; i < NO; i += 8) {
                         const uint4 v = make_uint4(pack_bf16(acc[i], acc[i + 1]), pack_bf16(acc[i + 2], acc[i + 3]),
@@ -713,6 +710,23 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 }
                 tc_fence_before();
                 arrive(kStaged + (it & 1));
+
+                // the state after this chunk
+                if (!(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
+                tc_fence_after();
+                if (s_on) {
+                    const float fn = dec.pow[n];
+                    uint32_t v[NS];
+                    tmem_ld<NS>(tm + kColU + i0, v);
+#pragma unroll
+                    for (int e = 0; e < NS; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(fn, fn), make_float2(s[e], s[e + 1]),
+                                                    make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                        s[e] = x.x;
+                        s[e + 1] = x.y;
+                    }
+                }
+                if (c + 1 < c1) put_state();
             }
             if (!fine) break;
 
@@ -773,8 +787,8 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 
 // The state a segment reaches from a zero start: only U, with every token weighted towards the
 // segment's end, so that the sum needs no rescaling between chunks, and chunks whose every weight
-// is zero in float32 are not read.  C'^T has two buffers of three planes; the threads fill one
-// while the product reads the other.
+// is zero in float32 are not read.  C'^T has two buffers of 64 tokens; the threads fill one while
+// the product reads the other.
 constexpr int kStages = 3;
 constexpr int kStateThreads = (kWarps + 2) * 32;
 template <int KB, int KC>
@@ -869,15 +883,19 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
             bool fine = true;
             for (int i = 0; i < nchunk; i++) {
                 if (!(fine = wait(kSbFull + i % kStages, (i / kStages) & 1))) break;
-                if (!(fine = wait(kSbReady + (i & 1), (i >> 1) & 1))) break;
-                tc_fence_after();
                 const uint32_t bn_desc = umma_desc_lo(smem_u32(smem + (i % kStages) * L::STAGE), kPanel);
-                const uint32_t cp = tmem + 128 + (i & 1) * 192;
+#pragma unroll 1
+                for (int e = 0; e < 2; e++) {
+                    if (!(fine = wait(kSbReady + e, i & 1))) break;
+                    tc_fence_after();
 #pragma unroll
-                for (int e = 0; e < 3 * kT / 16; e++)
-                    umma_ts(tmem, cp + e * 8, bn_desc + (e & 7) * (2048 >> 4), id_upd, i > 0 || e > 0);
+                    for (int m = 0; m < 16; m++)               // the smallest plane first
+                        umma_ts(tmem, tmem + 128 + e * 128 + m * 8, bn_desc + (e * 4 + (m & 3)) * (2048 >> 4), id_upd,
+                                i > 0 || e > 0 || m > 0);
+                    umma_commit(bars + kSbDone + e);
+                }
+                if (!fine) break;
                 umma_commit(bars + kSbFree + i % kStages);
-                umma_commit(bars + kSbDone + (i & 1));
             }
             if (!fine) {
                 umma_commit(bars + kSbDrain);
@@ -908,7 +926,7 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
             const float f = r.sigma * exp2f(g2 * (float)far(c));
 #pragma unroll 1
             for (int e = 0; e < 2; e++) {
-                const int s0 = half * 64 + e * 32;
+                const int s0 = e * 64 + half * 32;
                 Planes pl;
                 if (s_on)
                     decayed_planes(smem_u32(st + L::B), q * 32, s0, [&](int b) {
@@ -925,20 +943,19 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
                         w.z = __floats2bfloat162_rn(x - __low2float(w.v), y - __high2float(w.v));
                         return w;
                     }, pl);
-                if (e == 0 && i >= 2 && !(fine = ok(wait(kSbDone + (i & 1), ((i - 2) >> 1) & 1)))) break;   // the buffer is free
+                if (i > 0 && !(fine = ok(wait(kSbDone + e, (i - 1) & 1)))) break;   // the buffer is free
                 tc_fence_after();
                 if (s_on) {
-                    const uint32_t cp = tm + 128 + (i & 1) * 192 + s0 / 2;
 #pragma unroll
-                    for (int u = 0; u < 3; u++) store_plane(cp + u * 64, pl.p[2 - u]);   // smallest first
+                    for (int u = 0; u < 4; u++) store_plane(tm + 128 + e * 128 + u * 32 + half * 16, pl.p[3 - u]);
                     tmem_wait_st();
                 }
+                tc_fence_before();
+                arrive(kSbReady + e);
             }
             if (!fine) break;
-            tc_fence_before();
-            arrive(kSbReady + (i & 1));
         }
-        if (fine && nchunk > 0) fine = ok(wait(kSbDone + ((nchunk - 1) & 1), ((nchunk - 1) >> 1) & 1));
+        if (fine && nchunk > 0) fine = ok(wait(kSbDone + 1, (nchunk - 1) & 1));
         tc_fence_after();
         if (fine && s_on) {
             constexpr int NS = KB / 2;
