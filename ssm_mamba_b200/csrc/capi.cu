@@ -50,7 +50,7 @@ cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
 cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, int sms, cudaStream_t stream);
-cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream);
+cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream);
 cudaError_t launch_linattn_update(const LaUpdParams& p, int is_bf16, int vec, cudaStream_t stream);
 cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream);
 int layer_norm_parts(int64_t rows, int dim, int sms);
@@ -1002,16 +1002,17 @@ static int la_plan_segments(int64_t rows, int64_t seqlen, int sms, int* seglen) 
     return (int)((seqlen + len - 1) / len);
 }
 
-// Map of a bfloat16 (batch, token, head, channel) tensor; box of 64 channels x 128 tokens, 128-byte
-// swizzle, zeros outside.
-static int la_encode(CUtensorMap* map, const void* ptr, int64_t d, int64_t L, int64_t heads, int64_t batch, int64_t st,
-                     int64_t sh, int64_t sb) {
+// Map of a bfloat16 or float32 (batch, token, head, channel) tensor; box of 128 bytes of channels x
+// 128 tokens, 128-byte swizzle, zeros outside.
+static int la_encode(CUtensorMap* map, const void* ptr, int f32, int64_t d, int64_t L, int64_t heads, int64_t batch,
+                     int64_t st, int64_t sh, int64_t sb) {
+    const int64_t es = f32 ? 4 : 2;
     cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)L, (cuuint64_t)heads, (cuuint64_t)batch};
     // a dimension of size 1 may have any stride; give TMA a valid one
-    cuuint64_t strides[3] = {(cuuint64_t)(L == 1 ? 256 : st * 2), (cuuint64_t)(heads == 1 ? 256 : sh * 2),
-                             (cuuint64_t)(batch == 1 ? 256 : sb * 2)};
-    cuuint32_t box[4] = {64u, 128u, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
-    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr,
+    cuuint64_t strides[3] = {(cuuint64_t)(L == 1 ? 256 : st * es), (cuuint64_t)(heads == 1 ? 256 : sh * es),
+                             (cuuint64_t)(batch == 1 ? 256 : sb * es)};
+    cuuint32_t box[4] = {f32 ? 32u : 64u, 128u, 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
+    CUresult r = g_encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(SSM_ERR_CUDA, "cuTensorMapEncodeTiled (linear attention) failed (%d)", (int)r);
@@ -1130,7 +1131,8 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         LaRole& r = p.role[i];
         if (heads == H) {
             const LaTensor t = la_tensor(a, out, sb, st, sh, heads);
-            r.out = out; r.o_sb = sb; r.o_st = st; r.o_sh = sh; r.out_vec = t.vec;
+            r.out = out; r.o_sb = sb; r.o_st = st; r.o_sh = sh;
+            r.out_vec = la_tma_ok(t, a->seqlen, heads, a->batch);
         } else {
             r.out = ws + pl.part[i]; r.out_f32 = 1; r.out_vec = d % 4 == 0;
             r.o_sh = d; r.o_st = (int64_t)H * d; r.o_sb = a->seqlen * r.o_st;
@@ -1170,12 +1172,12 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         for (int i = 0; i < p.nroles; i++) {
             const LaRole& r = p.role[i];
             auto in = [&](CUtensorMap* m, const LaTensor& t, int d) {
-                return la_encode(m, t.p, d, a->seqlen, H / t.share, a->batch, t.st, t.sh, t.sb);
+                return la_encode(m, t.p, 0, d, a->seqlen, H / t.share, a->batch, t.st, t.sh, t.sb);
             };
             if ((rc = in(&maps.a[i], r.a, r.db)) || (rc = in(&maps.b[i], r.b, r.db)) || (rc = in(&maps.c[i], r.c, r.dc)))
                 return rc;
-            if (!r.out_f32 && r.out_vec &&
-                (rc = la_encode(&maps.o[i], r.out, r.dc, a->seqlen, H, a->batch, r.o_st, r.o_sh, r.o_sb)))
+            if (r.out_vec &&
+                (rc = la_encode(&maps.o[i], r.out, r.out_f32, r.dc, a->seqlen, H, a->batch, r.o_st, r.o_sh, r.o_sb)))
                 return rc;
         }
         const int kmax = dk > dv ? dk : dv;
@@ -1194,7 +1196,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         if (i == 0) { g.out = a->dq; g.o_sb = a->dq_batch_stride; g.o_st = a->dq_token_stride; g.o_sh = a->dq_head_stride; g.share = q.share; }
         if (i == 1) { g.out = a->dv_; g.o_sb = a->dv_batch_stride; g.o_st = a->dv_token_stride; g.o_sh = a->dv_head_stride; g.share = v.share; }
         if (i == 2) { g.out = a->dk_; g.o_sb = a->dk_batch_stride; g.o_st = a->dk_token_stride; g.o_sh = a->dk_head_stride; g.share = k.share; }
-        e = launch_linattn_group(g, is_bf16, di->sms, stream);
+        e = launch_linattn_group(g, is_bf16, stream);
         if (e != cudaSuccess) return cuda_fail(e, "linear attention head-sum launch");
     }
     return SSM_OK;

@@ -153,31 +153,64 @@ __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(
     __shared__ float fold[RPC > 1 ? RPC * TPR * VT : 1];
     const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     float dw[NV][VT] = {}, db[NV][VT] = {};
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPC + sub; row < p.rows; row += (int64_t)gridDim.x * RPC, turn ^= 1) {
+    // a row's inputs, fetched while the row before it is worked on
+    struct Fetched {
+        Raw<T, VT> x[NV], g[NV];
+        float mean, rstd;
+    };
+    auto fetch = [&](int64_t row, Fetched& f) {
+        if (row >= p.rows) return;
         const T* x = static_cast<const T*>(p.x) + row * p.x_s;
         const T* dy = static_cast<const T*>(p.dy) + row * p.dy_s;
-        Raw<T, VT> xr[NV], gr[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (tid + i * TPR) * VT;
             if (c < p.dim) {
-                xr[i].load(x + c);
-                gr[i].load(dy + c);
+                f.x[i].load(x + c);
+                f.g[i].load(dy + c);
             }
         }
-        const float mean = p.mean[row], rstd = p.rstd[row];
+        f.mean = p.mean[row];
+        f.rstd = p.rstd[row];
+    };
+    // narrow vectors: the weights stay in registers too
+    constexpr bool kKeep = VT < 8;
+    float kept[kKeep ? NV : 1][VT];
+    if (kKeep) {
+#pragma unroll
+        for (int i = 0; i < (kKeep ? NV : 1); i++) {
+            const int c = (tid + i * TPR) * VT;
+            if (p.weight && c < p.dim) load_f32<VT>(p.weight + c, kept[i]);
+            else
+#pragma unroll
+                for (int j = 0; j < VT; j++) kept[i][j] = 1.f;
+        }
+    }
+    auto weights = [&](int i, float (&w)[VT]) {
+        const int c = (tid + i * TPR) * VT;
+        if (!kKeep && p.weight) {
+            load_f32<VT>(p.weight + c, w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VT; j++) w[j] = kKeep ? kept[i][j] : 1.f;
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * RPC;
+    int turn = 0;
+    Fetched now, next;
+    fetch((int64_t)blockIdx.x * RPC + sub, now);
+    for (int64_t row = (int64_t)blockIdx.x * RPC + sub; row < p.rows; row += step, turn ^= 1) {
+        fetch(row + step, next);
+        const float mean = now.mean, rstd = now.rstd;
         float v[2] = {0.f, 0.f};                  // sum of c, sum of c h
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (tid + i * TPR) * VT;
-            if (c >= p.dim) continue;
+            if ((tid + i * TPR) * VT >= p.dim) continue;
             float w[VT];
-            if (p.weight) load_f32<VT>(p.weight + c, w);
+            weights(i, w);
 #pragma unroll
             for (int j = 0; j < VT; j++) {
-                const float g = gr[i].get(j), h = (xr[i].get(j) - mean) * rstd;
-                const float e = p.weight ? g * w[j] : g;
+                const float g = now.g[i].get(j), h = (now.x[i].get(j) - mean) * rstd, e = g * w[j];
                 v[0] += e;
                 v[1] = fmaf(e, h, v[1]);
                 dw[i][j] = fmaf(g, h, dw[i][j]);
@@ -192,15 +225,15 @@ __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(
             const int c = (tid + i * TPR) * VT;
             if (c >= p.dim) continue;
             float o[VT], w[VT];
-            if (p.weight) load_f32<VT>(p.weight + c, w);
+            weights(i, w);
 #pragma unroll
             for (int j = 0; j < VT; j++) {
-                const float g = gr[i].get(j), h = (xr[i].get(j) - mean) * rstd;
-                const float e = p.weight ? g * w[j] : g;
-                o[j] = rstd * (e - m0 - h * m1);
+                const float h = (now.x[i].get(j) - mean) * rstd;
+                o[j] = rstd * (now.g[i].get(j) * w[j] - m0 - h * m1);
             }
             store_elems<T, VT>(dx + c, o);
         }
+        now = next;
     }
     // one partial row per CTA: [cta][0] dw, [cta][1] db
     float* out = p.part + (int64_t)blockIdx.x * 2 * p.dim;
@@ -299,43 +332,69 @@ __global__ void __launch_bounds__(256) layer_norm_wide_dw_kernel(const __grid_co
     out[p.dim] = db;
 }
 
-// dweight / dbias = sums of the nparts partial rows: 32 columns x 8 threads per CTA, each
-// thread every 8th row, then the 8 sums in order
-__global__ void __launch_bounds__(256) layer_norm_dw_kernel(const float* part, int nparts, int dim, float* dweight,
-                                                            float* dbias) {
-    __shared__ float s[8][32];
+// dweight / dbias = sums of the nparts partial rows: 32 columns x 32 threads per CTA, each
+// thread every 32nd row, then the 32 sums in order
+__global__ void __launch_bounds__(1024) layer_norm_dw_kernel(const float* part, int nparts, int dim, float* dweight,
+                                                             float* dbias) {
+    __shared__ float s[32][33];
     const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float* out = blockIdx.y ? dbias : dweight;
     if (!out) return;
     float sum = 0.f;
     if (c < dim)
-        for (int i = y; i < nparts; i += 8) sum += part[((int64_t)i * 2 + blockIdx.y) * dim + c];
+#pragma unroll 4
+        for (int i = y; i < nparts; i += 32) sum += part[((int64_t)i * 2 + blockIdx.y) * dim + c];
     s[y][lane] = sum;
     __syncthreads();
-    if (y == 0 && c < dim) {
+    // warp y adds up column y
+    sum = s[lane][y];
 #pragma unroll
-        for (int i = 1; i < 8; i++) sum += s[i][lane];
-        out[c] = sum;
-    }
+    for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (lane == 0 && blockIdx.x * 32 + y < dim) out[blockIdx.x * 32 + y] = sum;
+}
+
+// CTAs of the backward: as many as fit on the SMs at once, no more than there are partial rows for
+template <typename K>
+int resident_ctas(K kernel, int threads, int most) {
+    int dev = 0, sms = 0, occ = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, 0) != cudaSuccess || occ < 1)
+        return most;
+    return sms * occ < most ? sms * occ : most;
 }
 
 template <typename T, int VT, int E, int TPR>
-cudaError_t launch_rows(const LnParams& p, int backward, cudaStream_t stream) {
+cudaError_t launch_rows(LnParams& p, int backward, cudaStream_t stream) {
     constexpr int RPC = kRowsPerCta<TPR>;
-    if (!backward) layer_norm_fwd_kernel<T, VT, E, TPR><<<(unsigned)((p.rows + RPC - 1) / RPC), TPR * RPC, 0, stream>>>(p);
-    else layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, 0, stream>>>(p);
+    if (!backward) {
+        layer_norm_fwd_kernel<T, VT, E, TPR><<<(unsigned)((p.rows + RPC - 1) / RPC), TPR * RPC, 0, stream>>>(p);
+    } else {
+        static const int resident = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, 1 << 20);
+        if (p.nparts > resident) p.nparts = resident;
+        layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, 0, stream>>>(p);
+    }
     return cudaGetLastError();
 }
 
+// Elements per thread are kept to 32 as raw bfloat16 and to 16 as float32 or single elements: the
+// backward holds two rows and two sums per column.
 template <typename T, int VT>
-cudaError_t dispatch(const LnParams& p, int backward, cudaStream_t stream) {
+cudaError_t dispatch(LnParams& p, int backward, cudaStream_t stream) {
     if (p.dim <= 256) return launch_rows<T, VT, 8, 32>(p, backward, stream);
     if (p.dim <= 512) return launch_rows<T, VT, 16, 32>(p, backward, stream);
-    if (p.dim <= 768) return launch_rows<T, VT, 24, 32>(p, backward, stream);
-    if (p.dim <= 1024) return launch_rows<T, VT, 32, 32>(p, backward, stream);
-    if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
-    if (p.dim <= 128 * 24) return launch_rows<T, VT, 24, 128>(p, backward, stream);
-    if (p.dim <= 4096) return launch_rows<T, VT, 32, 128>(p, backward, stream);
+    if constexpr (VT == 8) {
+        if (p.dim <= 768) return launch_rows<T, VT, 24, 32>(p, backward, stream);
+        if (p.dim <= 1024) return launch_rows<T, VT, 32, 32>(p, backward, stream);
+        if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
+        if (p.dim <= 128 * 24) return launch_rows<T, VT, 24, 128>(p, backward, stream);
+        if (p.dim <= 4096) return launch_rows<T, VT, 32, 128>(p, backward, stream);
+    } else {
+        if (p.dim <= 1024) return launch_rows<T, VT, 8, 128>(p, backward, stream);
+        if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
+        if (p.dim <= 256 * 12) return launch_rows<T, VT, 12, 256>(p, backward, stream);
+        if (p.dim <= 4096) return launch_rows<T, VT, 16, 256>(p, backward, stream);
+    }
     return launch_rows<T, VT, 16, 512>(p, backward, stream);
 }
 
@@ -353,16 +412,17 @@ cudaError_t dispatch_wide(const LnParams& p, int backward, cudaStream_t stream) 
 
 }  // namespace
 
-// Partial rows of dw and db: one per CTA of the backward, at most two CTAs per SM, none
-// without a row; for wide rows 64 slices of the rows.
+// Partial rows of dw and db there is room for: one per CTA of the backward, at most four CTAs per
+// SM, none without a row; for wide rows 64 slices of the rows.
 int layer_norm_parts(int64_t rows, int dim, int sms) {
     if (dim > kLnMaxDim) return (int)(rows < 64 ? rows : 64);
-    const int rpc = dim <= 1024 ? 4 : 1;
+    const int rpc = dim <= 512 ? 4 : 1;
     const int64_t ctas = (rows + rpc - 1) / rpc, most = (int64_t)sms * 4;
     return (int)(ctas < most ? ctas : most);
 }
 
-cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backward, cudaStream_t stream) {
+cudaError_t launch_layer_norm(const LnParams& params, int is_bf16, int vec, int backward, cudaStream_t stream) {
+    LnParams p = params;
     cudaError_t e;
     if (p.dim > kLnMaxDim) {
         e = is_bf16 ? dispatch_wide<__nv_bfloat16>(p, backward, stream) : dispatch_wide<float>(p, backward, stream);
@@ -372,7 +432,7 @@ cudaError_t launch_layer_norm(const LnParams& p, int is_bf16, int vec, int backw
         e = vec ? dispatch<float, 4>(p, backward, stream) : dispatch<float, 1>(p, backward, stream);
     }
     if (e != cudaSuccess || !backward || (!p.dweight && !p.dbias)) return e;
-    layer_norm_dw_kernel<<<dim3((p.dim + 31) / 32, 2), 256, 0, stream>>>(p.part, p.nparts, p.dim, p.dweight, p.dbias);
+    layer_norm_dw_kernel<<<dim3((p.dim + 31) / 32, 2), 1024, 0, stream>>>(p.part, p.nparts, p.dim, p.dweight, p.dbias);
     return cudaGetLastError();
 }
 

@@ -32,7 +32,7 @@ struct LaRole {
     LaTensor a, b, c;
     void* out; int64_t o_sb, o_st, o_sh;
     int out_f32;          // out is float32 whatever the stream type (per-head partials)
-    int out_vec;          // out rows start on 16 bytes
+    int out_vec;          // out's rows start on 16 bytes and its strides fit a TMA
     int db, dc;           // channels of a and b; channels of c and out
     int reverse;
     float alpha, beta, sigma;
@@ -57,7 +57,7 @@ struct LaParams {
     LaRole role[3];
 };
 
-// TMA maps of every role's tensors: (channel, token, head, batch), boxes of 64 channels x 128 tokens
+// TMA maps of every role's tensors: (channel, token, head, batch), boxes of 128 bytes x 128 tokens
 struct LaMaps {
     CUtensorMap a[3], b[3], c[3], o[3];
 };

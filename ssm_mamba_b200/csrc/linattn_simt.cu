@@ -301,20 +301,46 @@ cudaError_t launch_simt(const LaParams& p, int max_dc, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename T>
+// A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.
+constexpr int kGroupTokens = 16;
+template <typename T, int V>
 __global__ void __launch_bounds__(256) linattn_group_kernel(const __grid_constant__ LaGroupParams p) {
-    const int groups = p.heads / p.share;
-    const int64_t total = (int64_t)p.batch * p.seqlen * groups * p.d;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int c = (int)(i % p.d);
-        const int64_t bt = i / ((int64_t)p.d * groups);
-        const int g = (int)(i / p.d - bt * groups);
-        const float* s = p.src + (bt * p.heads + (int64_t)g * p.share) * p.d + c;
-        float sum = 0.f;
-        for (int k = 0; k < p.share; k++) sum += s[(int64_t)k * p.d];
-        const int64_t b = bt / p.seqlen, t = bt - b * p.seqlen;
-        static_cast<T*>(p.out)[b * p.o_sb + t * p.o_st + g * p.o_sh + c] = from_f<T>(sum);
+    const int groups = p.heads / p.share, dv = p.d / V, per = groups * dv;
+    const int64_t tokens = (int64_t)p.batch * p.seqlen, first = (int64_t)blockIdx.x * kGroupTokens;
+    const int64_t b0 = first / p.seqlen;
+    const int t0 = (int)(first - b0 * p.seqlen);
+    const int n = (int)(tokens - first < kGroupTokens ? tokens - first : kGroupTokens);
+    for (int i = threadIdx.x; i < n * per; i += 256) {
+        const int tl = i / per, pos = i - tl * per, g = pos / dv, c = (pos - g * dv) * V;
+        const float* s = p.src + ((first + tl) * p.heads + (int64_t)g * p.share) * p.d + c;
+        float sum[V] = {};
+        for (int k = 0; k < p.share; k++, s += p.d) {
+            if constexpr (V == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(s);
+                sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+            } else {
+                sum[0] += s[0];
+            }
+        }
+        int64_t b = b0;
+        int t = t0 + tl;
+        while (t >= p.seqlen) {
+            t -= p.seqlen;
+            b++;
+        }
+        T* out = static_cast<T*>(p.out) + b * p.o_sb + t * p.o_st + g * p.o_sh + c;
+#pragma unroll
+        for (int e = 0; e < V; e++) out[e] = from_f<T>(sum[e]);
     }
+}
+
+template <typename T>
+cudaError_t launch_group(const LaGroupParams& p, cudaStream_t stream) {
+    const int64_t tokens = (int64_t)p.batch * p.seqlen;
+    const unsigned grid = (unsigned)((tokens + kGroupTokens - 1) / kGroupTokens);
+    if (p.d % 4 == 0) linattn_group_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+    else linattn_group_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -329,13 +355,8 @@ cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t str
     return db <= 64 ? launch_simt<float, 64>(p, dc, stream) : launch_simt<float, 128>(p, dc, stream);
 }
 
-cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, int sms, cudaStream_t stream) {
-    const int64_t total = (int64_t)p.batch * p.seqlen * (p.heads / p.share) * p.d;
-    const int64_t want = (total + 255) / 256, most = (int64_t)sms * 16;
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    if (is_bf16) linattn_group_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-    else linattn_group_kernel<float><<<grid, 256, 0, stream>>>(p);
-    return cudaGetLastError();
+cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream) {
+    return is_bf16 ? launch_group<__nv_bfloat16>(p, stream) : launch_group<float>(p, stream);
 }
 
 }  // namespace ssm

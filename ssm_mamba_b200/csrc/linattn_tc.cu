@@ -393,12 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const LaRole& r = p.role[k.ri];
                 for (int c = c0; c < c1; c++, it++) {
                     if (!(fine = wait(kStaged + (it & 1), (it >> 1) & 1))) break;
-                    if (!r.out_f32 && r.out_vec) {
-                        const int t = chunk_first(k, r.reverse, c);
-#pragma unroll
-                        for (int i = 0; i < KC / 64; i++)
-                            if (i * 64 < r.dc)
-                                tma_store_4d(&maps.o[k.ri], smem + (it & 1) * L::STAGE + i * kPanel, i * 64, t, k.h, k.b);
+                    if (r.out_vec) {
+                        const int t = chunk_first(k, r.reverse, c), width = r.out_f32 ? 32 : 64;   // channels of a panel
+                        const unsigned char* src = smem + (it & 1) * L::STAGE;
+                        for (int x = 0; x < r.dc; x += width, src += kPanel)
+                            tma_store_4d(&maps.o[k.ri], src, x, t, k.h, k.b);
                         tma_store_commit();
                         tma_store_wait_read_all();
                     }
@@ -673,10 +672,10 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                         for (int e = 0; e < NO; e++) acc[e] = 0.f;
                 }
-                const bool tma = !r.out_f32 && r.out_vec;
-                // the tile is staged over a, and where that is not enough over b, which the update reads
-                if ((!tma || KC > KB) && !(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
-                if (tma) {
+                // the tile is staged over a, and where that is not enough over b and c, which the update reads
+                const bool bf16 = r.out_vec && !r.out_f32;
+                if ((!bf16 || KC > KB) && !(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
+                if (bf16) {
 #pragma unroll
                     for (int i = 0; i < NO; i += 8) {
                         const uint4 v = make_uint4(pack_bf16(acc[i], acc[i + 1]), pack_bf16(acc[i + 2], acc[i + 3]),
@@ -684,30 +683,35 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         const int oc = o0 + i;
                         *reinterpret_cast<uint4*>(st + (oc >> 6) * kPanel + swz128(row, (oc & 63) * 2)) = v;
                     }
-                    fence_proxy_async_smem();
                 } else {
-                    // float32 partials and rows a TMA cannot store: through the warp's own piece of the stage,
-                    // 16-byte pieces swizzled by the row, then row by row
-                    float* own = reinterpret_cast<float*>(st) + warp * 32 * NO;
-                    constexpr int M = 7;
+                    // float32: panels of 32 channels, for a TMA or for the loop below
 #pragma unroll
-                    for (int i = 0; i < NO; i += 4)
-                        *reinterpret_cast<float4*>(own + lane * NO + (((i >> 2) ^ (lane & M)) << 2)) =
+                    for (int i = 0; i < NO; i += 4) {
+                        const int oc = o0 + i;
+                        *reinterpret_cast<float4*>(st + (oc >> 5) * kPanel + swz128(row, (oc & 31) * 4)) =
                             make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                    }
+                }
+                if (!r.out_vec) {
+                    // rows that a TMA cannot store: a warp's 32 rows, one after the other
                     __syncwarp();
                     const int64_t at = k.b * r.o_sb + (int64_t)(chunk_first(k, reverse, c) + q * 32) * r.o_st +
                                        k.h * r.o_sh + o0;
                     const int cols = min(NO, r.dc - o0), rows = min(32, n - q * 32);
 #pragma unroll 1
-                    for (int i = lane; i < rows * NO; i += 32) {
-                        const int rw = i / NO, col = i % NO;
-                        const float x = own[rw * NO + (((col >> 2) ^ (rw & M)) << 2) + (col & 3)];
-                        if (col >= cols) continue;
-                        if (r.out_f32) static_cast<float*>(r.out)[at + rw * r.o_st + col] = x;
-                        else static_cast<__nv_bfloat16*>(r.out)[at + rw * r.o_st + col] = __float2bfloat16_rn(x);
+                    for (int rw = 0; rw < rows; rw++) {
+#pragma unroll
+                        for (int e = 0; e < NO; e += 32) {
+                            const int oc = o0 + e + lane;
+                            const float x = *reinterpret_cast<const float*>(st + (oc >> 5) * kPanel +
+                                                                            swz128(q * 32 + rw, (oc & 31) * 4));
+                            if (e + lane >= cols) continue;
+                            if (r.out_f32) static_cast<float*>(r.out)[at + rw * r.o_st + e + lane] = x;
+                            else static_cast<__nv_bfloat16*>(r.out)[at + rw * r.o_st + e + lane] = __float2bfloat16_rn(x);
+                        }
                     }
-                    fence_proxy_async_smem();
                 }
+                fence_proxy_async_smem();
                 tc_fence_before();
                 arrive(kStaged + (it & 1));
 
@@ -766,15 +770,17 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 }
             }
             if (ends) {
-                // tokens past the row's length
-                const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * KC;
+                // zeros for the tokens past the row's length, 16 bytes at a time where the rows allow it
+                const int es = r.out_f32 ? 4 : 2;
+                const int piece = r.out_vec && r.dc * es % 16 == 0 ? 16 : es, per = r.dc * es / piece;
+                const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * per;
+                char* dst = static_cast<char*>(r.out) + (k.b * r.o_sb + (int64_t)(k.tok0 + k.ntok) * r.o_st + k.h * r.o_sh) * es;
 #pragma unroll 1
                 for (int i = tid; i < total; i += kCompute) {
-                    const int t = k.ntok + i / KC, cc = i % KC;
-                    if (cc >= r.dc) continue;
-                    const int64_t at = k.b * r.o_sb + (int64_t)(k.tok0 + t) * r.o_st + k.h * r.o_sh + cc;
-                    if (r.out_f32) static_cast<float*>(r.out)[at] = 0.f;
-                    else static_cast<__nv_bfloat16*>(r.out)[at] = __float2bfloat16_rn(0.f);
+                    char* at = dst + (int64_t)(i / per) * r.o_st * es + i % per * piece;
+                    if (piece == 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+                    else if (piece == 4) *reinterpret_cast<float*>(at) = 0.f;
+                    else *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(0.f);
                 }
             }
         }

@@ -5,6 +5,7 @@
 // of RuntimeError; there is no CPU path -- non-CUDA tensors are rejected.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -743,6 +744,139 @@ std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& x, const std::optional<
     return {dx, dw, db};
 }
 
+// ---- linear attention and layer norm as differentiable functions -------------------------------
+// In C++: a call of these operators is short, and a Python autograd function would cost more than
+// its kernel at the sizes of a decode step.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::optional<at::Tensor> opt(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+at::Tensor unit_last_stride(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// Gradients that were asked for with a graph of their own: going through them is an error, not a zero.
+variable_list once_differentiable(const char* name, variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list some;
+    for (at::Tensor& g : grads)
+        if (g.defined()) some.push_back(g.detach().requires_grad_(true));
+    auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative",
+                                                               (int64_t)some.size());
+    some = (*err)(std::move(some));
+    size_t i = 0;
+    for (at::Tensor& g : grads)
+        if (g.defined()) g = some[i++];
+    return grads;
+}
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                 const at::Tensor& log_decay, const std::optional<at::Tensor>& initial_state,
+                                 const std::optional<at::Tensor>& lengths, double scale, bool want_last) {
+        std::vector<at::Tensor> r = linear_attn_fwd(q, k, v, log_decay, scale, initial_state, lengths, want_last);
+        ctx->save_for_backward({q, k, v, log_decay, initial_state.value_or(at::Tensor()), lengths.value_or(at::Tensor())});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["dinit"] = initial_state && initial_state->requires_grad();
+        ctx->set_materialize_grads(false);
+        if (!want_last) return {r[0]};
+        return {r[0], r[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const at::Tensor &q = s[0], &v = s[2], &decay = s[3];
+        at::Tensor dout = grads[0];
+        if (!dout.defined()) dout = at::zeros({q.size(0), q.size(1), decay.size(0), v.size(3)}, q.options());
+        at::Tensor dlast = grads.size() > 1 ? grads[1] : at::Tensor();
+        if (dlast.defined()) dlast = dlast.contiguous();
+        std::vector<at::Tensor> g = linear_attn_bwd(q, s[1], v, decay, ctx->saved_data["scale"].toDouble(), opt(s[4]),
+                                                    opt(s[5]), unit_last_stride(dout), opt(dlast),
+                                                    ctx->saved_data["dinit"].toBool());
+        return once_differentiable("linear_attention_fn", {g[0], g[1], g[2], at::Tensor(), g[3], at::Tensor(),
+                                                           at::Tensor(), at::Tensor()});
+    }
+};
+
+void check_la(const char* name, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+              const at::Tensor& log_decay) {
+    TORCH_CHECK_TYPE(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16, name,
+                     ": q must be float32 or bfloat16, got ", q.scalar_type());
+    TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), name,
+                     ": q, k and v must share a dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
+    TORCH_CHECK_VALUE(!log_decay.requires_grad(), name,
+                      ": log_decay is a constant of the layer and has no gradient; pass log_decay.detach()");
+    TORCH_CHECK(q.dim() > 0 && k.dim() > 0 && v.dim() > 0, name, ": q, k and v must not be scalars");
+}
+
+std::vector<at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                         const at::Tensor& log_decay, std::optional<double> scale,
+                                         const std::optional<at::Tensor>& initial_state,
+                                         const std::optional<at::Tensor>& lengths, bool want_last) {
+    check_la("linear_attention_fn", q, k, v, log_decay);
+    std::optional<at::Tensor> s0, len;
+    if (initial_state) {
+        TORCH_CHECK_TYPE(initial_state->scalar_type() == at::kFloat,
+                         "linear_attention_fn: initial_state must be float32, got ", initial_state->scalar_type());
+        s0 = initial_state->contiguous();
+    }
+    if (lengths) len = lengths->to(q.device(), at::kLong).contiguous();
+    const at::Tensor qc = unit_last_stride(q), kc = unit_last_stride(k), vc = unit_last_stride(v);
+    const at::Tensor g = log_decay.to(at::kFloat).contiguous();
+    const double sc = scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1)));
+    const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                                     (s0 && s0->requires_grad()));
+    if (!grad) return linear_attn_fwd(qc, kc, vc, g, sc, s0, len, want_last);
+    return LinearAttention::apply(qc, kc, vc, g, s0, len, sc, want_last);
+}
+
+at::Tensor linear_attention_update(const at::Tensor& state, const at::Tensor& q, const at::Tensor& k,
+                                   const at::Tensor& v, const at::Tensor& log_decay, std::optional<double> scale) {
+    check_la("linear_attention_update", q, k, v, log_decay);
+    return linear_attn_update(state, unit_last_stride(q), unit_last_stride(k), unit_last_stride(v),
+                              log_decay.to(at::kFloat).contiguous(),
+                              scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1))));
+}
+
+// x as (rows, dim) with unit element stride: a view where its strides allow
+at::Tensor as_rows(const at::Tensor& x) {
+    const int64_t dim = x.size(-1);
+    if (x.dim() == 2) return unit_last_stride(x);
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); i++) rows *= x.size(i);
+    return unit_last_stride(x.reshape({rows, dim}));
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                              const std::optional<at::Tensor>& bias, double eps) {
+        const at::Tensor rows = as_rows(x);
+        std::vector<at::Tensor> r = layer_norm_fwd(rows, weight, bias, eps, true);
+        ctx->save_for_backward({rows, weight.value_or(at::Tensor()), r[1], r[2]});
+        ctx->saved_data["shape"] = x.sizes();
+        ctx->saved_data["dw"] = weight && weight->requires_grad();
+        ctx->saved_data["db"] = bias && bias->requires_grad();
+        return r[0].view(x.sizes());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        std::vector<at::Tensor> g = layer_norm_bwd(s[0], opt(s[1]), s[2], s[3], as_rows(grads[0]),
+                                                   ctx->saved_data["dw"].toBool(), ctx->saved_data["db"].toBool());
+        return once_differentiable("layer_norm_fn",
+                                   {g[0].view(ctx->saved_data["shape"].toIntVector()), g[1], g[2], at::Tensor()});
+    }
+};
+
+at::Tensor layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                      const std::optional<at::Tensor>& bias, double eps) {
+    TORCH_CHECK_TYPE(x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16,
+                     "layer_norm_fn: x must be float32 or bfloat16, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm_fn: x must have at least one dimension");
+    std::optional<at::Tensor> w, b;
+    if (weight) w = weight->to(at::kFloat).contiguous();
+    if (bias) b = bias->to(at::kFloat).contiguous();
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad())))
+        return layer_norm_fwd(as_rows(x), w, b, eps, false)[0].view(x.sizes());
+    return LayerNorm::apply(x, w, b, eps);
+}
+
 int64_t check_device_error() {
     int code = 0;
     ssm_check_device_error(&code, at::cuda::getCurrentCUDAStream().stream());
@@ -763,11 +897,10 @@ PYBIND11_MODULE(_C, m) {
     m.def("conv1d_fwd", &conv1d_fwd, "causal depthwise conv1d (+ SiLU) forward");
     m.def("conv1d_bwd", &conv1d_bwd, "causal depthwise conv1d (+ SiLU) backward");
     m.def("conv1d_update", &conv1d_update, "causal depthwise conv1d (+ SiLU) decode step");
-    m.def("linear_attn_fwd", &linear_attn_fwd, "linear attention with a decay for each head, forward");
-    m.def("linear_attn_bwd", &linear_attn_bwd, "linear attention with a decay for each head, backward");
-    m.def("linear_attn_update", &linear_attn_update, "linear attention with a decay for each head, one decode step");
-    m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward");
-    m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward");
+    m.def("linear_attention", &linear_attention, "linear attention with a decay for each head, differentiable");
+    m.def("linear_attention_update", &linear_attention_update,
+          "linear attention with a decay for each head, one decode step");
+    m.def("layer_norm", &layer_norm, "layer norm, differentiable");
     m.def("ckpt_from_reference", &ckpt_from_reference, "compact checkpoints from reference chunk states");
     m.def("state_update", &state_update, "one decode step");
     m.def("ckpt_len", [](int64_t n) { return ssm_scan_ckpt_len(n); });
