@@ -1025,10 +1025,33 @@ static bool la_tma_ok(const LaTensor& t, int64_t L, int64_t heads, int64_t batch
     return t.vec && ok(L, t.st) && ok(heads, t.sh) && ok(batch, t.sb);
 }
 
+static LaTensor la_tensor(const ssm_linear_attn_args* a, const void* p, int64_t sb, int64_t st, int64_t sh,
+                          int64_t heads) {
+    const int64_t es = a->dtype == SSM_BF16 ? 2 : 4;
+    LaTensor t;
+    t.p = p; t.sb = sb; t.st = st; t.sh = sh; t.share = (int)(a->heads / heads);
+    t.vec = aligned16(p) && (a->batch == 1 || ((sb * es) & 15) == 0) && (a->seqlen == 1 || ((st * es) & 15) == 0) &&
+            (heads == 1 || ((sh * es) & 15) == 0);
+    return t;
+}
+
+// The tensor-core kernel takes bfloat16 tensors that a TMA can fetch; everything else runs on the
+// FP32 pipe.
+static bool la_uses_tc(const ssm_linear_attn_args* a, int backward) {
+    if (a->dtype != SSM_BF16) return false;
+    auto ok = [&](const void* p, int64_t sb, int64_t st, int64_t sh, int64_t heads) {
+        return la_tma_ok(la_tensor(a, p, sb, st, sh, heads), a->seqlen, heads, a->batch);
+    };
+    return ok(a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads) &&
+           ok(a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads) &&
+           ok(a->v, a->v_batch_stride, a->v_token_stride, a->v_head_stride, a->v_heads) &&
+           (!backward || ok(a->dout, a->dout_batch_stride, a->dout_token_stride, a->dout_head_stride, a->heads));
+}
+
 namespace {
 // Workspace: per role the segment states, then the per-head gradients of shared heads.
 struct LaPlan {
-    int nseg, seglen, split;
+    int tc, nseg, seglen, split;
     size_t seg[3], part[3], flags, handoff, bytes;   // byte offsets
 };
 }  // namespace
@@ -1038,17 +1061,19 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     memset(&pl, 0, sizeof(pl));
     const int nroles = backward ? 3 : 1;
     const int64_t rows = a->batch * a->heads * nroles;
-    if (a->dtype == SSM_BF16) {
+    pl.tc = la_uses_tc(a, backward);
+    if (pl.tc) {
         pl.nseg = la_plan_segments(rows, a->seqlen, sms, &pl.seglen);
     } else {
-        // the float32 kernel runs two or more smaller CTAs per SM: two per SM, of 512 tokens or more
-        int64_t n = (2 * (int64_t)sms + rows - 1) / rows;
-        n = n < a->seqlen / 512 ? n : a->seqlen / 512;
-        n = n < 1 ? 1 : n > 16 ? 16 : n;
-        pl.seglen = (int)(((a->seqlen + n - 1) / n + 127) / 128 * 128);
+        // four CTAs per SM (a CTA does 64 columns of the output), from one chunk of 64 tokens up
+        const int64_t wide = backward && a->dk > a->dv ? a->dk : a->dv, all = rows * ((wide + 63) / 64);
+        int64_t n = (4 * (int64_t)sms + all - 1) / all;
+        const int64_t chunks = (a->seqlen + 63) / 64;
+        n = n < chunks ? n : chunks;
+        pl.seglen = (int)((chunks + n - 1) / n * 64);
         pl.nseg = (int)((a->seqlen + pl.seglen - 1) / pl.seglen);
     }
-    pl.split = rows * pl.nseg > sms;
+    pl.split = pl.tc && rows * pl.nseg > sms;
     auto take = [&](size_t n) {
         const size_t at = pl.bytes;
         pl.bytes += (n + 255) / 256 * 256;
@@ -1057,7 +1082,7 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     if (pl.nseg > 1)
         for (int i = 0; i < nroles; i++)
             pl.seg[i] = take((size_t)a->batch * a->heads * pl.nseg * a->dk * a->dv * sizeof(float));
-    if (pl.split && a->dtype == SSM_BF16) {
+    if (pl.split) {
         pl.flags = take((size_t)(sms + 1) * sizeof(int));
         pl.handoff = take((size_t)(sms + 1) * 128 * 128 * sizeof(float));
     }
@@ -1068,16 +1093,6 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
                 pl.part[i] = take((size_t)a->batch * a->seqlen * a->heads * d[i] * sizeof(float));
     }
     return pl;
-}
-
-static LaTensor la_tensor(const ssm_linear_attn_args* a, const void* p, int64_t sb, int64_t st, int64_t sh,
-                          int64_t heads) {
-    const int64_t es = a->dtype == SSM_BF16 ? 2 : 4;
-    LaTensor t;
-    t.p = p; t.sb = sb; t.st = st; t.sh = sh; t.share = (int)(a->heads / heads);
-    t.vec = aligned16(p) && (a->batch == 1 || ((sb * es) & 15) == 0) && (a->seqlen == 1 || ((st * es) & 15) == 0) &&
-            (heads == 1 || ((sh * es) & 15) == 0);
-    return t;
 }
 
 size_t ssm_linear_attn_workspace_size(const ssm_linear_attn_args* a, int backward) {
@@ -1108,7 +1123,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
     p.batch = (int)a->batch; p.seqlen = (int)a->seqlen; p.heads = (int)a->heads;
     p.nseg = pl.nseg; p.seglen = pl.seglen;
     p.split = pl.split;
-    if (pl.split && a->dtype == SSM_BF16) {
+    if (pl.split) {
         p.flags = reinterpret_cast<int*>(ws + pl.flags);
         p.handoff = reinterpret_cast<float*>(ws + pl.handoff);
     }
@@ -1159,13 +1174,8 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.role[2].state0 = a->dlast_state;
     }
     const int is_bf16 = a->dtype == SSM_BF16;
-    bool tc = is_bf16 != 0;
-    for (int i = 0; i < p.nroles; i++) {
-        const LaRole& r = p.role[i];
-        for (const LaTensor* t : {&r.a, &r.b, &r.c}) tc = tc && la_tma_ok(*t, a->seqlen, H / t->share, a->batch);
-    }
     cudaError_t e;
-    if (tc) {
+    if (pl.tc) {
         if ((rc = get_encoder())) return rc;
         LaMaps maps;
         memset(&maps, 0, sizeof(maps));

@@ -1,19 +1,21 @@
 // Linear attention with a decay for each head on the FP32 pipe (every stream type, any sizes,
 // strides and head counts; the recurrence and its four uses are in linattn.h).
 //
-// Chunked form: a CTA owns one (batch row, head, segment) and a tile of 64 columns of c, and
-// walks the segment in chunks of 64 tokens.  The state tile (db x 64) stays in registers, with
-// a copy in shared memory for the product with a.  Per chunk, all in float32:
+// A CTA owns one (batch row, head, segment) and a tile of DC columns of c, and walks the segment in
+// chunks of 64 tokens.  The state tile (db x DC) stays in registers, with a copy in shared memory
+// for the product with a.  Per chunk, all in float32:
 //     P   = (A B^T) o W              64 x 64, W the decays of the causal triangle
 //     out = alpha P C + beta diag(w^.) A S
 //     S   = w^n S + sigma (diag(w^.) B)^T C
-// 256 threads as a 16 x 16 grid, each with a 4 x 4 tile of P and out and a (db / 16) x 4 tile
-// of S; the operands come from shared memory as 16-byte loads.  Splitting c (not b) keeps the
-// sum over b inside the CTA; the 64 x 64 scores are recomputed by each column tile.
+// 256 threads as a 16 x 16 grid, each with a 4 x 4 tile of P, a 4 x DC/16 tile of out and a
+// DB/16 x DC/16 tile of S; the operands come from shared memory as 16-byte loads.  Splitting c (not
+// b) keeps the sum over b inside the CTA; the scores are recomputed by each column tile.
 //
-// Few (batch, head) pairs leave SMs idle, so a long row is cut into segments: the STATE pass
-// leaves each segment's state from a zero start, and the main pass's CTAs fold the states of
-// the segments before theirs in order (the decay across n tokens is one factor w^n).
+// A chunk alone is a chain of loads, products and barriers that leaves the pipe idle, so a row is
+// cut into segments until there are several CTAs per SM: a first pass leaves each segment's state
+// from a zero start, a scan turns those into the states that the segments start from, and the
+// main pass runs all segments at once.  S is computed twice, a quarter more products; at
+// 2 x 1024 tokens of 24 heads of 64 forward and backward took 395 us with two segments.
 #include "common.cuh"
 #include "linattn.h"
 
@@ -22,14 +24,15 @@ namespace ssm {
 namespace {
 
 constexpr int kC = 64;         // tokens per chunk
-constexpr int kDc = 64;        // columns of c per CTA
 constexpr int kThreads = 256;
 
-template <int DB>
+template <int DB, int DC>
 struct SimtSmem {
     static constexpr int LDA = DB + 4;    // row strides: 16 bytes past a multiple of 128
-    static constexpr int LDC = kDc + 4;
-    float a[kC * LDA], b[kC * LDA], c[kC * LDC], s[DB * LDC], p[kC * LDC];
+    static constexpr int LDC = DC + 4;
+    static constexpr int LDP = kC + 4;
+    float b[kC * LDA], c[kC * LDC], s[DB * LDC];
+    float a[kC * (LDA > LDP ? LDA : LDP)];   // a, then P
     float w[kC + 1];                      // w^0 .. w^64
 };
 
@@ -63,14 +66,34 @@ __device__ __forceinline__ void load_tile(float* dst, const LaTensor& t, int b, 
     }
 }
 
-template <typename T, int DB, bool STATE>
+template <int N>
+__device__ __forceinline__ void load_row(const float* p, float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 x = lds128(p + i);
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+        }
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] = x.x; v[1] = x.y;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_row(float* p, const float (&v)[N]) {
+    static_assert(N == 2 || N == 4);
+    if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+}
+
+template <typename T, int DB, int DC, bool STATE>
 __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_constant__ LaParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    using Smem = SimtSmem<DB>;
-    constexpr int LDA = Smem::LDA, LDC = Smem::LDC, RS = DB / 16;
+    using Smem = SimtSmem<DB, DC>;
+    constexpr int LDA = Smem::LDA, LDC = Smem::LDC, LDP = Smem::LDP, RS = DB / 16, NC = DC / 16;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const LaRole& r = p.role[blockIdx.z];
-    const int col0 = blockIdx.y * kDc;
+    const int col0 = blockIdx.y * DC;
     if (col0 >= r.dc) return;
     // one CTA per (segment, batch row, head); heads vary fastest
     int64_t id = blockIdx.x;
@@ -80,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
     const int slot = (int)(id / p.batch);
     const int seg = r.reverse ? p.nseg - 1 - slot : slot;
     const int64_t bh = (int64_t)b * p.heads + h;
-    const int cols = min(kDc, r.dc - col0);
+    const int cols = min(DC, r.dc - col0);
     const int row_len = la_row_length(p, b);
     const int ntok = la_segment_tokens(p, row_len, seg);
     const int64_t tok0 = (int64_t)seg * p.seglen;
@@ -89,28 +112,18 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
 
     for (int i = tid; i <= kC; i += kThreads) sm.w[i] = exp2f(g2 * (float)i);
 
-    // state tile: rows ty * RS .. + RS, columns tx * 4 .. + 4
-    float s[RS][4];
-    auto valid = [&](int i, int j) { return ty * RS + i < r.db && tx * 4 + j < cols; };
+    // state tile: rows ty * RS .. + RS, columns tx * NC .. + NC; from the segment's start state, which the
+    // scan has left in its place, or from the initial state
+    float s[RS][NC];
+    auto valid = [&](int i, int j) { return ty * RS + i < r.db && tx * NC + j < cols; };
+    const float* start = !STATE && p.nseg > 1 ? r.seg + (bh * p.nseg + seg) * r.db * r.dc
+                         : !STATE && r.state0 ? r.state0 + bh * r.db * r.dc : nullptr;
+    const int64_t s_i = p.nseg > 1 ? r.dc : r.s_i, s_j = p.nseg > 1 ? 1 : r.s_j;
 #pragma unroll
     for (int i = 0; i < RS; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            s[i][j] = (!STATE && r.state0 && valid(i, j))
-                          ? r.state0[bh * r.db * r.dc + (int64_t)(ty * RS + i) * r.s_i + (col0 + tx * 4 + j) * r.s_j]
-                          : 0.f;
-    if (!STATE) {
-        for (int q = 0; q < slot; q++) {
-            const int sg = r.reverse ? p.nseg - 1 - q : q;
-            const float f = exp2f(g2 * (float)la_segment_tokens(p, row_len, sg));
-            const float* e = r.seg + (bh * p.nseg + sg) * r.db * r.dc;
-#pragma unroll
-            for (int i = 0; i < RS; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (valid(i, j)) s[i][j] = fmaf(f, s[i][j], e[(ty * RS + i) * r.dc + col0 + tx * 4 + j]);
-        }
-    }
+        for (int j = 0; j < NC; j++)
+            s[i][j] = start && valid(i, j) ? start[(ty * RS + i) * s_i + (col0 + tx * NC + j) * s_j] : 0.f;
 
     const int nchunk = (ntok + kC - 1) / kC;
     for (int it = 0; it < nchunk; it++) {
@@ -120,12 +133,11 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
         __syncthreads();                       // the previous chunk's readers are done
         if (!STATE) load_tile<T, DB, LDA>(sm.a, r.a, b, h, t0, n, 0, r.db);
         load_tile<T, DB, LDA>(sm.b, r.b, b, h, t0, n, 0, r.db);
-        load_tile<T, kDc, LDC>(sm.c, r.c, b, h, t0, n, col0, cols);
+        load_tile<T, DC, LDC>(sm.c, r.c, b, h, t0, n, col0, cols);
         if (!STATE) {
 #pragma unroll
             for (int i = 0; i < RS; i++)
-                *reinterpret_cast<float4*>(&sm.s[(ty * RS + i) * LDC + tx * 4]) =
-                    make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+                store_row<NC>(&sm.s[(ty * RS + i) * LDC + tx * NC], s[i]);
         }
         __syncthreads();
         if (!STATE) {
@@ -149,33 +161,23 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
                         acc[i][j] = fmaf(av[i].w, bv[j].w, acc[i][j]);
                     }
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int row = ty * 4 + i, col = tx + 16 * j;
-                    const int dist = r.reverse ? col - row : row - col;
-                    sm.p[row * LDC + col] = dist >= 0 ? r.alpha * acc[i][j] * sm.w[dist] : 0.f;
-                }
             // state part of the output
-            float o[4][4] = {};
+            float o[4][NC] = {};
 #pragma unroll 2
             for (int k = 0; k < DB; k += 4) {
-                float4 av[4], sv[4];
+                float4 av[4];
+                float sv[4][NC];
 #pragma unroll
                 for (int i = 0; i < 4; i++) av[i] = lds128(&sm.a[(ty * 4 + i) * LDA + k]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) sv[j] = lds128(&sm.s[(k + j) * LDC + tx * 4]);
+                for (int j = 0; j < 4; j++) load_row<NC>(&sm.s[(k + j) * LDC + tx * NC], sv[j]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float a4[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) {
-                        o[i][0] = fmaf(a4[kk], sv[kk].x, o[i][0]);
-                        o[i][1] = fmaf(a4[kk], sv[kk].y, o[i][1]);
-                        o[i][2] = fmaf(a4[kk], sv[kk].z, o[i][2]);
-                        o[i][3] = fmaf(a4[kk], sv[kk].w, o[i][3]);
-                    }
+                    for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                        for (int j = 0; j < NC; j++) o[i][j] = fmaf(a4[kk], sv[kk][j], o[i][j]);
                 }
             }
 #pragma unroll
@@ -184,45 +186,52 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
                 const int pos = r.reverse ? max(n - 1 - row, 0) : row + 1;
                 const float f = r.beta * sm.w[pos];
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[i][j] *= f;
+                for (int j = 0; j < NC; j++) o[i][j] *= f;
             }
-            __syncthreads();                   // p is complete
-            // causal part: the warp's rows are ty0 * 4 .. + 8 with ty0 = 2 * warp
+            __syncthreads();                   // a has been read: P goes over it
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int row = ty * 4 + i, col = tx + 16 * j;
+                    const int dist = r.reverse ? col - row : row - col;
+                    sm.a[row * LDP + col] = dist >= 0 ? r.alpha * acc[i][j] * sm.w[dist] : 0.f;
+                }
+            __syncthreads();                   // P is complete
+            // causal part: the warp's rows are 8 * warp .. + 8
             const int warp = tid >> 5;
             const int k_lo = r.reverse ? warp * 8 : 0, k_hi = r.reverse ? kC : warp * 8 + 8;
             for (int k = k_lo; k < k_hi; k += 4) {
-                float4 pv[4], cv[4];
+                float4 pv[4];
+                float cv[4][NC];
 #pragma unroll
-                for (int i = 0; i < 4; i++) pv[i] = lds128(&sm.p[(ty * 4 + i) * LDC + k]);
+                for (int i = 0; i < 4; i++) pv[i] = lds128(&sm.a[(ty * 4 + i) * LDP + k]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) cv[j] = lds128(&sm.c[(k + j) * LDC + tx * 4]);
+                for (int j = 0; j < 4; j++) load_row<NC>(&sm.c[(k + j) * LDC + tx * NC], cv[j]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float p4[4] = {pv[i].x, pv[i].y, pv[i].z, pv[i].w};
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) {
-                        o[i][0] = fmaf(p4[kk], cv[kk].x, o[i][0]);
-                        o[i][1] = fmaf(p4[kk], cv[kk].y, o[i][1]);
-                        o[i][2] = fmaf(p4[kk], cv[kk].z, o[i][2]);
-                        o[i][3] = fmaf(p4[kk], cv[kk].w, o[i][3]);
-                    }
+                    for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                        for (int j = 0; j < NC; j++) o[i][j] = fmaf(p4[kk], cv[kk][j], o[i][j]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int row = ty * 4 + i;
                 if (row >= n) continue;
-                const int64_t at = b * r.o_sb + (t0 + row) * r.o_st + h * r.o_sh + col0 + tx * 4;
+                const int64_t at = b * r.o_sb + (t0 + row) * r.o_st + h * r.o_sh + col0 + tx * NC;
                 if (r.out_f32) {
                     float* op = static_cast<float*>(r.out) + at;
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (tx * 4 + j < cols) op[j] = o[i][j];
+                    for (int j = 0; j < NC; j++)
+                        if (tx * NC + j < cols) op[j] = o[i][j];
                 } else {
                     T* op = static_cast<T*>(r.out) + at;
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (tx * 4 + j < cols) op[j] = from_f<T>(o[i][j]);
+                    for (int j = 0; j < NC; j++)
+                        if (tx * NC + j < cols) op[j] = from_f<T>(o[i][j]);
                 }
             }
         }
@@ -231,49 +240,36 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < RS; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[i][j] *= fn;
+            for (int j = 0; j < NC; j++) s[i][j] *= fn;
 #pragma unroll 4
         for (int k = 0; k < n; k++) {
             const float f = r.sigma * sm.w[r.reverse ? k + 1 : n - 1 - k];
-            float4 cv = lds128(&sm.c[k * LDC + tx * 4]);
-            cv.x *= f; cv.y *= f; cv.z *= f; cv.w *= f;
+            float cv[NC], bv[RS];
+            load_row<NC>(&sm.c[k * LDC + tx * NC], cv);
+            load_row<RS>(&sm.b[k * LDA + ty * RS], bv);
 #pragma unroll
-            for (int i4 = 0; i4 < RS; i4 += 4) {
-                const float4 bv = lds128(&sm.b[k * LDA + ty * RS + i4]);
-                const float b4[4] = {bv.x, bv.y, bv.z, bv.w};
+            for (int j = 0; j < NC; j++) cv[j] *= f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    s[i4 + i][0] = fmaf(b4[i], cv.x, s[i4 + i][0]);
-                    s[i4 + i][1] = fmaf(b4[i], cv.y, s[i4 + i][1]);
-                    s[i4 + i][2] = fmaf(b4[i], cv.z, s[i4 + i][2]);
-                    s[i4 + i][3] = fmaf(b4[i], cv.w, s[i4 + i][3]);
-                }
-            }
+            for (int i = 0; i < RS; i++)
+#pragma unroll
+                for (int j = 0; j < NC; j++) s[i][j] = fmaf(bv[i], cv[j], s[i][j]);
         }
     }
 
-    if (STATE) {
-        float* e = r.seg + (bh * p.nseg + seg) * r.db * r.dc;
+    if (STATE || (slot == p.nseg - 1 && r.state_out)) {
+        float* dst = STATE ? r.seg + (bh * p.nseg + seg) * r.db * r.dc : r.state_out + bh * r.db * r.dc;
+        const int64_t d_i = STATE ? r.dc : r.s_i, d_j = STATE ? 1 : r.s_j;
 #pragma unroll
         for (int i = 0; i < RS; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (valid(i, j)) e[(ty * RS + i) * r.dc + col0 + tx * 4 + j] = s[i][j];
-        return;
+            for (int j = 0; j < NC; j++)
+                if (valid(i, j)) dst[(ty * RS + i) * d_i + (col0 + tx * NC + j) * d_j] = s[i][j];
     }
-    if (slot == p.nseg - 1 && r.state_out) {
-#pragma unroll
-        for (int i = 0; i < RS; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (valid(i, j))
-                    r.state_out[bh * r.db * r.dc + (int64_t)(ty * RS + i) * r.s_i + (col0 + tx * 4 + j) * r.s_j] =
-                        s[i][j];
-    }
+    if (STATE) return;
     // tokens past the row's length
     const int seg_end = (int)min((int64_t)p.seglen, (int64_t)p.seqlen - tok0);
-    for (int i = tid; i < (seg_end - ntok) * kDc; i += kThreads) {
-        const int t = ntok + i / kDc, c = i % kDc;
+    for (int i = tid; i < (seg_end - ntok) * DC; i += kThreads) {
+        const int t = ntok + i / DC, c = i % DC;
         if (c >= cols) continue;
         const int64_t at = b * r.o_sb + (tok0 + t) * r.o_st + h * r.o_sh + col0 + c;
         if (r.out_f32) static_cast<float*>(r.out)[at] = 0.f;
@@ -281,24 +277,57 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
     }
 }
 
-template <typename T, int DB>
-cudaError_t launch_simt(const LaParams& p, int max_dc, cudaStream_t stream) {
-    constexpr int bytes = (int)sizeof(SimtSmem<DB>);
-    auto main_k = linattn_simt_kernel<T, DB, false>;
-    auto state_k = linattn_simt_kernel<T, DB, true>;
+// The segments' states from a zero start become the states they start from: thread = state element,
+// the segments in the order of walking, eight loads ahead of the fold.
+__global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant__ LaParams p) {
+    const LaRole& r = p.role[blockIdx.z];
+    const int e = blockIdx.y * 256 + threadIdx.x, size = r.db * r.dc;
+    if (e >= size) return;
+    const int64_t bh = blockIdx.x;
+    const int b = (int)(bh / p.heads), h = (int)(bh - (int64_t)b * p.heads);
+    const int row_len = la_row_length(p, b);
+    const float g2 = la_log2_decay(p.log_decay[h]);
+    float x = r.state0 ? r.state0[bh * size + (int64_t)(e / r.dc) * r.s_i + (e % r.dc) * r.s_j] : 0.f;
+    float* seg = r.seg + bh * p.nseg * size + e;
+    auto place = [&](int slot) { return r.reverse ? p.nseg - 1 - slot : slot; };
+    for (int s0 = 0; s0 < p.nseg; s0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = s0 + i < p.nseg - 1 ? seg[(int64_t)place(s0 + i) * size] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (s0 + i >= p.nseg) break;
+            const int s = place(s0 + i);
+            seg[(int64_t)s * size] = x;
+            x = fmaf(exp2f(g2 * (float)la_segment_tokens(p, row_len, s)), x, v[i]);
+        }
+    }
+}
+
+template <typename T, int DB, int DC>
+cudaError_t launch_simt(const LaParams& p, int max_db, int max_dc, cudaStream_t stream) {
+    constexpr int bytes = (int)sizeof(SimtSmem<DB, DC>);
+    auto main_k = linattn_simt_kernel<T, DB, DC, false>;
+    auto state_k = linattn_simt_kernel<T, DB, DC, true>;
     cudaError_t e = cudaFuncSetAttribute(main_k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(state_k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    const dim3 tiles(1, (max_dc + kDc - 1) / kDc, p.nroles);
+    const unsigned rows = (unsigned)(p.batch * p.heads), tiles = (max_dc + DC - 1) / DC;
     if (p.nseg > 1) {
-        // the last segment (in walking order) needs no state of its own
-        const dim3 g((unsigned)((int64_t)p.batch * p.heads * (p.nseg - 1)), tiles.y, tiles.z);
-        state_k<<<g, kThreads, bytes, stream>>>(p);
+        // the last segment (in walking order) feeds nobody
+        state_k<<<dim3(rows * (p.nseg - 1), tiles, p.nroles), kThreads, bytes, stream>>>(p);
+        linattn_scan_kernel<<<dim3(rows, (max_db * max_dc + 255) / 256, p.nroles), 256, 0, stream>>>(p);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    const dim3 g((unsigned)((int64_t)p.batch * p.heads * p.nseg), tiles.y, tiles.z);
-    main_k<<<g, kThreads, bytes, stream>>>(p);
+    main_k<<<dim3(rows * p.nseg, tiles, p.nroles), kThreads, bytes, stream>>>(p);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dispatch_simt(const LaParams& p, int db, int dc, cudaStream_t stream) {
+    if (db <= 32) return dc <= 32 ? launch_simt<T, 32, 32>(p, db, dc, stream) : launch_simt<T, 32, 64>(p, db, dc, stream);
+    if (db <= 64) return dc <= 32 ? launch_simt<T, 64, 32>(p, db, dc, stream) : launch_simt<T, 64, 64>(p, db, dc, stream);
+    return dc <= 32 ? launch_simt<T, 128, 32>(p, db, dc, stream) : launch_simt<T, 128, 64>(p, db, dc, stream);
 }
 
 // A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.
@@ -351,8 +380,7 @@ cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t str
         db = p.role[i].db > db ? p.role[i].db : db;
         dc = p.role[i].dc > dc ? p.role[i].dc : dc;
     }
-    if (is_bf16) return db <= 64 ? launch_simt<__nv_bfloat16, 64>(p, dc, stream) : launch_simt<__nv_bfloat16, 128>(p, dc, stream);
-    return db <= 64 ? launch_simt<float, 64>(p, dc, stream) : launch_simt<float, 128>(p, dc, stream);
+    return is_bf16 ? dispatch_simt<__nv_bfloat16>(p, db, dc, stream) : dispatch_simt<float>(p, db, dc, stream);
 }
 
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream) {
