@@ -127,6 +127,54 @@ class StateUpdateArgs(ctypes.Structure):
     ]
 
 
+class LinearAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("seqlen", _i64), ("heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("q_heads", _i64), ("k_heads", _i64), ("v_heads", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _p), ("q_batch_stride", _i64), ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("k", _p), ("k_batch_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v", _p), ("v_batch_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("log_decay", _p), ("initial_state", _p), ("length", _p),
+        ("out", _p), ("out_batch_stride", _i64), ("out_token_stride", _i64), ("out_head_stride", _i64),
+        ("last_state", _p),
+        ("dout", _p), ("dout_batch_stride", _i64), ("dout_token_stride", _i64), ("dout_head_stride", _i64),
+        ("dlast_state", _p),
+        ("dq", _p), ("dq_batch_stride", _i64), ("dq_token_stride", _i64), ("dq_head_stride", _i64),
+        ("dk_", _p), ("dk_batch_stride", _i64), ("dk_token_stride", _i64), ("dk_head_stride", _i64),
+        ("dv_", _p), ("dv_batch_stride", _i64), ("dv_token_stride", _i64), ("dv_head_stride", _i64),
+        ("dinitial_state", _p),
+    ]
+
+
+class LinearAttnUpdateArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("q_heads", _i64), ("k_heads", _i64), ("v_heads", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _p), ("q_batch_stride", _i64), ("q_head_stride", _i64),
+        ("k", _p), ("k_batch_stride", _i64), ("k_head_stride", _i64),
+        ("v", _p), ("v_batch_stride", _i64), ("v_head_stride", _i64),
+        ("log_decay", _p),
+        ("state", _p), ("state_batch_stride", _i64), ("state_head_stride", _i64), ("state_k_stride", _i64),
+        ("out", _p), ("out_batch_stride", _i64), ("out_head_stride", _i64),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64),
+        ("dtype", _i32), ("eps", ctypes.c_float),
+        ("x", _p), ("x_row_stride", _i64),
+        ("weight", _p), ("bias", _p),
+        ("y", _p), ("y_row_stride", _i64),
+        ("mean", _p), ("rstd", _p),
+        ("dy", _p), ("dy_row_stride", _i64),
+        ("dx", _p), ("dx_row_stride", _i64),
+        ("dweight", _p), ("dbias", _p),
+    ]
+
+
 _lib = None
 
 
@@ -169,6 +217,19 @@ def lib() -> ctypes.CDLL:
         L.ssm_conv1d_bwd.restype = ctypes.c_int
         L.ssm_conv1d_update.argtypes = [ctypes.POINTER(Conv1dArgs), _p]
         L.ssm_conv1d_update.restype = ctypes.c_int
+        L.ssm_linear_attn_workspace_size.argtypes = [ctypes.POINTER(LinearAttnArgs), ctypes.c_int]
+        L.ssm_linear_attn_workspace_size.restype = ctypes.c_size_t
+        for f in (L.ssm_linear_attn_fwd, L.ssm_linear_attn_bwd):
+            f.argtypes = [ctypes.POINTER(LinearAttnArgs), _p, ctypes.c_size_t, _p]
+            f.restype = ctypes.c_int
+        L.ssm_linear_attn_update.argtypes = [ctypes.POINTER(LinearAttnUpdateArgs), _p]
+        L.ssm_linear_attn_update.restype = ctypes.c_int
+        L.ssm_layer_norm_fwd.argtypes = [ctypes.POINTER(LayerNormArgs), _p]
+        L.ssm_layer_norm_fwd.restype = ctypes.c_int
+        L.ssm_layer_norm_bwd_workspace_size.argtypes = [ctypes.POINTER(LayerNormArgs)]
+        L.ssm_layer_norm_bwd_workspace_size.restype = ctypes.c_size_t
+        L.ssm_layer_norm_bwd.argtypes = [ctypes.POINTER(LayerNormArgs), _p, ctypes.c_size_t, _p]
+        L.ssm_layer_norm_bwd.restype = ctypes.c_int
         L.ssm_check_device_error.argtypes = [ctypes.POINTER(ctypes.c_int), _p]
         L.ssm_check_device_error.restype = ctypes.c_int
         L.ssm_exp2_compare.argtypes = [_p, _p, _p, _i64, _p]
@@ -407,6 +468,84 @@ def call_conv1d_update(args: Conv1dArgs, stream=None):
     _check(lib().ssm_conv1d_update(ctypes.byref(args), stream if stream is not None else _stream()))
 
 
+def fill_linear_attn(q, k, v, log_decay, scale, initial_state=None, length=None, out=None, last_state=None, dout=None,
+                     dlast_state=None, dq=None, dk=None, dv=None, dinitial_state=None) -> LinearAttnArgs:
+    """q, k, v, out and their gradients: (batch, seqlen, heads, channels); states: (batch, heads,
+    dk, dv) float32 contiguous; log_decay: (heads,) float32."""
+    a = LinearAttnArgs()
+    a.batch, a.seqlen, a.heads = q.shape[0], q.shape[1], log_decay.shape[0]
+    a.dk, a.dv = q.shape[3], v.shape[3]
+    a.q_heads, a.k_heads, a.v_heads = q.shape[2], k.shape[2], v.shape[2]
+    a.dtype, a.scale = _dtype_code(q), float(scale)
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+        if t is not None:
+            setattr(a, name + "_" if name in ("dk", "dv") else name, _t(t))
+            for i, d in enumerate(("batch", "token", "head")):
+                setattr(a, f"{name}_{d}_stride", t.stride(i))
+    a.log_decay, a.initial_state, a.length = _t(log_decay), _t(initial_state), _t(length)
+    a.last_state, a.dlast_state, a.dinitial_state = _t(last_state), _t(dlast_state), _t(dinitial_state)
+    return a
+
+
+def call_linear_attn(args: LinearAttnArgs, backward=False, workspace=None, stream=None):
+    """ssm_linear_attn_fwd, or ssm_linear_attn_bwd; allocates the workspace with torch when none
+    is given."""
+    n = lib().ssm_linear_attn_workspace_size(ctypes.byref(args), int(backward))
+    if workspace is None:
+        import torch
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    fn = lib().ssm_linear_attn_bwd if backward else lib().ssm_linear_attn_fwd
+    _check(fn(ctypes.byref(args), _t(workspace), workspace.numel(), stream if stream is not None else _stream()))
+
+
+def fill_linear_attn_update(state, q, k, v, log_decay, scale, out) -> LinearAttnUpdateArgs:
+    a = LinearAttnUpdateArgs()
+    a.batch, a.heads, a.dk, a.dv = state.shape
+    a.q_heads, a.k_heads, a.v_heads = q.shape[1], k.shape[1], v.shape[1]
+    a.dtype, a.scale = _dtype_code(q), float(scale)
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        setattr(a, name, _t(t))
+        setattr(a, name + "_batch_stride", t.stride(0))
+        setattr(a, name + "_head_stride", t.stride(1))
+    a.log_decay, a.state = _t(log_decay), _t(state)
+    a.state_batch_stride, a.state_head_stride, a.state_k_stride = state.stride(0), state.stride(1), state.stride(2)
+    return a
+
+
+def call_linear_attn_update(args: LinearAttnUpdateArgs, stream=None):
+    _check(lib().ssm_linear_attn_update(ctypes.byref(args), stream if stream is not None else _stream()))
+
+
+def fill_layer_norm(x, eps, weight=None, bias=None, y=None, mean=None, rstd=None, dy=None, dx=None, dweight=None,
+                    dbias=None) -> LayerNormArgs:
+    """x, y, dy, dx: (rows, dim) with unit element stride; the rest float32."""
+    a = LayerNormArgs()
+    a.rows, a.dim = x.shape
+    a.dtype, a.eps = _dtype_code(x), float(eps)
+    for name, t in (("x", x), ("y", y), ("dy", dy), ("dx", dx)):
+        if t is not None:
+            setattr(a, name, _t(t))
+            setattr(a, name + "_row_stride", t.stride(0))
+    a.weight, a.bias, a.mean, a.rstd = _t(weight), _t(bias), _t(mean), _t(rstd)
+    a.dweight, a.dbias = _t(dweight), _t(dbias)
+    return a
+
+
+def call_layer_norm_fwd(args: LayerNormArgs, stream=None):
+    _check(lib().ssm_layer_norm_fwd(ctypes.byref(args), stream if stream is not None else _stream()))
+
+
+def call_layer_norm_bwd(args: LayerNormArgs, workspace=None, stream=None):
+    n = lib().ssm_layer_norm_bwd_workspace_size(ctypes.byref(args))
+    if n == 0:
+        raise SsmError(SSM_ERR_INVALID, lib().ssm_last_error().decode())
+    if workspace is None:
+        import torch
+        workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
+    _check(lib().ssm_layer_norm_bwd(ctypes.byref(args), _t(workspace), workspace.numel(),
+                                    stream if stream is not None else _stream()))
+
+
 def check_device_error(stream=None) -> int:
     code = ctypes.c_int(0)
     lib().ssm_check_device_error(ctypes.byref(code), stream if stream is not None else _stream())
@@ -416,4 +555,5 @@ def check_device_error(stream=None) -> int:
 def struct_sizes() -> Dict[str, int]:
     return {"fwd": ctypes.sizeof(ScanFwdArgs), "bwd": ctypes.sizeof(ScanBwdArgs),
             "update": ctypes.sizeof(StateUpdateArgs), "carry": ctypes.sizeof(CarryArgs),
-            "conv1d": ctypes.sizeof(Conv1dArgs)}
+            "conv1d": ctypes.sizeof(Conv1dArgs), "linear_attn": ctypes.sizeof(LinearAttnArgs),
+            "linear_attn_update": ctypes.sizeof(LinearAttnUpdateArgs), "layer_norm": ctypes.sizeof(LayerNormArgs)}
