@@ -48,7 +48,8 @@ cudaError_t launch_conv1d(const ConvParams& p, int is_bf16, int width, int kind,
 cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width, float* dw, int64_t dw_sd,
                                  float* dbias, int sms, cudaStream_t stream);
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
-cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream);
+cudaError_t launch_linattn_simt(const LaParams& p, cudaStream_t stream);
+cudaError_t launch_linattn_pack(const LaPackParams& p, int even, cudaStream_t stream);
 cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream);
 cudaError_t launch_linattn_update(const LaUpdParams& p, int is_bf16, int vec, cudaStream_t stream);
@@ -1035,24 +1036,28 @@ static LaTensor la_tensor(const ssm_linear_attn_args* a, const void* p, int64_t 
     return t;
 }
 
-// The tensor-core kernel takes bfloat16 tensors that a TMA can fetch; everything else runs on the
-// FP32 pipe.
-static bool la_uses_tc(const ssm_linear_attn_args* a, int backward) {
-    if (a->dtype != SSM_BF16) return false;
-    auto ok = [&](const void* p, int64_t sb, int64_t st, int64_t sh, int64_t heads) {
-        return la_tma_ok(la_tensor(a, p, sb, st, sh, heads), a->seqlen, heads, a->batch);
-    };
-    return ok(a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads) &&
-           ok(a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads) &&
-           ok(a->v, a->v_batch_stride, a->v_token_stride, a->v_head_stride, a->v_heads) &&
-           (!backward || ok(a->dout, a->dout_batch_stride, a->dout_token_stride, a->dout_head_stride, a->heads));
+// q, k, v and (backward) dout with their head counts and channels
+struct LaInput {
+    LaTensor t;
+    int64_t heads, d;
+};
+static int la_inputs(const ssm_linear_attn_args* a, int backward, LaInput (&in)[4]) {
+    in[0] = {la_tensor(a, a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads), a->q_heads, a->dk};
+    in[1] = {la_tensor(a, a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads), a->k_heads, a->dk};
+    in[2] = {la_tensor(a, a->v, a->v_batch_stride, a->v_token_stride, a->v_head_stride, a->v_heads), a->v_heads, a->dv};
+    if (!backward) return 3;
+    in[3] = {la_tensor(a, a->dout, a->dout_batch_stride, a->dout_token_stride, a->dout_head_stride, a->heads), a->heads,
+             a->dv};
+    return 4;
 }
 
 namespace {
-// Workspace: per role the segment states, then the per-head gradients of shared heads.
+// Workspace: per role the segment states, the states that CTAs hand on, the per-head gradients of
+// shared heads, and copies of the bfloat16 inputs that a TMA cannot fetch.
 struct LaPlan {
     int tc, nseg, seglen, split;
-    size_t seg[3], part[3], flags, handoff, bytes;   // byte offsets
+    size_t seg[3], part[3], flags, handoff, packed[4], bytes;   // byte offsets
+    bool pack[4];
 };
 }  // namespace
 
@@ -1061,7 +1066,7 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     memset(&pl, 0, sizeof(pl));
     const int nroles = backward ? 3 : 1;
     const int64_t rows = a->batch * a->heads * nroles;
-    pl.tc = la_uses_tc(a, backward);
+    pl.tc = a->dtype == SSM_BF16;            // float32 runs on the FP32 pipe
     if (pl.tc) {
         pl.nseg = la_plan_segments(rows, a->seqlen, sms, &pl.seglen);
     } else {
@@ -1085,6 +1090,14 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     if (pl.split) {
         pl.flags = take((size_t)(sms + 1) * sizeof(int));
         pl.handoff = take((size_t)(sms + 1) * 128 * 128 * sizeof(float));
+    }
+    if (pl.tc) {
+        LaInput in[4];
+        const int n = la_inputs(a, backward, in);
+        for (int i = 0; i < n; i++) {
+            pl.pack[i] = !la_tma_ok(in[i].t, a->seqlen, in[i].heads, a->batch);
+            if (pl.pack[i]) pl.packed[i] = take((size_t)a->batch * a->seqlen * in[i].heads * ((in[i].d + 7) / 8) * 16);
+        }
     }
     if (backward) {
         const int64_t heads[3] = {a->q_heads, a->v_heads, a->k_heads}, d[3] = {a->dk, a->dv, a->dk};
@@ -1128,9 +1141,23 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.handoff = reinterpret_cast<float*>(ws + pl.handoff);
     }
     p.log_decay = a->log_decay; p.length = a->length; p.err = di->err;
-    const LaTensor q = la_tensor(a, a->q, a->q_batch_stride, a->q_token_stride, a->q_head_stride, a->q_heads);
-    const LaTensor k = la_tensor(a, a->k, a->k_batch_stride, a->k_token_stride, a->k_head_stride, a->k_heads);
-    const LaTensor v = la_tensor(a, a->v, a->v_batch_stride, a->v_token_stride, a->v_head_stride, a->v_heads);
+    LaInput in[4];
+    const int nin = la_inputs(a, backward, in);
+    cudaError_t e;
+    for (int i = 0; i < nin; i++) {
+        if (!pl.pack[i]) continue;
+        LaPackParams k;
+        memset(&k, 0, sizeof(k));
+        k.src = in[i].t.p; k.sb = in[i].t.sb; k.st = in[i].t.st; k.sh = in[i].t.sh;
+        k.dst = ws + pl.packed[i];
+        k.batch = p.batch; k.seqlen = p.seqlen; k.heads = (int)in[i].heads; k.d = (int)in[i].d;
+        const int even = k.d % 2 == 0 && k.sb % 2 == 0 && k.st % 2 == 0 && k.sh % 2 == 0 &&
+                         (reinterpret_cast<uintptr_t>(k.src) & 3u) == 0;
+        if ((e = launch_linattn_pack(k, even, stream)) != cudaSuccess) return cuda_fail(e, "linear attention copy launch");
+        LaTensor& t = in[i].t;
+        t.p = k.dst; t.sh = (in[i].d + 7) / 8 * 8; t.st = t.sh * in[i].heads; t.sb = t.st * a->seqlen; t.vec = 1;
+    }
+    const LaTensor &q = in[0].t, &k = in[1].t, &v = in[2].t;
     const int dk = (int)a->dk, dv = (int)a->dv, H = (int)a->heads;
     auto role = [&](int i, const LaTensor& ra, const LaTensor& rb, const LaTensor& rc_, int db, int dc, int reverse,
                     bool transposed) {
@@ -1144,12 +1171,13 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
     // a gradient goes straight to its tensor, or as float32 per-head partials to the workspace
     auto dest = [&](int i, void* out, int64_t sb, int64_t st, int64_t sh, int64_t heads, int d) {
         LaRole& r = p.role[i];
+        r.out_f32 = heads != H || a->dtype == SSM_F32;
         if (heads == H) {
             const LaTensor t = la_tensor(a, out, sb, st, sh, heads);
             r.out = out; r.o_sb = sb; r.o_st = st; r.o_sh = sh;
             r.out_vec = la_tma_ok(t, a->seqlen, heads, a->batch);
         } else {
-            r.out = ws + pl.part[i]; r.out_f32 = 1; r.out_vec = d % 4 == 0;
+            r.out = ws + pl.part[i]; r.out_vec = d % 4 == 0;
             r.o_sh = d; r.o_st = (int64_t)H * d; r.o_sb = a->seqlen * r.o_st;
         }
     };
@@ -1160,7 +1188,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.role[0].state0 = a->initial_state;
         p.role[0].state_out = a->last_state;
     } else {
-        const LaTensor dout = la_tensor(a, a->dout, a->dout_batch_stride, a->dout_token_stride, a->dout_head_stride, H);
+        const LaTensor& dout = in[3].t;
         p.nroles = 3;
         role(0, dout, v, k, dv, dk, 0, true);
         dest(0, a->dq, a->dq_batch_stride, a->dq_token_stride, a->dq_head_stride, a->q_heads, dk);
@@ -1174,7 +1202,6 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.role[2].state0 = a->dlast_state;
     }
     const int is_bf16 = a->dtype == SSM_BF16;
-    cudaError_t e;
     if (pl.tc) {
         if ((rc = get_encoder())) return rc;
         LaMaps maps;
@@ -1194,11 +1221,12 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         const int kb = backward ? kmax : dk, kc = backward ? kmax : dv;
         e = launch_linattn_tc(p, maps, kb <= 64 ? 64 : 128, kc <= 64 ? 64 : 128, di->sms, stream);
     } else {
-        e = launch_linattn_simt(p, is_bf16, stream);
+        e = launch_linattn_simt(p, stream);
     }
     if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
+    const int64_t grad_heads[3] = {a->q_heads, a->v_heads, a->k_heads};
     for (int i = 0; backward && i < 3; i++) {
-        if (!p.role[i].out_f32) continue;
+        if (grad_heads[i] == H) continue;
         LaGroupParams g;
         memset(&g, 0, sizeof(g));
         g.src = static_cast<const float*>(p.role[i].out);
@@ -1274,12 +1302,18 @@ static LnParams ln_params(const ssm_layer_norm_args* a) {
     return p;
 }
 
-// 16-byte vectors: every row of each tensor and the weights start on 16 bytes, no partial vector
+// Widest access: 2 where every row of each tensor and the weights start on 16 bytes and there is no
+// partial vector, 1 for pairs of bfloat16 (rows on 4 bytes, weights on 8), else 0: single elements.
 static int ln_vec(const ssm_layer_norm_args* a, bool backward) {
     const int64_t es = a->dtype == SSM_BF16 ? 2 : 4;
-    auto ok = [&](const void* p, int64_t s) { return aligned16(p) && (a->rows == 1 || ((s * es) & 15) == 0); };
-    return (a->dim * es) % 16 == 0 && ok(a->x, a->x_row_stride) && aligned16(a->weight) && aligned16(a->bias) &&
-           (backward ? ok(a->dy, a->dy_row_stride) && ok(a->dx, a->dx_row_stride) : ok(a->y, a->y_row_stride));
+    auto fits = [&](uintptr_t bytes, uintptr_t wbytes) {
+        auto on = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+        auto ok = [&](const void* p, int64_t s) { return on(p, bytes) && (a->rows == 1 || (uintptr_t)(s * es) % bytes == 0); };
+        return (uintptr_t)(a->dim * es) % bytes == 0 && ok(a->x, a->x_row_stride) && on(a->weight, wbytes) &&
+               on(a->bias, wbytes) &&
+               (backward ? ok(a->dy, a->dy_row_stride) && ok(a->dx, a->dx_row_stride) : ok(a->y, a->y_row_stride));
+    };
+    return fits(16, 16) ? 2 : es == 2 && fits(4, 8) ? 1 : 0;
 }
 
 int ssm_layer_norm_fwd(const ssm_layer_norm_args* a, void* stream) {

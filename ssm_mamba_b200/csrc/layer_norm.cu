@@ -28,24 +28,33 @@ template <> struct Raw<__nv_bfloat16, 8> { uint4 r; __device__ void load(const _
         const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
         return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
     } };
+template <> struct Raw<__nv_bfloat16, 2> { uint32_t r; __device__ void load(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ float get(int i) const { return __uint_as_float((i & 1) ? (r & 0xffff0000u) : (r << 16)); } };
 template <> struct Raw<__nv_bfloat16, 1> { __nv_bfloat16 r; __device__ void load(const __nv_bfloat16* p) { r = *p; }
     __device__ float get(int) const { return __bfloat162float(r); } };
 
 template <int VT>
 __device__ __forceinline__ void load_f32(const float* p, float (&v)[VT]) {
-    if constexpr (VT == 1) v[0] = *p;
-    else
+    if constexpr (VT == 1) {
+        v[0] = *p;
+    } else if constexpr (VT == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] = x.x; v[1] = x.y;
+    } else {
 #pragma unroll
         for (int i = 0; i < VT; i += 4) {
             const float4 x = *reinterpret_cast<const float4*>(p + i);
             v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
         }
+    }
 }
 
 template <typename T, int VT>
 __device__ __forceinline__ void store_elems(T* p, const float (&v)[VT]) {
     if constexpr (VT == 1) {
         *p = from_f<T>(v[0]);
+    } else if constexpr (VT == 2) {
+        store_pair<T>(p, make_float2(v[0], v[1]));
     } else if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -427,9 +436,10 @@ cudaError_t launch_layer_norm(const LnParams& params, int is_bf16, int vec, int 
     if (p.dim > kLnMaxDim) {
         e = is_bf16 ? dispatch_wide<__nv_bfloat16>(p, backward, stream) : dispatch_wide<float>(p, backward, stream);
     } else if (is_bf16) {
-        e = vec ? dispatch<__nv_bfloat16, 8>(p, backward, stream) : dispatch<__nv_bfloat16, 1>(p, backward, stream);
+        e = vec == 2 ? dispatch<__nv_bfloat16, 8>(p, backward, stream)
+            : vec == 1 ? dispatch<__nv_bfloat16, 2>(p, backward, stream) : dispatch<__nv_bfloat16, 1>(p, backward, stream);
     } else {
-        e = vec ? dispatch<float, 4>(p, backward, stream) : dispatch<float, 1>(p, backward, stream);
+        e = vec == 2 ? dispatch<float, 4>(p, backward, stream) : dispatch<float, 1>(p, backward, stream);
     }
     if (e != cudaSuccess || !backward || (!p.dweight && !p.dbias)) return e;
     layer_norm_dw_kernel<<<dim3((p.dim + 31) / 32, 2), 1024, 0, stream>>>(p.part, p.nparts, p.dim, p.dweight, p.dbias);

@@ -31,7 +31,7 @@ struct LaTensor {
 struct LaRole {
     LaTensor a, b, c;
     void* out; int64_t o_sb, o_st, o_sh;
-    int out_f32;          // out is float32 whatever the stream type (per-head partials)
+    int out_f32;          // out is float32 (always so on the FP32 pipe; per-head partials)
     int out_vec;          // out's rows start on 16 bytes and its strides fit a TMA
     int db, dc;           // channels of a and b; channels of c and out
     int reverse;
@@ -67,6 +67,13 @@ struct LaGroupParams {
     const float* src;
     void* out; int64_t o_sb, o_st, o_sh;
     int batch, seqlen, heads, d, share;
+};
+
+// A bfloat16 tensor copied to rows of 8 ceil(d / 8) channels, contiguous
+struct LaPackParams {
+    const void* src; int64_t sb, st, sh;
+    void* dst;
+    int batch, seqlen, heads, d;
 };
 
 // One token: state = w state + k v^T in place, out = scale q^T state.

@@ -1,5 +1,5 @@
-// Linear attention with a decay for each head on the FP32 pipe (every stream type, any sizes,
-// strides and head counts; the recurrence and its four uses are in linattn.h).
+// Linear attention with a decay for each head on the FP32 pipe: float32 streams of any sizes,
+// strides and head counts (the recurrence and its four uses are in linattn.h).
 //
 // A CTA owns one (batch row, head, segment) and a tile of DC columns of c, and walks the segment in
 // chunks of 64 tokens.  The state tile (db x DC) stays in registers, with a copy in shared memory
@@ -36,33 +36,26 @@ struct SimtSmem {
     float w[kC + 1];                      // w^0 .. w^64
 };
 
-// rows [0, n) x channels [0, d) of a chunk into float32 rows of stride LD, zeros up to (kC, W)
-template <typename T, int W, int LD>
+// rows [0, n) x channels [0, d) of a chunk into rows of stride LD, zeros up to (kC, W)
+template <int W, int LD>
 __device__ __forceinline__ void load_tile(float* dst, const LaTensor& t, int b, int h, int64_t tok, int n, int col0,
                                           int d) {
-    const T* base = static_cast<const T*>(t.p) + b * t.sb + (int64_t)(h / t.share) * t.sh + tok * t.st + col0;
-    constexpr int V = 16 / sizeof(T);
-    if (t.vec) {
-        for (int i = threadIdx.x; i < kC * (W / V); i += kThreads) {
-            const int r = i / (W / V), c = (i - r * (W / V)) * V;
-            float v[V];
-            if (r < n && c + V <= d) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(base + r * t.st + c);
-                const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-                for (int j = 0; j < V; j++) v[j] = to_f(e[j]);
+    const float* base = static_cast<const float*>(t.p) + b * t.sb + (int64_t)(h / t.share) * t.sh + tok * t.st + col0;
+    for (int i = threadIdx.x; i < kC * (W / 4); i += kThreads) {
+        const int r = i / (W / 4), c = (i - r * (W / 4)) * 4;
+        const float* p = base + r * t.st + c;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n) {
+            if (t.vec && c + 4 <= d) {
+                v = *reinterpret_cast<const float4*>(p);
             } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) v[j] = (r < n && c + j < d) ? to_f(base[r * t.st + c + j]) : 0.f;
+                if (c < d) v.x = p[0];
+                if (c + 1 < d) v.y = p[1];
+                if (c + 2 < d) v.z = p[2];
+                if (c + 3 < d) v.w = p[3];
             }
-#pragma unroll
-            for (int j = 0; j < V; j++) dst[r * LD + c + j] = v[j];
         }
-    } else {
-        for (int i = threadIdx.x; i < kC * W; i += kThreads) {
-            const int r = i / W, c = i - r * W;
-            dst[r * LD + c] = (r < n && c < d) ? to_f(base[r * t.st + c]) : 0.f;
-        }
+        *reinterpret_cast<float4*>(dst + r * LD + c) = v;
     }
 }
 
@@ -86,7 +79,7 @@ __device__ __forceinline__ void store_row(float* p, const float (&v)[N]) {
     else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
 }
 
-template <typename T, int DB, int DC, bool STATE>
+template <int DB, int DC, bool STATE>
 __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_constant__ LaParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     using Smem = SimtSmem<DB, DC>;
@@ -131,9 +124,9 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
         const int64_t t0 = tok0 + (int64_t)ch * kC;
         const int n = min(kC, ntok - ch * kC);
         __syncthreads();                       // the previous chunk's readers are done
-        if (!STATE) load_tile<T, DB, LDA>(sm.a, r.a, b, h, t0, n, 0, r.db);
-        load_tile<T, DB, LDA>(sm.b, r.b, b, h, t0, n, 0, r.db);
-        load_tile<T, DC, LDC>(sm.c, r.c, b, h, t0, n, col0, cols);
+        if (!STATE) load_tile<DB, LDA>(sm.a, r.a, b, h, t0, n, 0, r.db);
+        load_tile<DB, LDA>(sm.b, r.b, b, h, t0, n, 0, r.db);
+        load_tile<DC, LDC>(sm.c, r.c, b, h, t0, n, col0, cols);
         if (!STATE) {
 #pragma unroll
             for (int i = 0; i < RS; i++)
@@ -222,17 +215,10 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
                 const int row = ty * 4 + i;
                 if (row >= n) continue;
                 const int64_t at = b * r.o_sb + (t0 + row) * r.o_st + h * r.o_sh + col0 + tx * NC;
-                if (r.out_f32) {
-                    float* op = static_cast<float*>(r.out) + at;
+                float* op = static_cast<float*>(r.out) + at;
 #pragma unroll
-                    for (int j = 0; j < NC; j++)
-                        if (tx * NC + j < cols) op[j] = o[i][j];
-                } else {
-                    T* op = static_cast<T*>(r.out) + at;
-#pragma unroll
-                    for (int j = 0; j < NC; j++)
-                        if (tx * NC + j < cols) op[j] = from_f<T>(o[i][j]);
-                }
+                for (int j = 0; j < NC; j++)
+                    if (tx * NC + j < cols) op[j] = o[i][j];
             }
         }
         // state update
@@ -271,9 +257,7 @@ __global__ void __launch_bounds__(kThreads) linattn_simt_kernel(const __grid_con
     for (int i = tid; i < (seg_end - ntok) * DC; i += kThreads) {
         const int t = ntok + i / DC, c = i % DC;
         if (c >= cols) continue;
-        const int64_t at = b * r.o_sb + (tok0 + t) * r.o_st + h * r.o_sh + col0 + c;
-        if (r.out_f32) static_cast<float*>(r.out)[at] = 0.f;
-        else static_cast<T*>(r.out)[at] = from_f<T>(0.f);
+        static_cast<float*>(r.out)[b * r.o_sb + (tok0 + t) * r.o_st + h * r.o_sh + col0 + c] = 0.f;
     }
 }
 
@@ -304,11 +288,11 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant
     }
 }
 
-template <typename T, int DB, int DC>
+template <int DB, int DC>
 cudaError_t launch_simt(const LaParams& p, int max_db, int max_dc, cudaStream_t stream) {
     constexpr int bytes = (int)sizeof(SimtSmem<DB, DC>);
-    auto main_k = linattn_simt_kernel<T, DB, DC, false>;
-    auto state_k = linattn_simt_kernel<T, DB, DC, true>;
+    auto main_k = linattn_simt_kernel<DB, DC, false>;
+    auto state_k = linattn_simt_kernel<DB, DC, true>;
     cudaError_t e = cudaFuncSetAttribute(main_k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(state_k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
@@ -323,11 +307,30 @@ cudaError_t launch_simt(const LaParams& p, int max_db, int max_dc, cudaStream_t 
     return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t dispatch_simt(const LaParams& p, int db, int dc, cudaStream_t stream) {
-    if (db <= 32) return dc <= 32 ? launch_simt<T, 32, 32>(p, db, dc, stream) : launch_simt<T, 32, 64>(p, db, dc, stream);
-    if (db <= 64) return dc <= 32 ? launch_simt<T, 64, 32>(p, db, dc, stream) : launch_simt<T, 64, 64>(p, db, dc, stream);
-    return dc <= 32 ? launch_simt<T, 128, 32>(p, db, dc, stream) : launch_simt<T, 128, 64>(p, db, dc, stream);
+// bfloat16 (batch, token, head, channel) of any strides into rows of whole 16-byte pieces, which a TMA
+// can fetch; thread = piece.  EVEN: rows start on 4 bytes and have an even number of channels.
+template <bool EVEN>
+__global__ void __launch_bounds__(256) linattn_pack_kernel(const __grid_constant__ LaPackParams p) {
+    const int per = (p.d + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)p.seqlen * p.heads * per) return;
+    const int64_t row = i / per;
+    const int c = (int)(i - row * per) * 8, t = (int)(row / p.heads), h = (int)(row - (int64_t)t * p.heads);
+    const int n = p.d - c < 8 ? p.d - c : 8;
+    for (int64_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
+        const uint16_t* src = static_cast<const uint16_t*>(p.src) + b * p.sb + t * p.st + h * p.sh + c;
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (EVEN) {
+                if (2 * e < n) w[e] = reinterpret_cast<const uint32_t*>(src)[e];
+            } else {
+                if (2 * e < n) w[e] = src[2 * e];
+                if (2 * e + 1 < n) w[e] |= (uint32_t)src[2 * e + 1] << 16;
+            }
+        }
+        reinterpret_cast<uint4*>(p.dst)[b * p.seqlen * p.heads * per + i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.
@@ -374,13 +377,23 @@ cudaError_t launch_group(const LaGroupParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_linattn_simt(const LaParams& p, int is_bf16, cudaStream_t stream) {
+cudaError_t launch_linattn_simt(const LaParams& p, cudaStream_t stream) {
     int db = 0, dc = 0;
     for (int i = 0; i < p.nroles; i++) {
         db = p.role[i].db > db ? p.role[i].db : db;
         dc = p.role[i].dc > dc ? p.role[i].dc : dc;
     }
-    return is_bf16 ? dispatch_simt<__nv_bfloat16>(p, db, dc, stream) : dispatch_simt<float>(p, db, dc, stream);
+    if (db <= 32) return dc <= 32 ? launch_simt<32, 32>(p, db, dc, stream) : launch_simt<32, 64>(p, db, dc, stream);
+    if (db <= 64) return dc <= 32 ? launch_simt<64, 32>(p, db, dc, stream) : launch_simt<64, 64>(p, db, dc, stream);
+    return dc <= 32 ? launch_simt<128, 32>(p, db, dc, stream) : launch_simt<128, 64>(p, db, dc, stream);
+}
+
+cudaError_t launch_linattn_pack(const LaPackParams& p, int even, cudaStream_t stream) {
+    const int64_t pieces = (int64_t)p.seqlen * p.heads * ((p.d + 7) / 8);
+    const dim3 grid((unsigned)((pieces + 255) / 256), p.batch < 65535 ? p.batch : 65535);
+    if (even) linattn_pack_kernel<true><<<grid, 256, 0, stream>>>(p);
+    else linattn_pack_kernel<false><<<grid, 256, 0, stream>>>(p);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream) {
