@@ -982,9 +982,10 @@ static int la_common(const char* name, const ssm_linear_attn_args* a) {
 }
 
 // Segments of a row, for `rows` independent (batch row, head, role) triples.  More segments fill more
-// SMs but cost a second reading of b and c (the state pass, about 0.45 of a chunk's time per chunk)
-// and a launch (about two chunks' time); measured on B200 at 40 rows of 1024 chunks.  The SMs share
-// the chunks evenly once there are more rows than SMs.
+// SMs but cost a second reading of b and c (the state pass, about 0.4 of a chunk's time per chunk,
+// of which decays that reach zero leave about half) and two launches (about six chunks' time);
+// measured on B200 at 40 rows of 1024 chunks.  The SMs share the chunks evenly once there are more
+// rows than SMs.
 static int la_plan_segments(int64_t rows, int64_t seqlen, int sms, int* seglen) {
     const int64_t chunks = (seqlen + 127) / 128;
     int best = 1;
@@ -992,7 +993,10 @@ static int la_plan_segments(int64_t rows, int64_t seqlen, int sms, int* seglen) 
     for (int n = 1; n <= 16 && (n == 1 || chunks >= 4 * n); n++) {   // at least 512 tokens each
         const int64_t len = (chunks + n - 1) / n, all = rows * n;
         double t = all <= sms ? (double)len : (double)(rows * chunks) / sms + 1;
-        if (n > 1) t += 0.45 * (double)(len * ((rows * (n - 1) + sms - 1) / sms)) + 2;
+        if (n > 1) {
+            const double shared = 0.5 * (double)(len * rows * (n - 1)) / sms;
+            t += 0.4 * (shared > len ? shared : (double)len) + 6;
+        }
         if (n == 1 || t < best_t) {
             best = n;
             best_t = t;

@@ -288,8 +288,18 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant
     }
 }
 
+}  // namespace
+
+cudaError_t launch_linattn_scan(const LaParams& p, cudaStream_t stream) {
+    const int size = p.role[0].db * p.role[0].dc;         // every role's states have dk x dv elements
+    linattn_scan_kernel<<<dim3((unsigned)(p.batch * p.heads), (size + 255) / 256, p.nroles), 256, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+namespace {
+
 template <int DB, int DC>
-cudaError_t launch_simt(const LaParams& p, int max_db, int max_dc, cudaStream_t stream) {
+cudaError_t launch_simt(const LaParams& p, int max_dc, cudaStream_t stream) {
     constexpr int bytes = (int)sizeof(SimtSmem<DB, DC>);
     auto main_k = linattn_simt_kernel<DB, DC, false>;
     auto state_k = linattn_simt_kernel<DB, DC, true>;
@@ -300,8 +310,7 @@ cudaError_t launch_simt(const LaParams& p, int max_db, int max_dc, cudaStream_t 
     if (p.nseg > 1) {
         // the last segment (in walking order) feeds nobody
         state_k<<<dim3(rows * (p.nseg - 1), tiles, p.nroles), kThreads, bytes, stream>>>(p);
-        linattn_scan_kernel<<<dim3(rows, (max_db * max_dc + 255) / 256, p.nroles), 256, 0, stream>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        if ((e = cudaGetLastError()) != cudaSuccess || (e = launch_linattn_scan(p, stream)) != cudaSuccess) return e;
     }
     main_k<<<dim3(rows * p.nseg, tiles, p.nroles), kThreads, bytes, stream>>>(p);
     return cudaGetLastError();
@@ -383,9 +392,9 @@ cudaError_t launch_linattn_simt(const LaParams& p, cudaStream_t stream) {
         db = p.role[i].db > db ? p.role[i].db : db;
         dc = p.role[i].dc > dc ? p.role[i].dc : dc;
     }
-    if (db <= 32) return dc <= 32 ? launch_simt<32, 32>(p, db, dc, stream) : launch_simt<32, 64>(p, db, dc, stream);
-    if (db <= 64) return dc <= 32 ? launch_simt<64, 32>(p, db, dc, stream) : launch_simt<64, 64>(p, db, dc, stream);
-    return dc <= 32 ? launch_simt<128, 32>(p, db, dc, stream) : launch_simt<128, 64>(p, db, dc, stream);
+    if (db <= 32) return dc <= 32 ? launch_simt<32, 32>(p, dc, stream) : launch_simt<32, 64>(p, dc, stream);
+    if (db <= 64) return dc <= 32 ? launch_simt<64, 32>(p, dc, stream) : launch_simt<64, 64>(p, dc, stream);
+    return dc <= 32 ? launch_simt<128, 32>(p, dc, stream) : launch_simt<128, 64>(p, dc, stream);
 }
 
 cudaError_t launch_linattn_pack(const LaPackParams& p, int even, cudaStream_t stream) {

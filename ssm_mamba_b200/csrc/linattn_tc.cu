@@ -36,6 +36,8 @@
 
 namespace ssm {
 
+cudaError_t launch_linattn_scan(const LaParams& p, cudaStream_t stream);
+
 namespace {
 
 constexpr int kT = 128;                    // tokens per chunk
@@ -482,12 +484,12 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + bar);
         };
-        auto ok = [&](bool v) { return __all_sync(0xffffffffu, v); };
+        auto await = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
         int it = 0, fixed = 0, meets = 0;
         // every compute warp has come this far
         auto meet = [&]() {
             arrive(kItem);
-            return ok(wait(kItem, meets++ & 1));
+            return await(kItem, meets++ & 1);
         };
         bool fine = true;
 
@@ -500,9 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             if (!(fine = meet())) break;              // nobody reads the last row's tables any more
             fill_decays(dec, g2, r.alpha, r.sigma, reverse, k.nchunk > 0 ? k.ntok - (k.nchunk - 1) * kT : 0);
 
-            // S^T before chunk c0: the state that the CTA before this one has published, or the initial state
-            // and then the segments before this one.  Through TMEM, so that the loop over columns stays a
-            // loop (registers have no index).
+            // S^T before chunk c0: the state that the CTA before this one has published, or the one that the
+            // scan has left for the segment, or the initial state.  Through TMEM, so that the loop over columns
+            // stays a loop (registers have no index).
             if (c0 > 0) {
                 const int* flag = p.flags + blockIdx.x;
                 int there = 0;
@@ -511,33 +513,27 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(flag) : "memory");
                     if (there || wait.gone(start)) break;
                 }
-                if (!(fine = ok(there != 0))) break;
+                if (!(fine = __all_sync(0xffffffffu, there != 0))) break;
             }
             float s[NS];
             if (s_on) {
-                const float* src0 = nullptr;
+                const float* src = nullptr;
                 int64_t step = r.s_i;
                 if (c0 > 0) {
-                    src0 = p.handoff + (int64_t)blockIdx.x * KB * KC + row;
+                    src = p.handoff + (int64_t)blockIdx.x * KB * KC + row;
                     step = KC;
-                } else if (r.state0 && row < r.dc) {
-                    src0 = r.state0 + k.bh * r.db * r.dc + row * r.s_j;
+                } else if (row < r.dc && p.nseg > 1) {
+                    src = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc + row;
+                    step = r.dc;
+                } else if (row < r.dc && r.state0) {
+                    src = r.state0 + k.bh * r.db * r.dc + row * r.s_j;
                 }
-                const int cols = c0 > 0 ? KB : r.db, folds = c0 > 0 ? 0 : k.slot;
-                const float* src = r.seg + k.bh * p.nseg * r.db * r.dc + row;
+                const int cols = c0 > 0 ? KB : r.db;
 #pragma unroll 1
                 for (int i = 0; i < NS; i += 8) {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = src0 && i0 + i + e < cols ? __ldcg(src0 + (i0 + i + e) * step) : 0.f;
-#pragma unroll 1
-                    for (int g = 0; g < folds; g++) {
-                        const int sg = reverse ? p.nseg - 1 - g : g;
-                        const float f = exp2f(g2 * (float)la_segment_tokens(p, k.row_len, sg));
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            x[e] = fmaf(f, x[e], row < r.dc && i0 + i + e < r.db ? src[(sg * r.db + i0 + i + e) * r.dc] : 0.f);
-                    }
+                    for (int e = 0; e < 8; e++) x[e] = src && i0 + i + e < cols ? __ldcg(src + (i0 + i + e) * step) : 0.f;
                     uint32_t v[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) v[e] = __float_as_uint(x[e]);
@@ -571,12 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const uint32_t par = it & 1;
                 const int n = chunk_count(k, reverse, c);
                 unsigned char* st = smem + (it & 1) * L::STAGE;
-                if (!(fine = ok(wait(kFull + (it & 1), (it >> 1) & 1)))) break;
+                if (!(fine = await(kFull + (it & 1), (it >> 1) & 1))) break;
                 if (n < kT) {
                     // rows past the length hold whatever the caller's padding holds
                     zero_rows(st, L::STAGE / kPanel, n, tid);
                     arrive(kFixed);
-                    if (!(fine = ok(wait(kFixed, fixed++ & 1)))) break;
+                    if (!(fine = await(kFixed, fixed++ & 1))) break;
                 }
                 // planes of C'^T, 64 tokens at a time, of which this warp does 32
                 auto put_planes = [&](int sub) {
@@ -600,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 put_planes(0);
 
                 // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
-                if (!(fine = ok(wait(kScores, par)))) break;
+                if (!(fine = await(kScores, par))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
@@ -641,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     tmem_st16(tm + kColScores + sb * 32, o);
                 }
                 // A S leaves TMEM
-                if (!(fine = ok(wait(kAS, par)))) break;
+                if (!(fine = await(kAS, par))) break;
                 tc_fence_after();
                 uint32_t as[NO];
                 tmem_ld<NO>(tm + kColO + o0, as);
@@ -649,12 +645,12 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 tc_fence_before();
                 arrive(kPReady);
 
-                if (!(fine = ok(wait(kCFree, par)))) break;
+                if (!(fine = await(kCFree, par))) break;
                 tc_fence_after();
                 put_planes(1);
 
                 // O
-                if (!(fine = ok(wait(kPC, par)))) break;
+                if (!(fine = await(kPC, par))) break;
                 tc_fence_after();
                 float acc[NO];
                 {
@@ -674,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 }
                 // the tile is staged over a, and where that is not enough over b and c, which the update reads
                 const bool bf16 = r.out_vec && !r.out_f32;
-                if ((!bf16 || KC > KB) && !(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
+                if ((!bf16 || KC > KB) && !(fine = await(kUpd + par, (it >> 1) & 1))) break;
                 if (bf16) {
 #pragma unroll
                     for (int i = 0; i < NO; i += 8) {
@@ -716,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 arrive(kStaged + (it & 1));
 
                 // the state after this chunk
-                if (!(fine = ok(wait(kUpd + par, (it >> 1) & 1)))) break;
+                if (!(fine = await(kUpd + par, (it >> 1) & 1))) break;
                 tc_fence_after();
                 if (s_on) {
                     const float fn = dec.pow[n];
@@ -918,16 +914,16 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + bar);
         };
-        auto ok = [&](bool v) { return __all_sync(0xffffffffu, v); };
+        auto await = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
         bool fine = true;
         for (int i = 0; i < nchunk; i++) {
             const int c = cb + i, n = count(c);
             unsigned char* st = smem + (i % kStages) * L::STAGE;
-            if (!(fine = ok(wait(kSbFull + i % kStages, (i / kStages) & 1)))) break;
+            if (!(fine = await(kSbFull + i % kStages, (i / kStages) & 1))) break;
             if (n < kT) {
                 zero_rows(st, L::STAGE / kPanel, n, tid);
                 arrive(kSbFixed);
-                if (!(fine = ok(wait(kSbFixed, 0)))) break;
+                if (!(fine = await(kSbFixed, 0))) break;
             }
             const float f = r.sigma * exp2f(g2 * (float)far(c));
 #pragma unroll 1
@@ -949,7 +945,7 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
                         w.z = __floats2bfloat162_rn(x - __low2float(w.v), y - __high2float(w.v));
                         return w;
                     }, pl);
-                if (i > 0 && !(fine = ok(wait(kSbDone + e, (i - 1) & 1)))) break;   // the buffer is free
+                if (i > 0 && !(fine = await(kSbDone + e, (i - 1) & 1))) break;   // the buffer is free
                 tc_fence_after();
                 if (s_on) {
 #pragma unroll
@@ -961,7 +957,7 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
             }
             if (!fine) break;
         }
-        if (fine && nchunk > 0) fine = ok(wait(kSbDone + 1, (nchunk - 1) & 1));
+        if (fine && nchunk > 0) fine = await(kSbDone + 1, (nchunk - 1) & 1);
         tc_fence_after();
         if (fine && s_on) {
             constexpr int NS = KB / 2;
@@ -994,7 +990,7 @@ cudaError_t launch_tc(const LaParams& p, const LaMaps& maps, int sms, cudaStream
                                  StateSmem<KB, KC>::BYTES);
         if (e != cudaSuccess) return e;
         linattn_tc_state_kernel<KB, KC><<<(unsigned)(rows * (p.nseg - 1)), kStateThreads, StateSmem<KB, KC>::BYTES, stream>>>(p, maps);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        if ((e = cudaGetLastError()) != cudaSuccess || (e = launch_linattn_scan(p, stream)) != cudaSuccess) return e;
     }
     e = cudaFuncSetAttribute(linattn_tc_kernel<KB, KC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              TcSmem<KB, KC>::BYTES);
