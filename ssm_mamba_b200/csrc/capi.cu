@@ -48,7 +48,7 @@ cudaError_t launch_conv1d(const ConvParams& p, int is_bf16, int width, int kind,
 cudaError_t launch_conv1d_reduce(const float* ws, int nparts, int dim, int width, float* dw, int64_t dw_sd,
                                  float* dbias, int sms, cudaStream_t stream);
 cudaError_t launch_conv1d_update(const ConvParams& p, int is_bf16, int width, int sms, cudaStream_t stream);
-cudaError_t launch_linattn_simt(const LaParams& p, cudaStream_t stream);
+cudaError_t launch_linattn_f32(const LaParams& p, cudaStream_t stream);
 cudaError_t launch_linattn_pack(const LaPackParams& p, int even, cudaStream_t stream);
 cudaError_t launch_linattn_tc(const LaParams& p, const LaMaps& maps, int kb, int kc, int sms, cudaStream_t stream);
 cudaError_t launch_linattn_group(const LaGroupParams& p, int is_bf16, cudaStream_t stream);
@@ -1007,6 +1007,26 @@ static int la_plan_segments(int64_t rows, int64_t seqlen, int sms, int* seglen) 
     return (int)((seqlen + len - 1) / len);
 }
 
+// The same for the float32 kernel, of whose CTAs `slots` run at a time, in chunks of 64 tokens: the
+// waves of a main pass, and two fifths of that for the pass for the states; its launch and the scan's
+// cost as much as half a chunk.
+static int la_plan_f32(int64_t ctas, int64_t seqlen, int64_t slots, int* seglen) {
+    const int64_t chunks = (seqlen + 63) / 64;
+    int64_t best = chunks;                     // chunks per segment
+    double best_t = 0;
+    for (int64_t n = 1; n <= chunks && (n == 1 || ctas * (n - 1) < 2 * slots); n++) {
+        const int64_t len = (chunks + n - 1) / n, segs = (chunks + len - 1) / len;
+        double t = (double)((ctas * segs + slots - 1) / slots * len);
+        if (segs > 1) t += 0.4 * (double)((ctas * (segs - 1) + slots - 1) / slots * len) + 0.5;
+        if (n == 1 || t < best_t) {
+            best = len;
+            best_t = t;
+        }
+    }
+    *seglen = (int)(best * 64);
+    return (int)((chunks + best - 1) / best);
+}
+
 // Map of a bfloat16 or float32 (batch, token, head, channel) tensor; box of 128 bytes of channels x
 // 128 tokens, 128-byte swizzle, zeros outside.
 static int la_encode(CUtensorMap* map, const void* ptr, int f32, int64_t d, int64_t L, int64_t heads, int64_t batch,
@@ -1070,17 +1090,13 @@ static LaPlan la_plan(const ssm_linear_attn_args* a, int backward, int sms) {
     memset(&pl, 0, sizeof(pl));
     const int nroles = backward ? 3 : 1;
     const int64_t rows = a->batch * a->heads * nroles;
-    pl.tc = a->dtype == SSM_BF16;            // float32 runs on the FP32 pipe
+    pl.tc = a->dtype == SSM_BF16;            // float32 has a kernel of its own
     if (pl.tc) {
         pl.nseg = la_plan_segments(rows, a->seqlen, sms, &pl.seglen);
     } else {
-        // four CTAs per SM (a CTA does 64 columns of the output), from one chunk of 64 tokens up
-        const int64_t wide = backward && a->dk > a->dv ? a->dk : a->dv, all = rows * ((wide + 63) / 64);
-        int64_t n = (4 * (int64_t)sms + all - 1) / all;
-        const int64_t chunks = (a->seqlen + 63) / 64;
-        n = n < chunks ? n : chunks;
-        pl.seglen = (int)((chunks + n - 1) / n * 64);
-        pl.nseg = (int)((a->seqlen + pl.seglen - 1) / pl.seglen);
+        // a CTA does 64 columns of the output and shares its SM with one other (channels past 64: none)
+        const int64_t db = backward && a->dv > a->dk ? a->dv : a->dk, dc = backward && a->dk > a->dv ? a->dk : a->dv;
+        pl.nseg = la_plan_f32(rows * ((dc + 63) / 64), a->seqlen, db > 64 ? sms : 2 * sms, &pl.seglen);
     }
     pl.split = pl.tc && rows * pl.nseg > sms;
     auto take = [&](size_t n) {
@@ -1225,7 +1241,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         const int kb = backward ? kmax : dk, kc = backward ? kmax : dv;
         e = launch_linattn_tc(p, maps, kb <= 64 ? 64 : 128, kc <= 64 ? 64 : 128, di->sms, stream);
     } else {
-        e = launch_linattn_simt(p, stream);
+        e = launch_linattn_f32(p, stream);
     }
     if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
     const int64_t grad_heads[3] = {a->q_heads, a->v_heads, a->k_heads};

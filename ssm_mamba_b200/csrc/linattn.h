@@ -31,7 +31,7 @@ struct LaTensor {
 struct LaRole {
     LaTensor a, b, c;
     void* out; int64_t o_sb, o_st, o_sh;
-    int out_f32;          // out is float32 (always so on the FP32 pipe; per-head partials)
+    int out_f32;          // out is float32 (float32 streams, per-head partials)
     int out_vec;          // out's rows start on 16 bytes and its strides fit a TMA
     int db, dc;           // channels of a and b; channels of c and out
     int reverse;
