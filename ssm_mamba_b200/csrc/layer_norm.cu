@@ -5,6 +5,10 @@
 // it in registers (E elements each), so the second pass of the variance and the output need no
 // second reading.  All sums are float32.
 //
+// Measured (32768 rows, forward and backward): 2564 float32 99 us (6.8 TB/s) and 170 (5.9); 2565 float32,
+// whose rows allow no vectors, 121 (5.6) and 187 (5.4); 2560 bfloat16 70 (4.8) and 116 (4.3), where
+// the conversions and sums of each element weigh twice as much against its bytes.
+//
 // Backward: a thread owns the same columns of every row it meets, so the sums of dw and db
 // stay in its registers over all rows of a CTA; each CTA leaves one partial row, and a second
 // kernel adds the partial rows in a fixed order (deterministic, no floating-point atomics).
@@ -94,7 +98,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* slot) {
     }
 }
 
-template <int TPR> constexpr int kRowsPerCta = TPR >= 128 ? 1 : 4;
+template <int TPR> constexpr int kRowsPerCta = TPR > 32 ? 1 : 4;
 
 template <typename T, int VT, int E, int TPR>
 __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_fwd_kernel(const __grid_constant__ LnParams p) {
@@ -155,32 +159,64 @@ __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_fwd_kernel(
     }
 }
 
+// Rows on their way through shared memory, cnt elements from p to `at`, by TPR threads.  Vectors of 16
+// bytes go each to the place where the same thread takes it up again.  Rows that allow none are copied
+// in aligned pieces of 16 bytes and read from their first element on once all threads' pieces
+// are there (32768 rows of 1601 bfloat16: 157 us with a copy per element, 111 so; 2565 float32: 235, 187).  The
+// first piece begins up to 15 bytes before the row, in the aligned 16 bytes that hold its first
+// element; the last one ends with the row.
+template <typename T, int VT, int E, int TPR>
+struct Flight {
+    static constexpr bool kWhole = VT * sizeof(T) < 16;
+    static constexpr int kBytes = E * TPR * (int)sizeof(T) + (kWhole ? 16 : 0);     // of a row's place
+    static __device__ int head(const T* p) { return kWhole ? (int)(reinterpret_cast<uintptr_t>(p) & 15) : 0; }
+    static __device__ void start(unsigned char* at, const T* p, int cnt) {
+        const int tid = threadIdx.x % TPR, end = head(p) + cnt * (int)sizeof(T);
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(p) - head(p);
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(at);
+#pragma unroll
+        for (int i = 0; i < (kBytes / 16 + TPR - 1) / TPR; i++) {
+            const int k = (tid + i * TPR) * 16;
+            if (k < end)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k), "l"(from + k),
+                             "r"(min(end - k, 16))
+                             : "memory");
+        }
+    }
+};
+
+// Backward: rows in flight per row in work, so that an SM has the 40 KB and more under way that HBM
+// needs; with one row ahead in registers 32768 float32 rows of 2565 took 255 us.
+constexpr int kAhead = 2;
+template <typename T, int VT, int E, int TPR>
+constexpr int kBwdBytes = (kAhead + 1) * kRowsPerCta<TPR> * (2 * Flight<T, VT, E, TPR>::kBytes + TPR / 32 * 8);
+
 template <typename T, int VT, int E, int TPR>
 __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(const __grid_constant__ LnParams p) {
-    constexpr int NV = E / VT, RPC = kRowsPerCta<TPR>;
+    constexpr int NV = E / VT, RPC = kRowsPerCta<TPR>, WARPS = TPR * RPC / 32;
+    using Rows = Flight<T, VT, E, TPR>;
     __shared__ float slots[2][2 * (TPR / 32)];
     __shared__ float fold[RPC > 1 ? RPC * TPR * VT : 1];
+    // [stage][x, dy][row], then [stage][warp] mean and rstd
+    extern __shared__ __align__(16) unsigned char flight[];
+    float2* stats = reinterpret_cast<float2*>(flight + (kAhead + 1) * 2 * RPC * Rows::kBytes);
     const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     float dw[NV][VT] = {}, db[NV][VT] = {};
-    // a row's inputs, fetched while the row before it is worked on
-    struct Fetched {
-        Raw<T, VT> x[NV], g[NV];
-        float mean, rstd;
-    };
-    auto fetch = [&](int64_t row, Fetched& f) {
-        if (row >= p.rows) return;
-        const T* x = static_cast<const T*>(p.x) + row * p.x_s;
-        const T* dy = static_cast<const T*>(p.dy) + row * p.dy_s;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (tid + i * TPR) * VT;
-            if (c < p.dim) {
-                f.x[i].load(x + c);
-                f.g[i].load(dy + c);
+    auto place = [&](int stage, int which) { return flight + ((stage * 2 + which) * RPC + sub) * Rows::kBytes; };
+    auto stat = [&](int stage) { return stats + stage * WARPS + threadIdx.x / 32; };
+    auto x_row = [&](int64_t row) { return static_cast<const T*>(p.x) + row * p.x_s; };
+    auto dy_row = [&](int64_t row) { return static_cast<const T*>(p.dy) + row * p.dy_s; };
+    auto fetch = [&](int64_t row, int stage) {
+        if (row < p.rows) {
+            Rows::start(place(stage, 0), x_row(row), p.dim);
+            Rows::start(place(stage, 1), dy_row(row), p.dim);
+            if (threadIdx.x % 32 == 0) {
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(stat(stage));
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(p.mean + row) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4), "l"(p.rstd + row) : "memory");
             }
         }
-        f.mean = p.mean[row];
-        f.rstd = p.rstd[row];
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // narrow vectors: the weights stay in registers too
     constexpr bool kKeep = VT < 8;
@@ -204,17 +240,28 @@ __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(
             for (int j = 0; j < VT; j++) w[j] = kKeep ? kept[i][j] : 1.f;
         }
     };
-    const int64_t step = (int64_t)gridDim.x * RPC;
-    int turn = 0;
-    Fetched now, next;
-    fetch((int64_t)blockIdx.x * RPC + sub, now);
-    for (int64_t row = (int64_t)blockIdx.x * RPC + sub; row < p.rows; row += step, turn ^= 1) {
-        fetch(row + step, next);
-        const float mean = now.mean, rstd = now.rstd;
+    const int64_t step = (int64_t)gridDim.x * RPC, first = (int64_t)blockIdx.x * RPC + sub;
+    int turn = 0, stage = 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) fetch(first + i * step, i);
+    for (int64_t row = first; row < p.rows; row += step, turn ^= 1, stage = stage == kAhead ? 0 : stage + 1) {
+        fetch(row + kAhead * step, stage == 0 ? kAhead : stage - 1);     // the stage of the row before
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+        if (Rows::kWhole && TPR > 32) __syncthreads();
+        else __syncwarp();                        // mean and rstd come by lane 0
+        const T* xs = reinterpret_cast<const T*>(place(stage, 0) + Rows::head(x_row(row)));
+        const T* gs = reinterpret_cast<const T*>(place(stage, 1) + Rows::head(dy_row(row)));
+        const float mean = stat(stage)->x, rstd = stat(stage)->y;
+        struct {
+            Raw<T, VT> x[NV], g[NV];
+        } now;
         float v[2] = {0.f, 0.f};                  // sum of c, sum of c h
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            if ((tid + i * TPR) * VT >= p.dim) continue;
+            const int c = (tid + i * TPR) * VT;
+            if (c >= p.dim) continue;
+            now.x[i].load(xs + c);
+            now.g[i].load(gs + c);
             float w[VT];
             weights(i, w);
 #pragma unroll
@@ -242,7 +289,6 @@ __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>) layer_norm_bwd_kernel(
             }
             store_elems<T, VT>(dx + c, o);
         }
-        now = next;
     }
     // one partial row per CTA: [cta][0] dw, [cta][1] db
     float* out = p.part + (int64_t)blockIdx.x * 2 * p.dim;
@@ -364,47 +410,81 @@ __global__ void __launch_bounds__(1024) layer_norm_dw_kernel(const float* part, 
 
 // CTAs of the backward: as many as fit on the SMs at once, no more than there are partial rows for
 template <typename K>
-int resident_ctas(K kernel, int threads, int most) {
+int resident_ctas(K kernel, int threads, int bytes, int most) {
     int dev = 0, sms = 0, occ = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, 0) != cudaSuccess || occ < 1)
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, bytes) != cudaSuccess || occ < 1)
         return most;
     return sms * occ < most ? sms * occ : most;
 }
 
 template <typename T, int VT, int E, int TPR>
-cudaError_t launch_rows(LnParams& p, int backward, cudaStream_t stream) {
+cudaError_t launch_fwd(const LnParams& p, cudaStream_t stream) {
     constexpr int RPC = kRowsPerCta<TPR>;
-    if (!backward) {
-        layer_norm_fwd_kernel<T, VT, E, TPR><<<(unsigned)((p.rows + RPC - 1) / RPC), TPR * RPC, 0, stream>>>(p);
-    } else {
-        static const int resident = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, 1 << 20);
-        if (p.nparts > resident) p.nparts = resident;
-        layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, 0, stream>>>(p);
-    }
+    layer_norm_fwd_kernel<T, VT, E, TPR><<<(unsigned)((p.rows + RPC - 1) / RPC), TPR * RPC, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+template <typename T, int VT, int E, int TPR>
+cudaError_t launch_bwd(LnParams& p, cudaStream_t stream) {
+    constexpr int RPC = kRowsPerCta<TPR>, bytes = kBwdBytes<T, VT, E, TPR>;
+    static const int resident = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, bytes, 1 << 20);
+    if (p.nparts > resident) p.nparts = resident;
+    layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, bytes, stream>>>(p);
     return cudaGetLastError();
 }
 
-// Elements per thread are kept to 32 as raw bfloat16 and to 16 as float32 or single elements: the
-// backward holds two rows and two sums per column.
+// Forward: what a thread holds is what it has in flight, so a row gets as few threads as can hold it
+// (32768 rows of 5120 bfloat16: 217 us with 512 threads of 16, 141 with 256 of 24; 700 float32: 32 with
+// 128 of 8, 27 with 32 of 24).  Single elements cost more instructions than they fill the pipes
+// with, and up to 4096 go to more threads (801 bfloat16: 60 us with 32 of 32, 40 with 128 of 8).
+template <typename T, int VT>
+cudaError_t dispatch_fwd(const LnParams& p, cudaStream_t stream) {
+    if (p.dim <= 256) return launch_fwd<T, VT, 8, 32>(p, stream);
+    if (p.dim <= 512) return launch_fwd<T, VT, 16, 32>(p, stream);
+    if constexpr (VT == 1) {
+        if (p.dim <= 1024) return launch_fwd<T, VT, 8, 128>(p, stream);
+        if (p.dim <= 2048) return launch_fwd<T, VT, 8, 256>(p, stream);
+        if (p.dim <= 256 * 12) return launch_fwd<T, VT, 12, 256>(p, stream);
+        if (p.dim <= 256 * 16) return launch_fwd<T, VT, 16, 256>(p, stream);
+    } else {
+        if (p.dim <= 768) return launch_fwd<T, VT, 24, 32>(p, stream);
+        if (p.dim <= 1024) return launch_fwd<T, VT, 32, 32>(p, stream);
+        if (p.dim <= 64 * 24) return launch_fwd<T, VT, 24, 64>(p, stream);
+        if (p.dim <= 64 * 32) return launch_fwd<T, VT, 32, 64>(p, stream);
+        if (p.dim <= 128 * 24) return launch_fwd<T, VT, 24, 128>(p, stream);
+        if (p.dim <= 128 * 32) return launch_fwd<T, VT, 32, 128>(p, stream);
+    }
+    if (p.dim <= 256 * 24) return launch_fwd<T, VT, 24, 256>(p, stream);
+    return launch_fwd<T, VT, 32, 256>(p, stream);
+}
+// Backward: up to 32 elements per thread as vectors of 16 bytes of bfloat16, else 16: there are two sums
+// per column as well.  What a row costs besides its elements favours few threads with many (2565
+// float32: 263 us with 512 of 6, 235 with 256 of 12; 5120 bfloat16: 369 with 512 of 16, 236 with 256 of 24).
+template <typename T, int VT>
+cudaError_t dispatch_bwd(LnParams& p, cudaStream_t stream) {
+    if (p.dim <= 256) return launch_bwd<T, VT, 8, 32>(p, stream);
+    if (p.dim <= 512) return launch_bwd<T, VT, 16, 32>(p, stream);
+    if constexpr (VT == 8) {
+        if (p.dim <= 768) return launch_bwd<T, VT, 24, 32>(p, stream);
+        if (p.dim <= 1024) return launch_bwd<T, VT, 16, 64>(p, stream);
+        if (p.dim <= 2048) return launch_bwd<T, VT, 16, 128>(p, stream);
+        if (p.dim <= 128 * 24) return launch_bwd<T, VT, 24, 128>(p, stream);
+        if (p.dim <= 4096) return launch_bwd<T, VT, 32, 128>(p, stream);
+        if (p.dim <= 256 * 24) return launch_bwd<T, VT, 24, 256>(p, stream);
+        return launch_bwd<T, VT, 32, 256>(p, stream);
+    } else {
+        if (p.dim <= 1024) return launch_bwd<T, VT, 16, 64>(p, stream);
+        if (p.dim <= 2048) return launch_bwd<T, VT, 16, 128>(p, stream);
+        if (p.dim <= 256 * 12) return launch_bwd<T, VT, 12, 256>(p, stream);
+        if (p.dim <= 4096) return launch_bwd<T, VT, VT == 4 ? 8 : 16, VT == 4 ? 512 : 256>(p, stream);
+        return launch_bwd<T, VT, 16, 512>(p, stream);
+    }
+}
 template <typename T, int VT>
 cudaError_t dispatch(LnParams& p, int backward, cudaStream_t stream) {
-    if (p.dim <= 256) return launch_rows<T, VT, 8, 32>(p, backward, stream);
-    if (p.dim <= 512) return launch_rows<T, VT, 16, 32>(p, backward, stream);
-    if constexpr (VT == 8) {
-        if (p.dim <= 768) return launch_rows<T, VT, 24, 32>(p, backward, stream);
-        if (p.dim <= 1024) return launch_rows<T, VT, 32, 32>(p, backward, stream);
-        if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
-        if (p.dim <= 128 * 24) return launch_rows<T, VT, 24, 128>(p, backward, stream);
-        if (p.dim <= 4096) return launch_rows<T, VT, 32, 128>(p, backward, stream);
-    } else {
-        if (p.dim <= 1024) return launch_rows<T, VT, 8, 128>(p, backward, stream);
-        if (p.dim <= 2048) return launch_rows<T, VT, 16, 128>(p, backward, stream);
-        if (p.dim <= 256 * 12) return launch_rows<T, VT, 12, 256>(p, backward, stream);
-        if (p.dim <= 4096) return launch_rows<T, VT, 16, 256>(p, backward, stream);
-    }
-    return launch_rows<T, VT, 16, 512>(p, backward, stream);
+    return backward ? dispatch_bwd<T, VT>(p, stream) : dispatch_fwd<T, VT>(p, stream);
 }
 
 template <typename T>
@@ -421,12 +501,13 @@ cudaError_t dispatch_wide(const LnParams& p, int backward, cudaStream_t stream) 
 
 }  // namespace
 
-// Partial rows of dw and db there is room for: one per CTA of the backward, at most four CTAs per
-// SM, none without a row; for wide rows 64 slices of the rows.
+// Partial rows of dw and db there is room for: one per CTA of the backward, none without a row, at most
+// four CTAs per SM, or eight of those with 64 threads (32768 rows of 801 bfloat16: 80 and 53 us); for wide
+// rows 64 slices of the rows.
 int layer_norm_parts(int64_t rows, int dim, int sms) {
     if (dim > kLnMaxDim) return (int)(rows < 64 ? rows : 64);
     const int rpc = dim <= 512 ? 4 : 1;
-    const int64_t ctas = (rows + rpc - 1) / rpc, most = (int64_t)sms * 4;
+    const int64_t ctas = (rows + rpc - 1) / rpc, most = (int64_t)sms * (dim <= 1024 ? 8 : 4);
     return (int)(ctas < most ? ctas : most);
 }
 
