@@ -15,6 +15,8 @@
 //
 // Rows of more than 8192 elements do not fit the registers: they are read again for each pass
 // (from L2), and dw and db get a pass of their own.
+#include <atomic>
+
 #include "common.cuh"
 #include "params.h"
 
@@ -408,16 +410,22 @@ __global__ void __launch_bounds__(1024) layer_norm_dw_kernel(const float* part, 
     if (lane == 0 && blockIdx.x * 32 + y < dim) out[blockIdx.x * 32 + y] = sum;
 }
 
-// CTAs of the backward: as many as fit on the SMs at once, no more than there are partial rows for
+// CTAs of the backward: as many as fit on the SMs of the current device at once.  The first call on a
+// device also lets the kernel have its shared memory there.
+constexpr int kDevices = 64;
 template <typename K>
-int resident_ctas(K kernel, int threads, int bytes, int most) {
+cudaError_t resident_ctas(K kernel, int threads, int bytes, std::atomic<int> (&known)[kDevices], int* ctas) {
     int dev = 0, sms = 0, occ = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-        cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, bytes) != cudaSuccess || occ < 1)
-        return most;
-    return sms * occ < most ? sms * occ : most;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < kDevices && (*ctas = known[dev].load(std::memory_order_acquire)) != 0) return cudaSuccess;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess ||
+        (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess ||
+        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, bytes)) != cudaSuccess)
+        return e;
+    *ctas = sms * (occ < 1 ? 1 : occ);
+    if (dev < kDevices) known[dev].store(*ctas, std::memory_order_release);
+    return cudaSuccess;
 }
 
 template <typename T, int VT, int E, int TPR>
@@ -429,7 +437,10 @@ cudaError_t launch_fwd(const LnParams& p, cudaStream_t stream) {
 template <typename T, int VT, int E, int TPR>
 cudaError_t launch_bwd(LnParams& p, cudaStream_t stream) {
     constexpr int RPC = kRowsPerCta<TPR>, bytes = kBwdBytes<T, VT, E, TPR>;
-    static const int resident = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, bytes, 1 << 20);
+    static std::atomic<int> known[kDevices];
+    int resident = 0;
+    cudaError_t e = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, bytes, known, &resident);
+    if (e != cudaSuccess) return e;
     if (p.nparts > resident) p.nparts = resident;
     layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, bytes, stream>>>(p);
     return cudaGetLastError();

@@ -177,3 +177,20 @@ def test_refusals(cuda):
                       (ValueError, lambda: layer_norm_fn(torch.zeros((), device=cuda)))]:
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 131, 776, 1023, 1602, 2565, 3500, 4104, 6143, 8191])
+def test_many_rows_between_nans(cuda, dim, dtype):
+    """Several rows per CTA, x and its gradient at different offsets from 16 bytes, NaN on either
+    side of every row."""
+    gen = torch.Generator(device=cuda).manual_seed(dim)
+
+    def among_nans(at):
+        t = torch.full((4000, dim + 16), math.nan, device=cuda, dtype=dtype)
+        t[:, at:at + dim] = torch.randn(4000, dim, generator=gen, device=cuda)
+        return t[:, at:at + dim]
+
+    w, b = (torch.randn(dim, generator=gen, device=cuda) for _ in range(2))
+    for at in ((8, 16), (5, 2)):
+        _both(among_nans(at[0]), w, b, 1e-5, among_nans(at[1]))
