@@ -2,7 +2,13 @@
 restatement: output, gradients, prompt-to-decode hand-over, decoding from a CUDA graph.
 Relative 2-norm tolerances: float32 1e-5 and gradients 5e-5 (two norms and two projections
 multiply the operators' 1e-5); bfloat16 1e-2 (seven roundings of 1.7e-3, one after each stage,
-and 4e-3 of the attention)."""
+and 4e-3 of the attention).
+
+The norm after the attention makes some gradients ill-conditioned whatever computes them: the first
+token's output is (q . k) v, whose direction does not depend on q . k, so the gradient with respect to
+q . k is a small difference divided by it.  With q . k near zero the roundings of the stages alone
+move the gradient of hidden by 2% and more (one random input in twelve in bfloat16), so gradients are
+allowed twice the error of a torch composition with the same roundings on top."""
 import pytest
 import torch
 import torch.nn.functional as F
@@ -35,8 +41,23 @@ def _ref(w, hidden, params, state=None, lengths=None):
     return hidden + F.linear(norm(o).flatten(-2) * F.silu(F.linear(x, gate)), out), last
 
 
+def _plain(w, hidden, params):
+    """The block with every stage exact inside and rounded to the stream type."""
+    nw, nb, qkv, gate, out = params
+    norm = lambda t: F.layer_norm(t.double(), (t.shape[-1],))  # noqa: E731
+    x = (norm(hidden) * nw + nb).to(hidden.dtype)
+    q, k, v = (t.double() for t in w.split(F.linear(x, qkv)))
+    o, _ = attention(q, k, v, w.log_decay, w.dk ** -0.5, None, None)
+    o = norm(o.to(hidden.dtype)).to(hidden.dtype)
+    return hidden + F.linear(o.flatten(-2) * F.silu(F.linear(x, gate)), out)
+
+
+def _error(a, b):
+    return float((a.detach().double() - b.detach().double()).norm() / b.detach().double().norm())
+
+
 def _near(a, b, rel, name=""):
-    err = float((a.detach().double() - b.detach().double()).norm() / b.detach().double().norm())
+    err = _error(a, b)
     assert err <= rel, (name, err)
 
 
@@ -56,8 +77,10 @@ def test_forward_and_gradients(cuda, dtype):
     want_out, _ = _ref(w, ref[0], ref[1:])
     want = torch.autograd.grad(want_out, ref, dout.double())
     _near(out, want_out, 1e-5 if dtype == F32 else 1e-2, "out")
-    for n, a, b in zip(["hidden"] + names, got, want):
-        _near(a, b, 5e-5 if dtype == F32 else 2e-2, n)
+    again = [hidden.clone().requires_grad_()] + [getattr(w, n) for n in names]
+    rounded = torch.autograd.grad(_plain(w, again[0], again[1:]), again, dout)
+    for n, a, b, c in zip(["hidden"] + names, got, want, rounded):
+        _near(a, b, (5e-5 if dtype == F32 else 2e-2) + 2 * _error(c, b), n)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
