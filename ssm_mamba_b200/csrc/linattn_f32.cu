@@ -14,9 +14,9 @@
 // the FMAs); tcgen05 takes tf32 operands from shared memory along K only and would need the split
 // tiles stored, more than a CTA has at 128 channels.  An infinity becomes a NaN when it is split.
 //
-// Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 246 us (329 us on FMAs); 11 x 94
-// tokens of 40 heads, 96 and 80 channels, forward, 147 us.  What bounds it is the latency of a
-// chunk's steps at 16 warps an SM: the tensor pipe is busy 28% of the time, issue 45%.
+// Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 211 us (325 us on FMAs); 11 x 94
+// tokens of 40 heads, 96 and 80 channels, forward, 128 us.  What bounds it is the latency of a
+// chunk's steps at 16 warps an SM: the tensor pipe is busy 30% of the time, issue 45%.
 //
 // Shared-memory rows are strided so that a fragment's 32 elements lie on different banks: 4 (mod
 // 32) for operands read along their rows, 8 for operands read across them; b, which is read both
@@ -72,13 +72,14 @@ __device__ __forceinline__ void load_tile(float* dst, const LaTensor& t, int b, 
     }
 }
 
-// x = hi + lo, hi a tf32; the unit reads the leading 11 bits of lo
+// x = hi + lo, hi a tf32 (rounded by integers: cvt.rna.tf32 made the training step below 239 instead of 221 us);
+// the unit reads the leading 11 bits of lo
 struct Split {
     uint32_t hi, lo;
 };
 __device__ __forceinline__ Split split(float x) {
     Split s;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.hi) : "f"(x));
+    s.hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     s.lo = __float_as_uint(x - __uint_as_float(s.hi));
     return s;
 }
@@ -91,30 +92,46 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A tile of 16 x 8, split: a(row 0..15, k 0..7) reads an element
+// Two tiles of 16 x 8, split: a(row 0..15, k 0..15) reads an element
 struct Rows {
-    Split f[4];
+    Split f[2][4];
 };
 template <typename A>
 __device__ __forceinline__ Rows rows(A a) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    return {{split(a(g, t)), split(a(g + 8, t)), split(a(g, t + 4)), split(a(g + 8, t + 4))}};
+    Rows r;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) r.f[i][e] = split(a(g + (e & 1) * 8, t + i * 8 + (e >> 1) * 4));
+    return r;
 }
-// c[j] += A B_j for N tiles of 16 x 8, 8 of the summed index: b(k, column of tile j) reads an element;
+// c[j] += A B_j for N tiles of 16 x 8, 16 of the summed index: b(k, column of tile j) reads an element;
 // live(j) (the same for the whole warp) says whether tile j is wanted.  The unit truncates its sums
 // (1.6e-6 of relative error over a layer's backward), so each one starts from zero and is added,
-// rounded, on the FMA pipe (1.9e-7).
+// rounded, on the FMA pipe (2.0e-7, and 1.9e-7 at 221 instead of 211 us if after every 8).
 template <int N, typename B, typename Live>
 __device__ __forceinline__ void product(float (&c)[N][4], const Rows& a, B b, Live live) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int j = 0; j < N; j++) {
         if (!live(j)) continue;
-        const Split b0 = split(b(t, j * 8 + g)), b1 = split(b(t + 4, j * 8 + g));
         float d[4] = {};
-        mma_tf32(d, a.f[0].lo, a.f[1].lo, a.f[2].lo, a.f[3].lo, b0.hi, b1.hi);
-        mma_tf32(d, a.f[0].hi, a.f[1].hi, a.f[2].hi, a.f[3].hi, b0.lo, b1.lo);
-        mma_tf32(d, a.f[0].hi, a.f[1].hi, a.f[2].hi, a.f[3].hi, b0.hi, b1.hi);
+        Split s[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const auto& f = a.f[i];
+            const Split b0 = split(b(t + 8 * i, j * 8 + g)), b1 = split(b(t + 8 * i + 4, j * 8 + g));
+            mma_tf32(d, f[0].lo, f[1].lo, f[2].lo, f[3].lo, b0.hi, b1.hi);
+            mma_tf32(d, f[0].hi, f[1].hi, f[2].hi, f[3].hi, b0.lo, b1.lo);
+            s[i][0] = b0;
+            s[i][1] = b1;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const auto& f = a.f[i];
+            mma_tf32(d, f[0].hi, f[1].hi, f[2].hi, f[3].hi, s[i][0].hi, s[i][1].hi);
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) c[j][e] += d[e];
     }
@@ -202,8 +219,8 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
             float acc[NP][4] = {}, o[NO][4] = {};
             // scores, of which the causal mask leaves a warp the tiles up to (reverse: from) its rows
             auto live = [&](int j) { return r.reverse ? n0 + 8 * j + 7 >= m0 : n0 + 8 * j <= m0 + 15; };
-#pragma unroll 2
-            for (int k = 0; k < DB; k += 8) {
+#pragma unroll 1
+            for (int k = 0; k < DB; k += 16) {
                 const Rows a = rows([&](int m, int i) { return sm.a[(m0 + m) * LDB + k + i]; });
                 product(acc, a, [&](int i, int c) { return sb[(n0 + c) * LDB + k + i]; }, live);
                 product(o, a, [&](int i, int c) { return sm.s[(k + i) * LDN + on0 + c]; }, all);   // the state's part
@@ -231,8 +248,8 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
             __syncthreads();                   // P is complete
             // causal part
             const int k_lo = r.reverse ? m0 : 0, k_hi = r.reverse ? kC : m0 + 16;
-#pragma unroll 2
-            for (int k = k_lo; k < k_hi; k += 8)
+#pragma unroll 1
+            for (int k = k_lo; k < k_hi; k += 16)
                 product(o, rows([&](int m, int i) { return sm.s[(m0 + m) * LDP + k + i]; }),
                         [&](int i, int c) { return sc[(k + i) * LDN + on0 + c]; }, all);
 #pragma unroll
@@ -258,12 +275,16 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
         for (int j = 0; j < NS; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) s[j][e] *= fn;
-        for (int k = 0; k < n; k += 8) {
-            // weights of the two tokens of this thread's elements; rows past n are zero
-            const int k0 = k + t, k1 = k + t + 4;
-            const float f0 = r.sigma * sm.w[r.reverse ? k0 + 1 : max(n - 1 - k0, 0)];
-            const float f1 = r.sigma * sm.w[r.reverse ? k1 + 1 : max(n - 1 - k1, 0)];
-            product(s, rows([&](int m, int i) { return sb[(k + i) * LDB + sm0 + m] * (i < 4 ? f0 : f1); }),
+#pragma unroll 1
+        for (int k = 0; k < n; k += 16) {
+            // weights of the tokens of this thread's elements; rows past n are zero
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = k + t + 4 * i;
+                f[i] = r.sigma * sm.w[r.reverse ? at + 1 : max(n - 1 - at, 0)];
+            }
+            product(s, rows([&](int m, int i) { return sb[(k + i) * LDB + sm0 + m] * f[i >> 2]; }),
                     [&](int i, int c) { return sc[(k + i) * LDN + sn0 + c]; }, all);
         }
     }
