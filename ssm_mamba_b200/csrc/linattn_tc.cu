@@ -111,7 +111,8 @@ template <int KB, int KC>
 struct TcSmem {
     static constexpr int A = KB / 64 * kPanel, C = KC / 64 * kPanel;
     static constexpr int STAGE = 2 * A + C;
-    static constexpr int S = KB / 64 * KC * 128;       // [i panel][j row][64 i]
+    static constexpr bool TWO = KB == 64 && KC == 64;  // the state in two parts
+    static constexpr int S = (TWO ? 2 : KB / 64) * KC * 128;   // [i panel or part][j row][64 i]
     static constexpr int OFF_S = 2 * STAGE;
     static constexpr int OFF_W = OFF_S + S;
     static constexpr int OFF_BAR = OFF_W + (int)sizeof(Decays);
@@ -444,18 +445,28 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     if (it > 0 && !(fine = wait(kStaged + (par ^ 1), ((it - 1) >> 1) & 1))) break;   // O has been read
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < KB / 16; i++)
-                        umma_ss(tmem + kColO, a_desc + (((i >> 2) * kPanel + (i & 3) * 32) >> 4),
+                    for (int i = 0; i < (L::TWO ? 2 : 1) * KB / 16; i++)
+                        umma_ss(tmem + kColO, a_desc + (((L::TWO ? 0 : i >> 2) * kPanel + (i & 3) * 32) >> 4),
                                 s_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, i > 0);
                     umma_commit(bars + kAS);
                     // N-major panels of 64 channels: 16 tokens are 2048 bytes
                     const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
-                    if (!(fine = wait(kCReady, 0))) break;
+                    if (!(fine = wait(kCReady, L::TWO ? par : 0))) break;
                     tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < 16; i++)               // the smallest plane first
                         umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (i & 3) * (2048 >> 4), id_upd, i > 0);
-                    umma_commit(bars + kCFree);
+                    if constexpr (L::TWO) {
+                        // lanes 0-63 and 64-127 each hold the channels for one half of the tokens; what the
+                        // other half's columns get of them is not read
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            umma_ts(tmem + kColU + 64, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd,
+                                    i > 0);
+                        umma_commit(bars + kUpd + par);
+                    } else {
+                        umma_commit(bars + kCFree);
+                    }
                     if (!(fine = wait(kPReady, par))) break;
                     tc_fence_after();
 #pragma unroll
@@ -463,12 +474,14 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         umma_ts(tmem + kColO, tmem + kColScores + (i >> 1) * 32 + (i & 1) * 8, cn_desc + i * (2048 >> 4),
                                 id_pc, i > 0);
                     umma_commit(bars + kPC);
-                    if (!(fine = wait(kCReady, 1))) break;
-                    tc_fence_after();
+                    if constexpr (!L::TWO) {
+                        if (!(fine = wait(kCReady, 1))) break;
+                        tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd, true);
-                    umma_commit(bars + kUpd + par);
+                        for (int i = 0; i < 16; i++)
+                            umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd, true);
+                        umma_commit(bars + kUpd + par);
+                    }
                 }
             }
             if (!fine) {
@@ -482,11 +495,14 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         regs_claim<kRegsCompute>();
         const int q = warp & 3, half = warp >> 2;     // TMEM lanes 32 q .. + 32; half of the columns
         const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16);
-        const int row = q * 32 + lane;                // token of P and O, channel of c (row j of S^T)
+        const int row = q * 32 + lane;                // token of P and O
         constexpr int NS = KB / 2;                    // columns of S^T per thread
         constexpr int NO = KC / 2;                    // columns of O per thread
-        const bool s_on = q * 32 < KC;                // S^T has KC rows
+        const int part = L::TWO ? q >> 1 : 0;         // of the state
+        const int sq = L::TWO ? q & 1 : q, srow = sq * 32 + lane;     // rows of S^T: channels of c
+        const bool s_on = sq * 32 < KC;               // S^T has KC rows
         const int i0 = half * NS, o0 = half * NO;
+        const uint32_t ucol = kColU + part * 64 + i0;
         auto arrive = [&](int bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + bar);
@@ -526,29 +542,30 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             if (s_on) {
                 const float* src = nullptr;
                 int64_t step = r.s_i;
-                if (c0 > 0) {
-                    src = p.handoff + (int64_t)blockIdx.x * KB * KC + row;
+                if (part == 1) {
+                    // the second part starts from zero
+                } else if (c0 > 0) {
+                    src = p.handoff + (int64_t)blockIdx.x * KB * KC + srow;
                     step = KC;
-                } else if (row < r.dc && p.nseg > 1) {
-                    src = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc + row;
+                } else if (srow < r.dc && p.nseg > 1) {
+                    src = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc + srow;
                     step = r.dc;
-                } else if (row < r.dc && r.state0) {
-                    src = r.state0 + k.bh * r.db * r.dc + row * r.s_j;
+                } else if (srow < r.dc && r.state0) {
+                    src = r.state0 + k.bh * r.db * r.dc + srow * r.s_j;
                 }
                 const int cols = c0 > 0 ? KB : r.db;
+                // 32 loads at a time: they are what a row's start waits for
 #pragma unroll 1
-                for (int i = 0; i < NS; i += 8) {
-                    float x[8];
+                for (int i = 0; i < NS; i += 32) {
+                    uint32_t v[32];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = src && i0 + i + e < cols ? __ldcg(src + (i0 + i + e) * step) : 0.f;
-                    uint32_t v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = __float_as_uint(x[e]);
-                    tmem_st8(tm + kColU + i0 + i, v);
+                    for (int e = 0; e < 32; e++)
+                        v[e] = src && i0 + i + e < cols ? __float_as_uint(__ldcg(src + (i0 + i + e) * step)) : 0u;
+                    tmem_st32(tm + ucol + i, v);
                 }
                 tmem_wait_st();
                 uint32_t v[NS];
-                tmem_ld<NS>(tm + kColU + i0, v);
+                tmem_ld<NS>(tm + ucol, v);
 #pragma unroll
                 for (int e = 0; e < NS; e++) s[e] = __uint_as_float(v[e]);
             }
@@ -560,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         const uint4 v = make_uint4(pack_bf16(s[i], s[i + 1]), pack_bf16(s[i + 2], s[i + 3]),
                                                    pack_bf16(s[i + 4], s[i + 5]), pack_bf16(s[i + 6], s[i + 7]));
                         const int ii = i0 + i;
-                        *reinterpret_cast<uint4*>(smem + L::OFF_S + (ii >> 6) * (KC * 128) + swz128(row, (ii & 63) * 2)) = v;
+                        *reinterpret_cast<uint4*>(smem + L::OFF_S + ((ii >> 6) + part) * (KC * 128) + swz128(srow, (ii & 63) * 2)) = v;
                     }
                 }
                 fence_proxy_async_smem();
@@ -581,13 +598,13 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     arrive(kFixed);
                     if (!(fine = await(kFixed, fixed++ & 1))) break;
                 }
-                // planes of C'^T, 64 tokens at a time, of which this warp does 32
+                // planes of C'^T, 64 tokens at a time (of two parts: all at once), of which this warp does 32
                 auto put_planes = [&](int sub) {
                     if (s_on) {
                         const __nv_bfloat16(*wt)[kT] = dec.plane[n < kT];
                         const int s0 = sub * 64 + half * 32;
                         Planes pl;
-                        decayed_planes(smem_u32(st + 2 * L::A), q * 32, s0, [&](int e) {
+                        decayed_planes(smem_u32(st + 2 * L::A), sq * 32, s0, [&](int e) {
                             const int at = s0 + 8 * e + 2 * (lane & 3);
                             return SplitPair{*reinterpret_cast<const __nv_bfloat162*>(&wt[0][at]),
                                              *reinterpret_cast<const __nv_bfloat162*>(&wt[1][at]),
@@ -600,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     tc_fence_before();
                     arrive(kCReady);
                 };
-                put_planes(0);
+                put_planes(part);
 
                 // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
                 if (!(fine = await(kScores, par))) break;
@@ -652,9 +669,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 tc_fence_before();
                 arrive(kPReady);
 
-                if (!(fine = await(kCFree, par))) break;
-                tc_fence_after();
-                put_planes(1);
+                if constexpr (!L::TWO) {
+                    if (!(fine = await(kCFree, par))) break;
+                    tc_fence_after();
+                    put_planes(1);
+                }
 
                 // O
                 if (!(fine = await(kPC, par))) break;
@@ -724,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 if (s_on) {
                     const float fn = dec.pow[n];
                     uint32_t v[NS];
-                    tmem_ld<NS>(tm + kColU + i0, v);
+                    tmem_ld<NS>(tm + ucol, v);
 #pragma unroll
                     for (int e = 0; e < NS; e += 2) {
                         const float2 x = __ffma2_rn(make_float2(fn, fn), make_float2(s[e], s[e + 1]),
@@ -741,27 +760,38 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             const bool ends = c1 == k.nchunk;
             const bool out = ends && k.slot == p.nseg - 1 && r.state_out;
             if (!ends || out) {
-                if (s_on) {
+                if constexpr (L::TWO) {
+                    // the parts are joined through the place of their copies, which no product reads any more
+                    float* other = reinterpret_cast<float*>(smem + L::OFF_S) + srow;
+                    if (part == 1)
+#pragma unroll
+                        for (int e = 0; e < NS; e++) other[(i0 + e) * KC] = s[e];
+                    if (!(fine = meet())) break;
+                    if (part == 0)
+#pragma unroll
+                        for (int e = 0; e < NS; e++) s[e] += other[(i0 + e) * KC];
+                }
+                if (s_on && part == 0) {
 #pragma unroll
                     for (int i = 0; i < NS; i += 32) {
                         uint32_t v[32];
 #pragma unroll
                         for (int e = 0; e < 32; e++) v[e] = __float_as_uint(s[i + e]);
-                        tmem_st32(tm + kColU + i0 + i, v);
+                        tmem_st32(tm + ucol + i, v);
                     }
                     tmem_wait_st();
-                    float* dst = ends ? r.state_out + k.bh * r.db * r.dc + row * r.s_j
-                                      : p.handoff + (int64_t)(blockIdx.x + 1) * KB * KC + row;
+                    float* dst = ends ? r.state_out + k.bh * r.db * r.dc + srow * r.s_j
+                                      : p.handoff + (int64_t)(blockIdx.x + 1) * KB * KC + srow;
                     const int64_t step = ends ? r.s_i : KC;
                     const int rows = ends ? r.dc : KC, cols = ends ? r.db : KB;
 #pragma unroll 1
                     for (int i = 0; i < NS; i += 8) {
                         uint32_t u[8];
-                        tmem_ld8(tm + kColU + i0 + i, u);
+                        tmem_ld8(tm + ucol + i, u);
                         tmem_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            if (row < rows && i0 + i + e < cols) dst[(i0 + i + e) * step] = __uint_as_float(u[e]);
+                            if (srow < rows && i0 + i + e < cols) dst[(i0 + i + e) * step] = __uint_as_float(u[e]);
                     }
                 }
                 if (!ends) {
