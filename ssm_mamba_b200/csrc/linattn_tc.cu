@@ -113,24 +113,25 @@ struct TcSmem {
     static constexpr int STAGE = 2 * A + C;
     static constexpr bool TWO = KB == 64 && KC == 64;  // the state in two parts
     static constexpr int S = (TWO ? 2 : KB / 64) * KC * 128;   // [i panel or part][j row][64 i]
-    static constexpr int OFF_S = 2 * STAGE;
+    static constexpr int STAGES = TWO ? 4 : 2;
+    static constexpr int OFF_S = STAGES * STAGE;
     static constexpr int OFF_W = OFF_S + S;
     static constexpr int OFF_BAR = OFF_W + (int)sizeof(Decays);
-    static constexpr int NBAR = 18;
+    static constexpr int NBAR = 26;
     static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
     static constexpr int USED = OFF_MISC + 16 + (int)sizeof(Range);
     // more than half an SM, so that two CTAs never share one SM's TMEM
     static constexpr int BYTES = USED > 120 * 1024 ? USED : 120 * 1024;
 };
 
-// mbarriers.  Those of a pair belong to one stage, whose next use nobody can reach before everybody
+// mbarriers.  Those of an array belong to one stage, whose next use nobody can reach before everybody
 // has seen this one: a waiter never falls two phases behind.
 enum Bar {
-    kFull = 0,       // [2] a stage's tiles are there
-    kStaged = 2,     // [2] O is staged over them
-    kFree = 4,       // [2] and stored, and every product has read them
-    kUpd = 6,        // [2] U is complete
-    kScores = 8, kAS, kPC, kCFree,      // products complete; kCFree: those of the first 64 tokens' planes
+    kFull = 0,       // [stages] a stage's tiles are there
+    kStaged = 4,     // O is staged over them
+    kFree = 8,       // and stored, and every product has read them
+    kUpd = 12,       // U is complete
+    kScores = 16, kAS, kPC, kCFree,      // products complete; kCFree: those of the first 64 tokens' planes
     kSReady, kCReady, kPReady, kFixed, kItem, kDrain
 };
 
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         if (lane == 0) *range_slot = r;
     }
     if (tid == 32) {
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < L::STAGES; i++) {
             mbar_init(bars + kFull + i, 1);
             mbar_init(bars + kStaged + i, kWarps);
             mbar_init(bars + kFree + i, 1);
@@ -368,31 +369,41 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         regs_release<kRegsControl>();
         if (warp == kWarps + 1 && elect_one()) {
             // ---- loads --------------------------------------------------------------------------
-            int it = 0;
+            int it = 0, begun = 0;
+            uint32_t was_over_a = 0;                  // by stage
             bool fine = true;
             for (int n = 0; n < nitems && fine; n++) {
                 int c0, c1;
                 const Row k = items.row(n, c0, c1);
                 const LaRole& r = p.role[k.ri];
                 const int ha = k.h / r.a.share, hb = k.h / r.b.share, hc = k.h / r.c.share;
+                // an output tile over a alone leaves b and c free once the products have read them
+                const uint32_t over_a = !L::TWO && KC <= KB && r.out_vec && !r.out_f32;
                 for (int c = c0; c < c1; c++, it++) {
-                    if (it >= 2 && !(fine = wait(kFree + (it & 1), ((it >> 1) - 1) & 1))) break;
-                    unsigned char* st = smem + (it & 1) * L::STAGE;
-                    uint64_t* bar = bars + kFull + (it & 1);
+                    const int sg = it % L::STAGES;
+                    const uint32_t last = (it / L::STAGES - 1) & 1, early = (was_over_a >> sg) & 1;
+                    if (it >= L::STAGES && !(fine = wait((early ? kUpd : kFree) + sg, last))) break;
+                    was_over_a = (was_over_a & ~(1u << sg)) | over_a << sg;
+                    unsigned char* st = smem + sg * L::STAGE;
+                    uint64_t* bar = bars + kFull + sg;
                     const int t = chunk_first(k, r.reverse, c);
                     mbar_arrive_expect_tx(bar, L::STAGE);
 #pragma unroll
-                    for (int i = 0; i < KB / 64; i++) {
-                        tma_load_4d(st + i * kPanel, &maps.a[k.ri], bar, i * 64, t, ha, k.b);
+                    for (int i = 0; i < KB / 64; i++)
                         tma_load_4d(st + L::A + i * kPanel, &maps.b[k.ri], bar, i * 64, t, hb, k.b);
-                    }
 #pragma unroll
                     for (int i = 0; i < KC / 64; i++)
                         tma_load_4d(st + 2 * L::A + i * kPanel, &maps.c[k.ri], bar, i * 64, t, hc, k.b);
+                    begun = it + 1;
+                    if (early && !(fine = wait(kFree + sg, last))) break;
+#pragma unroll
+                    for (int i = 0; i < KB / 64; i++)
+                        tma_load_4d(st + i * kPanel, &maps.a[k.ri], bar, i * 64, t, ha, k.b);
                 }
             }
             if (!fine)       // copies in flight still write to this CTA's shared memory
-                for (int i = max(0, it - 2); i < it; i++) mbar_wait_bounded(bars + kFull + (i & 1), (i >> 1) & 1);
+                for (int i = max(0, begun - L::STAGES); i < begun; i++)
+                    mbar_wait_bounded(bars + kFull + i % L::STAGES, (i / L::STAGES) & 1);
         } else if (warp == kWarps + 2 && elect_one()) {
             // ---- stores -------------------------------------------------------------------------
             int it = 0;
@@ -402,17 +413,19 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const Row k = items.row(n, c0, c1);
                 const LaRole& r = p.role[k.ri];
                 for (int c = c0; c < c1; c++, it++) {
-                    if (!(fine = wait(kStaged + (it & 1), (it >> 1) & 1))) break;
+                    const int sg = it % L::STAGES;
+                    const uint32_t turn = (it / L::STAGES) & 1;
+                    if (!(fine = wait(kStaged + sg, turn))) break;
                     if (r.out_vec) {
                         const int t = chunk_first(k, r.reverse, c), width = r.out_f32 ? 32 : 64;   // channels of a panel
-                        const unsigned char* src = smem + (it & 1) * L::STAGE;
+                        const unsigned char* src = smem + sg * L::STAGE;
                         for (int x = 0; x < r.dc; x += width, src += kPanel)
                             tma_store_4d(&maps.o[k.ri], src, x, t, k.h, k.b);
                         tma_store_commit();
                         tma_store_wait_read_all();
                     }
-                    if (!(fine = wait(kUpd + (it & 1), (it >> 1) & 1))) break;    // the last product to read the stage
-                    mbar_arrive(bars + kFree + (it & 1));
+                    if (!(fine = wait(kUpd + sg, turn))) break;    // the last product to read the stage
+                    mbar_arrive(bars + kFree + sg);
                 }
             }
             tma_store_wait_all();
@@ -428,8 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const Row k = items.row(n, c0, c1);
                 const int reverse = p.role[k.ri].reverse;
                 for (int c = c0; c < c1; c++, it++) {
-                    const uint32_t st = smem_u32(smem + (it & 1) * L::STAGE), par = it & 1;
-                    if (!(fine = wait(kFull + (it & 1), (it >> 1) & 1))) break;
+                    const int sg = it % L::STAGES;
+                    const uint32_t st = smem_u32(smem + sg * L::STAGE), par = it & 1;
+                    if (!(fine = wait(kFull + sg, (it / L::STAGES) & 1))) break;
                     if (chunk_count(k, reverse, c) < kT && !(fine = wait(kFixed, fixed++ & 1))) break;
                     if (it > 0 && !(fine = wait(kPC, par ^ 1))) break;       // the last P has been read
                     tc_fence_after();
@@ -442,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     }
                     umma_commit(bars + kScores);
                     if (!(fine = wait(kSReady, par))) break;
-                    if (it > 0 && !(fine = wait(kStaged + (par ^ 1), ((it - 1) >> 1) & 1))) break;   // O has been read
+                    if (it > 0 && !(fine = wait(kStaged + (it - 1) % L::STAGES, ((it - 1) / L::STAGES) & 1))) break;   // O has been read
                     tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < (L::TWO ? 2 : 1) * KB / 16; i++)
@@ -463,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         for (int i = 0; i < 16; i++)
                             umma_ts(tmem + kColU + 64, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd,
                                     i > 0);
-                        umma_commit(bars + kUpd + par);
+                        umma_commit(bars + kUpd + sg);
                     } else {
                         umma_commit(bars + kCFree);
                     }
@@ -480,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                         for (int i = 0; i < 16; i++)
                             umma_ts(tmem + kColU, tmem + kColC + i * 8, bn_desc + (4 + (i & 3)) * (2048 >> 4), id_upd, true);
-                        umma_commit(bars + kUpd + par);
+                        umma_commit(bars + kUpd + sg);
                     }
                 }
             }
@@ -588,10 +602,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             if (!(fine = meet())) break;              // the tables are there
 
             for (int c = c0; c < c1; c++, it++) {
-                const uint32_t par = it & 1;
+                const uint32_t par = it & 1, turn = (it / L::STAGES) & 1;
+                const int sg = it % L::STAGES;
                 const int n = chunk_count(k, reverse, c);
-                unsigned char* st = smem + (it & 1) * L::STAGE;
-                if (!(fine = await(kFull + (it & 1), (it >> 1) & 1))) break;
+                unsigned char* st = smem + sg * L::STAGE;
+                if (!(fine = await(kFull + sg, turn))) break;
                 if (n < kT) {
                     // rows past the length hold whatever the caller's padding holds
                     zero_rows(st, L::STAGE / kPanel, n, tid);
@@ -696,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 }
                 // the tile is staged over a, and where that is not enough over b and c, which the update reads
                 const bool bf16 = r.out_vec && !r.out_f32;
-                if ((!bf16 || KC > KB) && !(fine = await(kUpd + par, (it >> 1) & 1))) break;
+                if ((!bf16 || KC > KB) && !(fine = await(kUpd + sg, turn))) break;
                 if (bf16) {
 #pragma unroll
                     for (int i = 0; i < NO; i += 8) {
@@ -735,10 +750,10 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
-                arrive(kStaged + (it & 1));
+                arrive(kStaged + sg);
 
                 // the state after this chunk
-                if (!(fine = await(kUpd + par, (it >> 1) & 1))) break;
+                if (!(fine = await(kUpd + sg, turn))) break;
                 tc_fence_after();
                 if (s_on) {
                     const float fn = dec.pow[n];
