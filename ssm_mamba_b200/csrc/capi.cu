@@ -1161,6 +1161,7 @@ static int la_impl(const char* name, const ssm_linear_attn_args* a, int backward
         p.handoff = reinterpret_cast<float*>(ws + pl.handoff);
     }
     p.log_decay = a->log_decay; p.length = a->length; p.err = di->err;
+    p.test_withhold = pl.tc && getenv("SSM_TEST_WITHHOLD_TMA") != nullptr;     // as in ssm_scan_fwd
     LaInput in[4];
     const int nin = la_inputs(a, backward, in);
     cudaError_t e;

@@ -49,6 +49,7 @@ struct LaParams {
     const float* log_decay;
     const int64_t* length;  // may be null
     int* err;             // device error word
+    int test_withhold;    // test hook: no loads are issued, so that the waits for them run out
     // tensor-core kernel: the CTAs share the chunks of all rows evenly (more rows than CTAs), and a row
     // that two CTAs share passes its state through handoff, one state and one flag per CTA
     int split;

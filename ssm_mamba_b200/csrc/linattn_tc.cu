@@ -7,7 +7,7 @@
 //     O      = P C + beta diag(w^.) (A S)    two products; the second is taken out of TMEM and
 //                                            scaled per row before the first uses its columns
 //     U      = (C'^T) B,  S^T = w^n S^T + U      C' = sigma diag(w^.) C
-// Operands: A, B, C arrive by TMA in 128-byte-swizzled tiles (two stages); B serves as the K-major
+// Operands: A, B, C arrive by TMA in 128-byte-swizzled tiles (in two or four stages); B serves as the K-major
 // operand of the scores and as the N-major operand of U, C as the N-major operand of P C; P and
 // C'^T are written by the threads into TMEM as A operands; bfloat16(S) goes to shared memory.
 //
@@ -21,6 +21,11 @@
 // the stores.  The order of the phases lets each run beside a product:
 //     C'(c), first 64 tokens | scores, A S;   P(c) | U, first half;   C'(c), last 64 | P C;
 //     O(c) | U, last half;   S(c + 1) | scores(c + 1).
+// Heads of up to 64 channels would leave half of the lanes of C'^T idle.  For them lanes 0-63 take a
+// chunk's first 64 tokens and lanes 64-127 the last 64, all warps at once, and the state is kept in two
+// parts, each decayed alike and with the U of its half; A S sums over both, and they are joined
+// where the state leaves the CTA.  Their smaller tiles have four stages.  1280 tokens of 148 heads:
+// 35.0 us without parts and with two stages, 33.0 so.
 //
 // With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
 // range, so its first row may have been begun by the CTA before it and its last may be finished
@@ -28,8 +33,8 @@
 // the end of its first row last: by then the state it needs is there, since the two parts of a
 // row together are no longer than a CTA's range.
 //
-// Measured: 4 x 2048 tokens of 40 heads of 128, forward, 86 us (3.9 TB/s of its 346 MB): 3.9 us a chunk, where
-// HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 2.4 us against 1.5.  What bounds
+// Measured: 4 x 2048 tokens of 40 heads of 128, forward, 83 us (4.2 TB/s of its 346 MB): 3.9 us a chunk, where
+// HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 2.5 us against 1.5.  What bounds
 // it is the chain of a chunk: six times the compute warps wait for a product and hand one on, 150 to 250
 // cycles each, between 600 and 1200 cycles of conversions.  Groups of warps with one step each took
 // twice as long (their code together misses the instruction cache), 16 compute warps 4.5 us a chunk
@@ -60,9 +65,9 @@ constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P 
 constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
 constexpr uint32_t kColC = 384;            // 4 x 32: planes of C'^T for 64 tokens
-// Tries before a wait has run out: each lasts 30 cycles or more (a try may suspend for longer), so
-// 0.06 s or more, against the microseconds of the longest wait that ends
-constexpr int kTries = 1 << 22;
+// Tries before a wait has run out: one that fails takes some 200 cycles among many waiters and 7800 alone
+// (measured), so 0.1 to 4 s, against the microseconds of the longest wait that ends
+constexpr int kTries = 1 << 20;
 constexpr float kZeroLog2 = -151.f;        // exp2 of anything below is zero in float32
 
 // A weight as a sum of three bfloat16 of 8 bits each.
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
             // ---- loads --------------------------------------------------------------------------
             int it = 0, begun = 0;
             uint32_t was_over_a = 0;                  // by stage
-            bool fine = true;
+            bool fine = !p.test_withhold;
             for (int n = 0; n < nitems && fine; n++) {
                 int c0, c1;
                 const Row k = items.row(n, c0, c1);
