@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
     constexpr int LDB = Smem::LDB, LDN = Smem::LDN, LDP = Smem::LDP;
     // warps over the state: DB / 16 rows of tiles, the rest along its columns; over P and out: 4 rows
     constexpr int NT = kThreads<DB>, NW = NT / 32, MT = DB / 16, CS = DC / (NW / MT), NS = CS / 8;
-    constexpr int CP = kC / (NW / 4), NP = CP / 8, CO = DC / (NW / 4), NO = CO / 8;
+    constexpr int NP = kC / (NW / 4) / 8, CO = DC / (NW / 4), NO = CO / 8;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const LaRole& r = p.role[blockIdx.z];
     const int col0 = blockIdx.y * DC;
@@ -163,7 +163,10 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
     const int64_t tok0 = (int64_t)seg * p.seglen;
     const int tid = threadIdx.x, warp = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
     const int sm0 = warp % MT * 16, sn0 = warp / MT * CS;          // this warp's tiles of the state
-    const int m0 = warp / (NW / 4) * 16, n0 = warp % (NW / 4) * CP, on0 = warp % (NW / 4) * CO;   // of P, of out
+    // of P and of out: the mask leaves the later rows more to do, and of 8 warps each scheduler has two rows
+    constexpr int CW = NW / 4;
+    const int mt = warp / CW, cw = warp % CW, m0 = (NW == 8 && mt >= 2 ? 5 - mt : mt) * 16, on0 = cw * CO;
+    auto p_col = [&](int j) { return (j * CW + cw) * 8; };
     const float g2 = la_log2_decay(p.log_decay[h]);
 
     for (int i = tid; i <= kC; i += NT) sm.w[i] = exp2f(g2 * (float)i);
@@ -218,11 +221,11 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
             __syncthreads();
             float acc[NP][4] = {}, o[NO][4] = {};
             // scores, of which the causal mask leaves a warp the tiles up to (reverse: from) its rows
-            auto live = [&](int j) { return r.reverse ? n0 + 8 * j + 7 >= m0 : n0 + 8 * j <= m0 + 15; };
+            auto live = [&](int j) { return r.reverse ? p_col(j) + 7 >= m0 : p_col(j) <= m0 + 15; };
 #pragma unroll 1
             for (int k = 0; k < DB; k += 16) {
                 const Rows a = rows([&](int m, int i) { return sm.a[(m0 + m) * LDB + k + i]; });
-                product(acc, a, [&](int i, int c) { return sb[(n0 + c) * LDB + k + i]; }, live);
+                product(acc, a, [&](int i, int c) { return sb[(p_col(c >> 3) + (c & 7)) * LDB + k + i]; }, live);
                 product(o, a, [&](int i, int c) { return sm.s[(k + i) * LDN + on0 + c]; }, all);   // the state's part
             }
 #pragma unroll
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
             for (int j = 0; j < NP; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int row = m0 + g + (e & 2) * 4, col = n0 + 8 * j + 2 * t + (e & 1);
+                    const int row = m0 + g + (e & 2) * 4, col = p_col(j) + 2 * t + (e & 1);
                     const int dist = r.reverse ? col - row : row - col;
                     sm.s[row * LDP + col] = dist >= 0 ? r.alpha * acc[j][e] * sm.w[dist] : 0.f;
                 }
