@@ -34,6 +34,8 @@ namespace ssm {
 namespace {
 
 constexpr int kC = 64;         // tokens per chunk
+// up to so many segments each CTA folds the states of those before its own; more are scanned
+constexpr int kFold = 8;
 
 // threads of a CTA: with 128 channels it has an SM to itself
 template <int DB>
@@ -171,22 +173,6 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
 
     for (int i = tid; i <= kC; i += NT) sm.w[i] = exp2f(g2 * (float)i);
 
-    // state fragments: element e of tile j is row sm0 + g (+ 8), column sn0 + 8 j + 2 t (+ 1); from the
-    // segment's start state, which the scan has left in its place, or from the initial state
-    float s[NS][4];
-    auto s_row = [&](int e) { return sm0 + g + (e & 2) * 4; };
-    auto s_col = [&](int j, int e) { return sn0 + 8 * j + 2 * t + (e & 1); };
-    auto valid = [&](int j, int e) { return s_row(e) < r.db && s_col(j, e) < cols; };
-    const float* start = !STATE && p.nseg > 1 ? r.seg + (bh * p.nseg + seg) * r.db * r.dc
-                         : !STATE && r.state0 ? r.state0 + bh * r.db * r.dc : nullptr;
-    const int64_t s_i = p.nseg > 1 ? r.dc : r.s_i, s_j = p.nseg > 1 ? 1 : r.s_j;
-#pragma unroll
-    for (int j = 0; j < NS; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            s[j][e] = start && valid(j, e) ? start[s_row(e) * s_i + (col0 + s_col(j, e)) * s_j] : 0.f;
-
-    const auto all = [](int) { return true; };
     const int nchunk = (ntok + kC - 1) / kC;
     // copies of chunk `it`, one group for b and c and one for a; the groups may be empty
     auto chunk_start = [&](int it) { return (int64_t)(r.reverse ? nchunk - 1 - it : it) * kC; };
@@ -205,6 +191,38 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
     };
     load_bc(0);
     load_a(0);
+
+    // state fragments: element e of tile j is row sm0 + g (+ 8), column sn0 + 8 j + 2 t (+ 1); from the state that
+    // the scan has left in the segment's place, or from the initial state and the segments before
+    float s[NS][4];
+    auto s_row = [&](int e) { return sm0 + g + (e & 2) * 4; };
+    auto s_col = [&](int j, int e) { return sn0 + 8 * j + 2 * t + (e & 1); };
+    auto valid = [&](int j, int e) { return s_row(e) < r.db && s_col(j, e) < cols; };
+    const float* segs = r.seg + bh * p.nseg * r.db * r.dc;
+    const bool scanned = p.nseg > kFold;
+    const float* start = STATE ? nullptr : scanned ? segs + (int64_t)seg * r.db * r.dc
+                         : r.state0 ? r.state0 + bh * r.db * r.dc : nullptr;
+    const int64_t s_i = scanned ? r.dc : r.s_i, s_j = scanned ? 1 : r.s_j;
+#pragma unroll
+    for (int j = 0; j < NS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            s[j][e] = start && valid(j, e) ? start[s_row(e) * s_i + (col0 + s_col(j, e)) * s_j] : 0.f;
+    if (!STATE && !scanned) {
+#pragma unroll 2
+        for (int before = 0; before < slot; before++) {
+            const int at = r.reverse ? p.nseg - 1 - before : before;
+            const float f = exp2f(g2 * (float)la_segment_tokens(p, row_len, at));
+            const float* v = segs + (int64_t)at * r.db * r.dc + col0;
+#pragma unroll
+            for (int j = 0; j < NS; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    s[j][e] = fmaf(f, s[j][e], valid(j, e) ? v[s_row(e) * r.dc + s_col(j, e)] : 0.f);
+        }
+    }
+
+    const auto all = [](int) { return true; };
     for (int it = 0; it < nchunk; it++) {
         const int64_t t0 = tok0 + chunk_start(it);
         const int n = (int)min((int64_t)kC, ntok - chunk_start(it));
@@ -361,7 +379,8 @@ cudaError_t launch_f32(const LaParams& p, int max_dc, cudaStream_t stream) {
     if (p.nseg > 1) {
         // the last segment (in walking order) feeds nobody
         state_k<<<dim3(rows * (p.nseg - 1), tiles, p.nroles), kThreads<DB>, bytes, stream>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess || (e = launch_linattn_scan(p, stream)) != cudaSuccess) return e;
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        if (p.nseg > kFold && (e = launch_linattn_scan(p, stream)) != cudaSuccess) return e;
     }
     main_k<<<dim3(rows * p.nseg, tiles, p.nroles), kThreads<DB>, bytes, stream>>>(p);
     return cudaGetLastError();
