@@ -14,8 +14,8 @@
 // the FMAs); tcgen05 takes tf32 operands from shared memory along K only and would need the split
 // tiles stored, more than a CTA has at 128 channels.  An infinity becomes a NaN when it is split.
 //
-// Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 211 us (325 us on FMAs); 11 x 94
-// tokens of 40 heads, 96 and 80 channels, forward, 128 us.  What bounds it is the latency of a
+// Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 193 us (325 us on FMAs); 11 x 94
+// tokens of 40 heads, 96 and 80 channels, forward, 113 us.  What bounds it is the latency of a
 // chunk's steps at 16 warps an SM: the tensor pipe is busy 30% of the time, issue 45%.
 //
 // Shared-memory rows are strided so that a fragment's 32 elements lie on different banks: 4 (mod
@@ -23,9 +23,10 @@
 // ways, has 4 and two elements to some banks when read across.  The next chunk is copied meanwhile.
 //
 // A chunk alone is a chain of loads, products and barriers that leaves the pipe idle, so a row is
-// cut into segments until there are several CTAs per SM: a first pass leaves each segment's state
-// from a zero start, a scan turns those into the states that the segments start from, and the
-// main pass runs all segments at once.  S is computed twice, a quarter more products.
+// cut into segments until there are two CTAs per SM: a first pass leaves each segment's state from a
+// zero start, and the main pass runs all segments at once from the states that those add up to,
+// folded by each CTA or, of many segments, scanned before.  S is computed twice, a quarter more
+// products.
 #include "common.cuh"
 #include "linattn.h"
 
@@ -34,7 +35,8 @@ namespace ssm {
 namespace {
 
 constexpr int kC = 64;         // tokens per chunk
-// up to so many segments each CTA folds the states of those before its own; more are scanned
+// Up to so many segments each CTA folds the states of those before its own; more are scanned (six and two
+// segments of the training step above: 202 us scanned, 193 folded).
 constexpr int kFold = 8;
 
 // threads of a CTA: with 128 channels it has an SM to itself
@@ -239,9 +241,14 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
             __syncthreads();
             float acc[NP][4] = {}, o[NO][4] = {};
             // scores, of which the causal mask leaves a warp the tiles up to (reverse: from) its rows
-            auto live = [&](int j) { return r.reverse ? p_col(j) + 7 >= m0 : p_col(j) <= m0 + 15; };
+            uint32_t tiles = 0;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                tiles |= (p_col(j) < n && (r.reverse ? p_col(j) + 7 >= m0 : p_col(j) <= m0 + 15)) << j;
+            auto live = [&](int j) { return (tiles >> j & 1) != 0; };
+            const int k_end = m0 < n ? DB : 0;             // rows past the last token need nothing
 #pragma unroll 1
-            for (int k = 0; k < DB; k += 16) {
+            for (int k = 0; k < k_end; k += 16) {
                 const Rows a = rows([&](int m, int i) { return sm.a[(m0 + m) * LDB + k + i]; });
                 product(acc, a, [&](int i, int c) { return sb[(p_col(c >> 3) + (c & 7)) * LDB + k + i]; }, live);
                 product(o, a, [&](int i, int c) { return sm.s[(k + i) * LDN + on0 + c]; }, all);   // the state's part
@@ -268,7 +275,7 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
                 }
             __syncthreads();                   // P is complete
             // causal part
-            const int k_lo = r.reverse ? m0 : 0, k_hi = r.reverse ? kC : m0 + 16;
+            const int k_lo = r.reverse ? m0 : 0, k_hi = k_end == 0 ? 0 : r.reverse ? n : m0 + 16;
 #pragma unroll 1
             for (int k = k_lo; k < k_hi; k += 16)
                 product(o, rows([&](int m, int i) { return sm.s[(m0 + m) * LDP + k + i]; }),
