@@ -751,6 +751,11 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 std::optional<at::Tensor> opt(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+// without a trip through the dispatcher where there is nothing to do
+at::Tensor contiguous_f32(const at::Tensor& t) {
+    return (t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)).contiguous();
+}
+at::Tensor with_sizes(const at::Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
 at::Tensor unit_last_stride(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
 // Gradients that were asked for with a graph of their own: going through them is an error, not a zero.
@@ -819,7 +824,7 @@ std::vector<at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& 
     }
     if (lengths) len = lengths->to(q.device(), at::kLong).contiguous();
     const at::Tensor qc = unit_last_stride(q), kc = unit_last_stride(k), vc = unit_last_stride(v);
-    const at::Tensor g = log_decay.to(at::kFloat).contiguous();
+    const at::Tensor g = contiguous_f32(log_decay);
     const double sc = scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1)));
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                      (s0 && s0->requires_grad()));
@@ -831,7 +836,7 @@ at::Tensor linear_attention_update(const at::Tensor& state, const at::Tensor& q,
                                    const at::Tensor& v, const at::Tensor& log_decay, std::optional<double> scale) {
     check_la("linear_attention_update", q, k, v, log_decay);
     return linear_attn_update(state, unit_last_stride(q), unit_last_stride(k), unit_last_stride(v),
-                              log_decay.to(at::kFloat).contiguous(),
+                              contiguous_f32(log_decay),
                               scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1))));
 }
 
@@ -853,14 +858,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         ctx->saved_data["shape"] = x.sizes();
         ctx->saved_data["dw"] = weight && weight->requires_grad();
         ctx->saved_data["db"] = bias && bias->requires_grad();
-        return r[0].view(x.sizes());
+        return with_sizes(r[0], x.sizes());
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
         std::vector<at::Tensor> g = layer_norm_bwd(s[0], opt(s[1]), s[2], s[3], as_rows(grads[0]),
                                                    ctx->saved_data["dw"].toBool(), ctx->saved_data["db"].toBool());
         return once_differentiable("layer_norm_fn",
-                                   {g[0].view(ctx->saved_data["shape"].toIntVector()), g[1], g[2], at::Tensor()});
+                                   {with_sizes(g[0], ctx->saved_data["shape"].toIntVector()), g[1], g[2], at::Tensor()});
     }
 };
 
@@ -870,10 +875,10 @@ at::Tensor layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& weig
                      "layer_norm_fn: x must be float32 or bfloat16, got ", x.scalar_type());
     TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm_fn: x must have at least one dimension");
     std::optional<at::Tensor> w, b;
-    if (weight) w = weight->to(at::kFloat).contiguous();
-    if (bias) b = bias->to(at::kFloat).contiguous();
+    if (weight) w = contiguous_f32(*weight);
+    if (bias) b = contiguous_f32(*bias);
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad())))
-        return layer_norm_fwd(as_rows(x), w, b, eps, false)[0].view(x.sizes());
+        return with_sizes(layer_norm_fwd(as_rows(x), w, b, eps, false)[0], x.sizes());
     return LayerNorm::apply(x, w, b, eps);
 }
 
