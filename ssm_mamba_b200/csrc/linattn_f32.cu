@@ -16,7 +16,8 @@
 //
 // Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 193 us (325 us on FMAs); 11 x 94
 // tokens of 40 heads, 96 and 80 channels, forward, 113 us.  What bounds it is the latency of a
-// chunk's steps at 16 warps an SM: the tensor pipe is busy 30% of the time, issue 45%.
+// chunk's steps at 16 warps an SM: the tensor pipe is busy 30 to 40% of the time, issue 40 to 50%
+// (two tiles' products interleaved by hand: 191 us and 115 us).
 //
 // Shared-memory rows are strided so that a fragment's 32 elements lie on different banks: 4 (mod
 // 32) for operands read along their rows, 8 for operands read across them; b, which is read both
