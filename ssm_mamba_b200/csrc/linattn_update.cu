@@ -1,10 +1,10 @@
 // One decode step of linear attention with a decay for each head:
 //     S = w S + k v^T (in place),   out = scale q^T S,   w = exp(log_decay[h])
 // per (batch row, head).  Bound by HBM: the float32 state is read and written once, everything
-// else is three short rows.  A CTA of 8 warps owns one (batch row, head): a row of S is one
-// coalesced run of float4 over LPR lanes, a warp takes 32 / LPR rows at a time and issues the
+// else is three short rows.  A CTA of 8 warps owns up to 64 columns of one (batch row, head): its part of
+// a row of S is one coalesced run of float4 over LPR lanes, a warp takes 32 / LPR rows at a time and issues the
 // loads of all its rows before it uses any; the column sums of q^T S are joined over the warps
-// through shared memory in a fixed order.  64 x 40 heads of 128 x 128 take 66 us (5.1 TB/s, half of
+// through shared memory in a fixed order.  64 x 40 heads of 128 x 128 take 61 us (5.6 TB/s, half of
 // it writes).
 #include "common.cuh"
 #include "linattn.h"
@@ -96,8 +96,9 @@ cudaError_t dispatch_update(const LaUpdParams& p, int vec, cudaStream_t stream) 
     if (!vec) return launch_update<T, 1, 32>(p, stream);
     if (p.dv <= 16) return launch_update<T, 4, 4>(p, stream);
     if (p.dv <= 32) return launch_update<T, 4, 8>(p, stream);
-    if (p.dv <= 64) return launch_update<T, 4, 16>(p, stream);
-    return launch_update<T, 4, 32>(p, stream);
+    // 64 columns per CTA: 4 CTAs of 64 registers share an SM, and their loads and stores overlap (64 x 40 heads of
+    // 128 x 128: 66 us with 128 columns, 61 with 64, 62 with 32)
+    return launch_update<T, 4, 16>(p, stream);
 }
 
 }  // namespace
