@@ -3,24 +3,26 @@
 //
 // A row is one (batch row, head, role, segment); it is walked in chunks of 128 tokens.  Per chunk,
 // with w = exp(log_decay[h]) and the float32 state S^T (row = channel of c) in registers:
-//     scores = A B^T                         128 x 128, then P = alpha scores o W as bfloat16
+//     scores = A B^T                         128 x 128, then P = alpha scores o W
 //     O      = P C + beta diag(w^.) (A S)    two products; the second is taken out of TMEM and
 //                                            scaled per row before the first uses its columns
 //     U      = (C'^T) B,  S^T = w^n S^T + U      C' = sigma diag(w^.) C
 // Operands: A, B, C arrive by TMA in 128-byte-swizzled tiles (in two or four stages); B serves as the K-major
 // operand of the scores and as the N-major operand of U, C as the N-major operand of P C; P and
-// C'^T are written by the threads into TMEM as A operands; bfloat16(S) goes to shared memory.
+// C'^T are written by the threads into TMEM as A operands; S goes to shared memory.
 //
-// Roundings below float32: P and the copy of S that A multiplies are bfloat16, each on its own
-// part of O, whose result is rounded to bfloat16 anyway.  The state itself is float32: C' is
-// carried as a sum of four bfloat16 planes (24 bits of the weight) and U is added to the decayed
-// state in float32.
+// Roundings below float32: P and the copy of S that A multiplies are each the sum of two bfloat16, an upper
+// and a lower half (2^-16; with the upper half alone an output was 2.35e-3 off, of which its own rounding to
+// bfloat16 makes 1.66e-3).  The state itself is float32: C' is carried as a sum of four bfloat16 planes
+// (24 bits of the weight) and U is added to the decayed state in float32.
 //
 // One CTA per SM.  Warps 0-7 do the work between products, two for each quarter of the TMEM
 // lanes, each with half of the columns; warp 8 issues the products, warp 9 the loads, warp 10
 // the stores.  The order of the phases lets each run beside a product:
 //     C'(c), first 64 tokens | scores, A S;   P(c) | U, first half;   C'(c), last 64 | P C;
 //     O(c) | U, last half;   S(c + 1) | scores(c + 1).
+// At 128 x 128 channels shared memory has room for one half of S: the lower one takes the place of the upper
+// between C'(c) and P(c).
 // Heads of up to 64 channels would leave half of the lanes of C'^T idle.  For them lanes 0-63 take a
 // chunk's first 64 tokens and lanes 64-127 the last 64, all warps at once, and the state is kept in two
 // parts, each decayed alike and with the U of its half; A S sums over both, and they are joined
@@ -57,11 +59,11 @@ constexpr int kPanel = kT * 128;           // bytes of 128 rows x 64 channels
 constexpr int kWarps = 8;                  // compute warps
 constexpr int kCompute = kWarps * 32;
 constexpr int kThreads = kCompute + 128;   // the last warpgroup issues copies and products
-// Registers: launched with 168 each (384 * 168 = 256 * 224 + 128 * 56)
-constexpr int kRegsCompute = 224, kRegsControl = 56;
+// Registers: launched with 168 each (384 * 168 = 256 * 216 + 128 * 72; with 56 the warp of the products spills)
+constexpr int kRegsCompute = 216, kRegsControl = 72;
 constexpr uint32_t kTmemCols = 512;
 // TMEM columns
-constexpr uint32_t kColScores = 0;         // 128: scores; of each 32 columns P then takes the first 16
+constexpr uint32_t kColScores = 0;         // 128: scores, then P: of each 32 columns 16 for the upper halves, 16 for the lower
 constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
 constexpr uint32_t kColC = 384;            // 4 x 32: planes of C'^T for 64 tokens
@@ -117,7 +119,10 @@ struct TcSmem {
     static constexpr int A = KB / 64 * kPanel, C = KC / 64 * kPanel;
     static constexpr int STAGE = 2 * A + C;
     static constexpr bool TWO = KB == 64 && KC == 64;  // the state in two parts
-    static constexpr int S = (TWO ? 2 : KB / 64) * KC * 128;   // [i panel or part][j row][64 i]
+    static constexpr int S1 = (TWO ? 2 : KB / 64) * KC * 128;  // a half of S: [i panel or part][j row][64 i]
+    // both halves of S at once; at 128 x 128 channels there is room for one, and the second follows the first
+    static constexpr bool BOTH = KB * KC < 128 * 128;
+    static constexpr int S = (BOTH ? 2 : 1) * S1;
     static constexpr int STAGES = TWO ? 4 : 2;
     static constexpr int OFF_S = STAGES * STAGE;
     static constexpr int OFF_W = OFF_S + S;
@@ -165,6 +170,16 @@ struct Waiter {
     }
 };
 
+// Two floats as two pairs of bfloat16: their upper 16 bits, cut off, and what these leave, rounded (exact to 2^-16)
+__device__ __forceinline__ uint32_t upper_bf16(float x, float y) {
+    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+}
+__device__ __forceinline__ uint32_t lower_bf16(float x, float y) {
+    auto minus_upper = [](float v) { return __uint_as_float((__float_as_uint(v) & 0xffff0000u) ^ 0x80000000u); };
+    const float2 d = __fadd2_rn(make_float2(x, y), make_float2(minus_upper(x), minus_upper(y)));
+    const __nv_bfloat162 v = __floats2bfloat162_rn(d.x, d.y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -460,13 +475,25 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                         umma_ss(tmem + kColScores, a_desc + off, b_desc + off, id_scores, i > 0);
                     }
                     umma_commit(bars + kScores);
-                    if (!(fine = wait(kSReady, par))) break;
+                    if (!(fine = wait(kSReady, L::BOTH ? par : 0))) break;
                     if (it > 0 && !(fine = wait(kStaged + (it - 1) % L::STAGES, ((it - 1) / L::STAGES) & 1))) break;   // O has been read
                     tc_fence_after();
+                    auto a_s = [&](uint32_t half_desc, bool first) {
 #pragma unroll
-                    for (int i = 0; i < (L::TWO ? 2 : 1) * KB / 16; i++)
-                        umma_ss(tmem + kColO, a_desc + (((L::TWO ? 0 : i >> 2) * kPanel + (i & 3) * 32) >> 4),
-                                s_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, i > 0);
+                        for (int i = 0; i < (L::TWO ? 2 : 1) * KB / 16; i++)
+                            umma_ss(tmem + kColO, a_desc + (((L::TWO ? 0 : i >> 2) * kPanel + (i & 3) * 32) >> 4),
+                                    half_desc + (((i >> 2) * (KC * 128) + (i & 3) * 32) >> 4), id_as, !first || i > 0);
+                    };
+                    if constexpr (L::BOTH) {
+#pragma unroll 1
+                        for (int e = 0; e < 2; e++) a_s(s_desc + e * (L::S1 >> 4), e == 0);
+                    } else {
+                        a_s(s_desc, true);
+                        umma_commit(bars + kAS);
+                        if (!(fine = wait(kSReady, 1))) break;
+                        tc_fence_after();
+                        a_s(s_desc, false);
+                    }
                     umma_commit(bars + kAS);
                     // N-major panels of 64 channels: 16 tokens are 2048 bytes
                     const uint32_t bn_desc = umma_desc_lo(st + L::A, kPanel), cn_desc = umma_desc_lo(st + 2 * L::A, kPanel);
@@ -488,10 +515,12 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     }
                     if (!(fine = wait(kPReady, par))) break;
                     tc_fence_after();
+#pragma unroll 1
+                    for (int e = 0; e < 2; e++)                // the lower half first
 #pragma unroll
-                    for (int i = 0; i < kT / 16; i++)
-                        umma_ts(tmem + kColO, tmem + kColScores + (i >> 1) * 32 + (i & 1) * 8, cn_desc + i * (2048 >> 4),
-                                id_pc, i > 0);
+                        for (int i = 0; i < kT / 16; i++)
+                            umma_ts(tmem + kColO, tmem + kColScores + (16 - e * 16) + (i >> 1) * 32 + (i & 1) * 8,
+                                    cn_desc + i * (2048 >> 4), id_pc, e > 0 || i > 0);
                     umma_commit(bars + kPC);
                     if constexpr (!L::TWO) {
                         if (!(fine = wait(kCReady, 1))) break;
@@ -588,20 +617,30 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                 for (int e = 0; e < NS; e++) s[e] = __uint_as_float(v[e]);
             }
-            // bfloat16(S^T) to shared memory for A S
-            auto put_state = [&]() {
+            // a half of S^T to shared memory for A S
+            auto put_half = [&](bool upper, int at) {
                 if (s_on) {
 #pragma unroll
                     for (int i = 0; i < NS; i += 8) {
-                        const uint4 v = make_uint4(pack_bf16(s[i], s[i + 1]), pack_bf16(s[i + 2], s[i + 3]),
-                                                   pack_bf16(s[i + 4], s[i + 5]), pack_bf16(s[i + 6], s[i + 7]));
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            w[e] = upper ? upper_bf16(s[i + 2 * e], s[i + 2 * e + 1]) : lower_bf16(s[i + 2 * e], s[i + 2 * e + 1]);
                         const int ii = i0 + i;
-                        *reinterpret_cast<uint4*>(smem + L::OFF_S + ((ii >> 6) + part) * (KC * 128) + swz128(srow, (ii & 63) * 2)) = v;
+                        *reinterpret_cast<uint4*>(smem + L::OFF_S + at + ((ii >> 6) + part) * (KC * 128) +
+                                                  swz128(srow, (ii & 63) * 2)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
+            };
+            auto hand_state = [&]() {
                 fence_proxy_async_smem();
                 tc_fence_before();
                 arrive(kSReady);
+            };
+            auto put_state = [&]() {
+                put_half(true, 0);
+                if constexpr (L::BOTH) put_half(false, L::S1);
+                hand_state();
             };
             if (c0 < c1) put_state();
             if (!(fine = meet())) break;              // the tables are there
@@ -638,6 +677,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                     arrive(kCReady);
                 };
                 put_planes(part);
+                if constexpr (!L::BOTH) {
+                    if (!(fine = await(kAS, 0))) break;        // the product with the upper half has read it
+                    put_half(false, 0);
+                    hand_state();
+                }
 
                 // P in blocks of 32 x 32, which the mask empties, halves or leaves whole
                 if (!(fine = await(kScores, par))) break;
@@ -645,7 +689,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int sb = half * 2 + i;
-                    uint32_t o[16];
+                    uint32_t o[32];                            // upper halves, lower halves
+                    auto put = [&](int e, float x, float y) {
+                        o[e / 2] = upper_bf16(x, y);
+                        o[16 + e / 2] = lower_bf16(x, y);
+                    };
                     if (reverse ? sb >= q : sb <= q) {
                         uint32_t v[32];
                         tmem_ld<32>(tm + kColScores + sb * 32, v);
@@ -660,8 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                                                             __fmul2_rn(f2, make_float2(wb.x, wb.y)));
                                 const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])),
                                                             __fmul2_rn(f2, make_float2(wb.z, wb.w)));
-                                o[e / 2] = pack_bf16(x.x, x.y);
-                                o[e / 2 + 1] = pack_bf16(y.x, y.y);
+                                put(e, x.x, x.y);
+                                put(e + 2, y.x, y.y);
                             }
                         } else {
                             // the table runs with the columns: its entry for column e of the block is wt[e]
@@ -670,18 +718,18 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
                                 const float x = __uint_as_float(v[e]) * wt[e], y = __uint_as_float(v[e + 1]) * wt[e + 1];
-                                o[e / 2] = pack_bf16(live & (1u << e) ? x : 0.f, live & (2u << e) ? y : 0.f);
+                                put(e, live & (1u << e) ? x : 0.f, live & (2u << e) ? y : 0.f);
                             }
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = 0;
+                        for (int e = 0; e < 32; e++) o[e] = 0;
                     }
                     // over scores that this thread alone reads, and has read
-                    tmem_st16(tm + kColScores + sb * 32, o);
+                    tmem_st32(tm + kColScores + sb * 32, o);
                 }
                 // A S leaves TMEM
-                if (!(fine = await(kAS, par))) break;
+                if (!(fine = await(kAS, L::BOTH ? par : 1))) break;
                 tc_fence_after();
                 uint32_t as[NO];
                 tmem_ld<NO>(tm + kColO + o0, as);
