@@ -894,9 +894,11 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 
 // The state a segment reaches from a zero start: only U, with every token weighted towards the
 // segment's end, so that the sum needs no rescaling between chunks, and chunks whose every weight
-// is zero in float32 are not read.  C'^T has two buffers of 64 tokens; the threads fill one while
-// the product reads the other, and bound it (42 rows of 8 segments of 20 chunks, 128 channels: 83 us,
-// 65 at HBM's rate).
+// is zero in float32 are not read.  The tensor core cuts its sums off, so U starts from zero for each chunk,
+// in one of two places by turns, and is added to the sum in registers, rounded, while the next one is formed
+// (summed in the unit over 128 chunks of k and v with means of one, the state was 4.9e-5 off).  C'^T has two
+// buffers of 64 tokens; the threads fill one while the product reads the other, and bound it (42 rows of 8
+// segments of 20 chunks, 128 channels: 83 us, 65 at HBM's rate).
 constexpr int kStages = 3;
 constexpr int kStateThreads = (kWarps + 2) * 32;
 template <int KB, int KC>
@@ -909,6 +911,8 @@ struct StateSmem {
     static constexpr int USED = OFF_MISC + 16;
     static constexpr int BYTES = USED > 120 * 1024 ? USED : 120 * 1024;
 };
+// TMEM columns: U of even and of odd chunks, and from 128 on the planes of two buffers
+constexpr uint32_t kColEven = 0, kColOdd = 384;
 enum StateBar { kSbFull = 0, kSbFree = 3, kSbReady = 6, kSbDone = 8, kSbFixed = 10, kSbDrain = 11 };
 
 template <int KB, int KC>
@@ -998,8 +1002,8 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
                     tc_fence_after();
 #pragma unroll
                     for (int m = 0; m < 16; m++)               // the smallest plane first
-                        umma_ts(tmem, tmem + 128 + e * 128 + m * 8, bn_desc + (e * 4 + (m & 3)) * (2048 >> 4), id_upd,
-                                i > 0 || e > 0 || m > 0);
+                        umma_ts(tmem + (i & 1 ? kColOdd : kColEven), tmem + 128 + e * 128 + m * 8,
+                                bn_desc + (e * 4 + (m & 3)) * (2048 >> 4), id_upd, e > 0 || m > 0);
                     umma_commit(bars + kSbDone + e);
                 }
                 if (!fine) break;
@@ -1022,6 +1026,15 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
         };
         auto await = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
         bool fine = true;
+        constexpr int NS = KB / 2;
+        float s[NS] = {};
+        auto add = [&](int i) {               // U of chunk i
+            if (!s_on) return;
+            uint32_t v[NS];
+            tmem_ld<NS>(tm + (i & 1 ? kColOdd : kColEven) + half * NS, v);
+#pragma unroll
+            for (int u = 0; u < NS; u++) s[u] += __uint_as_float(v[u]);
+        };
         for (int i = 0; i < nchunk; i++) {
             const int c = cb + i, n = count(c);
             unsigned char* st = smem + (i % kStages) * L::STAGE;
@@ -1062,23 +1075,16 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
                 arrive(kSbReady + e);
             }
             if (!fine) break;
+            if (i > 0) add(i - 1);            // complete: the second buffer's last use has ended
         }
         if (fine && nchunk > 0) fine = await(kSbDone + 1, (nchunk - 1) & 1);
         tc_fence_after();
         if (fine && s_on) {
-            constexpr int NS = KB / 2;
-            float* e = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc;
-#pragma unroll 1
-            for (int i = half * NS; i < half * NS + NS; i += 8) {
-                uint32_t v[8] = {};
-                if (nchunk > 0) {
-                    tmem_ld8(tm + i, v);
-                    tmem_wait_ld();
-                }
+            if (nchunk > 0) add(nchunk - 1);
+            float* e = r.seg + (k.bh * p.nseg + k.seg) * r.db * r.dc + row;
 #pragma unroll
-                for (int u = 0; u < 8; u++)
-                    if (row < r.dc && i + u < r.db) e[(i + u) * r.dc + row] = __uint_as_float(v[u]);
-            }
+            for (int u = 0; u < NS; u++)
+                if (row < r.dc && half * NS + u < r.db) e[(half * NS + u) * r.dc] = s[u];
         }
     }
     tc_fence_before();
