@@ -32,8 +32,9 @@
 // With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
 // range, so its first row may have been begun by the CTA before it and its last may be finished
 // by the next.  It does the beginning of its last row first and publishes the state it reaches, and
-// the end of its first row last: by then the state it needs is there, since the two parts of a
-// row together are no longer than a CTA's range.
+// the end of its first row last: with rows of one length the state it needs is there by then, since the two
+// parts of a row together are no longer than a CTA's range.  With ragged lengths a row can be longer than several
+// ranges: its CTAs then run one after the other, each waiting for the one before.
 //
 // Measured: 4 x 2048 tokens of 40 heads of 128, forward, 83 us (4.2 TB/s of its 346 MB): 3.9 us a chunk, where
 // HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 2.5 us against 1.5.  What bounds
@@ -68,8 +69,11 @@ constexpr uint32_t kColO = 128;            // 128: A S, then P C
 constexpr uint32_t kColU = 256;            // 128: U
 constexpr uint32_t kColC = 384;            // 4 x 32: planes of C'^T for 64 tokens
 // Tries before a wait has run out: one that fails takes some 200 cycles among many waiters and 7800 alone
-// (measured), so 0.1 to 4 s, against the microseconds of the longest wait that ends
+// (measured), so 0.1 to 4 s, against the microseconds of the longest wait for a product or a copy.  Tries made
+// while the CTA waits for another one's state do not count: that wait has clocks of its own, 1 s and 20 us
+// for every chunk that the row has before (one takes 3 to 5)
 constexpr int kTries = 1 << 20;
+constexpr long long kStateClocks = 2000000000LL, kChunkClocks = 40000;
 constexpr float kZeroLog2 = -151.f;        // exp2 of anything below is zero in float32
 
 // A weight as a sum of three bfloat16 of 8 bits each.
@@ -147,23 +151,25 @@ enum Bar {
 
 struct Waiter {
     uint64_t* bars;
-    volatile int* abort;
+    volatile int* abort;         // and behind it: does the CTA wait for another one's state?
     int* err;
     // false once any wait of the CTA has run out
     __device__ __forceinline__ bool operator()(int bar, uint32_t parity) const {
         int tries = 0;
-        while (!mbar_try_wait(bars + bar, parity))
+        while (!mbar_try_wait(bars + bar, parity)) {
+            if (abort[1]) tries = 0;
             if (*abort || ++tries == kTries) {
                 *abort = 1;
                 *err = kDevErrTmaTimeout;
                 return false;
             }
+        }
         return true;
     }
     // has any wait run out, or this one, of a flag in global memory, begun at `start`?
-    __device__ __forceinline__ bool gone(long long start) const {
+    __device__ __forceinline__ bool gone(long long start, int chunks_before) const {
         if (*abort) return true;
-        if (clock64() - start <= 2000000000LL) return false;
+        if (clock64() - start <= kStateClocks + chunks_before * kChunkClocks) return false;
         *abort = 1;
         *err = kDevErrTmaTimeout;
         return true;
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
     Decays& dec = *reinterpret_cast<Decays*>(smem + L::OFF_W);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 8);
     Range* range_slot = reinterpret_cast<Range*>(smem + L::OFF_MISC + 16);
     const Waiter wait{bars, abort, p.err};
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
         }
         for (int i : {kScores, kAS, kPC, kCFree, kDrain}) mbar_init(bars + i, 1);
         for (int i : {kSReady, kCReady, kPReady, kFixed, kItem}) mbar_init(bars + i, kWarps);
-        *abort = 0;
+        abort[0] = abort[1] = 0;
         fence_mbar_init();
     }
     tc_fence_before();
@@ -580,10 +586,12 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 const int* flag = p.flags + blockIdx.x;
                 int there = 0;
                 const long long start = clock64();
+                if (tid == 0) abort[1] = 1;
                 while (true) {
                     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(flag) : "memory");
-                    if (there || wait.gone(start)) break;
+                    if (there || wait.gone(start, c0)) break;
                 }
+                if (tid == 0) abort[1] = 0;
                 if (!(fine = __all_sync(0xffffffffu, there != 0))) break;
             }
             float s[NS];
@@ -923,7 +931,7 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
     Decays& dec = *reinterpret_cast<Decays*>(smem + L::OFF_W);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC + 8);
     const Waiter wait{bars, abort, p.err};
 
     // the last segment in the order of walking feeds nobody: segments 0 .. nseg - 2, or 1 .. reversed
@@ -958,7 +966,7 @@ __global__ void __launch_bounds__(kStateThreads, 1) linattn_tc_state_kernel(cons
         }
         mbar_init(bars + kSbFixed, kWarps);
         mbar_init(bars + kSbDrain, 1);
-        *abort = 0;
+        abort[0] = abort[1] = 0;
         fence_mbar_init();
     }
     fill_decays(dec, g2, r.alpha, r.sigma, reverse, k.nchunk > 0 ? k.ntok - (k.nchunk - 1) * kT : 0);
