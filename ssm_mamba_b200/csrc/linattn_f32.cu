@@ -330,8 +330,9 @@ __global__ void __launch_bounds__(kThreads<DB>) linattn_f32_kernel(const __grid_
     if (STATE) return;
     // tokens past the row's length
     const int seg_end = (int)min((int64_t)p.seglen, (int64_t)p.seqlen - tok0);
-    for (int i = tid; i < (seg_end - ntok) * DC; i += NT) {
-        const int tk = ntok + i / DC, c = i % DC;
+    const int64_t total = (int64_t)(seg_end - ntok) * DC;
+    for (int64_t i = tid; i < total; i += NT) {
+        const int tk = ntok + (int)(i / DC), c = (int)(i % DC);
         if (c >= cols) continue;
         static_cast<float*>(r.out)[b * r.o_sb + (tok0 + tk) * r.o_st + h * r.o_sh + col0 + c] = 0.f;
     }

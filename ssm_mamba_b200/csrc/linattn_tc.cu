@@ -882,14 +882,20 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
                 // zeros for the tokens past the row's length, 16 bytes at a time where the rows allow it
                 const int es = r.out_f32 ? 4 : 2;
                 const int piece = r.out_vec && r.dc * es % 16 == 0 ? 16 : es, per = r.dc * es / piece;
-                const int total = (min(p.seglen, p.seqlen - k.tok0) - k.ntok) * per;
-                char* dst = static_cast<char*>(r.out) + (k.b * r.o_sb + (int64_t)(k.tok0 + k.ntok) * r.o_st + k.h * r.o_sh) * es;
+                const int end = min(p.seglen, p.seqlen - k.tok0);
+                // so many tokens at a time that their pieces count in 32 bits
+                constexpr int kFill = 1 << 20;
 #pragma unroll 1
-                for (int i = tid; i < total; i += kCompute) {
-                    char* at = dst + (int64_t)(i / per) * r.o_st * es + i % per * piece;
-                    if (piece == 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
-                    else if (piece == 4) *reinterpret_cast<float*>(at) = 0.f;
-                    else *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(0.f);
+                for (int t = k.ntok; t < end; t += kFill) {
+                    const int total = min(kFill, end - t) * per;
+                    char* dst = static_cast<char*>(r.out) + (k.b * r.o_sb + (int64_t)(k.tok0 + t) * r.o_st + k.h * r.o_sh) * es;
+#pragma unroll 1
+                    for (int i = tid; i < total; i += kCompute) {
+                        char* at = dst + (int64_t)(i / per) * r.o_st * es + i % per * piece;
+                        if (piece == 16) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+                        else if (piece == 4) *reinterpret_cast<float*>(at) = 0.f;
+                        else *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(0.f);
+                    }
                 }
             }
         }
