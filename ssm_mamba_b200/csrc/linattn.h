@@ -68,6 +68,7 @@ struct LaGroupParams {
     const float* src;
     void* out; int64_t o_sb, o_st, o_sh;
     int batch, seqlen, heads, d, share;
+    int tokens;          // of a CTA; set by the launch
 };
 
 // A bfloat16 tensor copied to rows of 8 ceil(d / 8) channels, contiguous

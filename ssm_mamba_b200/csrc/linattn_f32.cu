@@ -423,16 +423,15 @@ __global__ void __launch_bounds__(256) linattn_pack_kernel(const __grid_constant
     }
 }
 
-// A CTA does kGroupTokens tokens; V channels (V divides d) per thread and step.  Bound by HBM: 22560
+// A CTA does p.tokens tokens; V channels (V divides d) per thread and step.  Bound by HBM: 22560
 // tokens of 14 float32 heads of 100 into 7 of bfloat16 in 40 us (3.9 TB/s).
-constexpr int kGroupTokens = 16;
 template <typename T, int V>
 __global__ void __launch_bounds__(256) linattn_group_kernel(const __grid_constant__ LaGroupParams p) {
     const int groups = p.heads / p.share, dv = p.d / V, per = groups * dv;
-    const int64_t tokens = (int64_t)p.batch * p.seqlen, first = (int64_t)blockIdx.x * kGroupTokens;
+    const int64_t tokens = (int64_t)p.batch * p.seqlen, first = (int64_t)blockIdx.x * p.tokens;
     const int64_t b0 = first / p.seqlen;
     const int t0 = (int)(first - b0 * p.seqlen);
-    const int n = (int)(tokens - first < kGroupTokens ? tokens - first : kGroupTokens);
+    const int n = (int)(tokens - first < p.tokens ? tokens - first : p.tokens);
     for (int i = threadIdx.x; i < n * per; i += 256) {
         const int tl = i / per, pos = i - tl * per, g = pos / dv, c = (pos - g * dv) * V;
         const float* s = p.src + ((first + tl) * p.heads + (int64_t)g * p.share) * p.d + c;
@@ -458,9 +457,11 @@ __global__ void __launch_bounds__(256) linattn_group_kernel(const __grid_constan
 }
 
 template <typename T>
-cudaError_t launch_group(const LaGroupParams& p, cudaStream_t stream) {
+cudaError_t launch_group(LaGroupParams p, cudaStream_t stream) {
     const int64_t tokens = (int64_t)p.batch * p.seqlen;
-    const unsigned grid = (unsigned)((tokens + kGroupTokens - 1) / kGroupTokens);
+    // so many that a CTA's elements count in 32 bits (one token has at most 2^23 heads of 128)
+    p.tokens = (int64_t)p.heads / p.share * p.d < (1 << 26) ? 16 : 1;
+    const unsigned grid = (unsigned)((tokens + p.tokens - 1) / p.tokens);
     if (p.d % 4 == 0) linattn_group_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
     else linattn_group_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
     return cudaGetLastError();

@@ -1,7 +1,8 @@
-"""Rows so long that the elements of their padding pass 2^31: all of them are written as zeros.
+"""Rows so long that the elements of their padding pass 2^31, all of which are written as zeros, and heads so
+many that the elements of 16 tokens do.
 
 Through the C ABI, with tensors whose tokens share memory so that nothing large is allocated: tokens of the
-output have a stride of zero (all of them write the same zeros), those of the inputs one that overlaps."""
+outputs have a stride of zero (all of them write the same values), those of the inputs one that overlaps."""
 import math
 
 import pytest
@@ -35,3 +36,19 @@ def test_float32(cuda):
 
 def test_bfloat16(cuda):
     _run(cuda, torch.bfloat16, 1 << 24, _sms(cuda) + 1, 8, 128, 8)       # rows shared between CTAs, single elements
+
+
+def test_gradients_of_many_shared_heads(cuda):
+    """With a decay of zero and inputs of one every head's gradient of v is one, and the sum over two of
+    them two (17 GB of workspace for the heads' gradients)."""
+    from ssm_mamba_b200 import capi
+    H, V = 2 * 1_060_000, 127
+    one = torch.ones(V, device=cuda)
+    q, v, dout = (one.as_strided((1, 16, h, n), (0, 0, 0, 1)) for h, n in ((H, 1), (H // 2, V), (H, V)))
+    room = torch.full((V + 2,), math.nan, device=cuda)
+    dv = room[1:-1].as_strided((1, 16, H // 2, V), (0, 0, 0, 1))
+    dq, dk = (torch.empty(1, 16, H, 1, device=cuda) for _ in range(2))
+    decay = torch.full((H,), -math.inf, device=cuda)
+    capi.call_linear_attn(capi.fill_linear_attn(q, q, v, decay, 1.0, dout=dout, dq=dq, dk=dk, dv=dv), backward=True)
+    assert torch.isnan(room[0]) and torch.isnan(room[-1])
+    assert (room[1:-1] == 2).all() and (dq == V).all() and (dk == V).all()
