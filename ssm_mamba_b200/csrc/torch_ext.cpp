@@ -665,6 +665,9 @@ at::Tensor linear_attn_update(const at::Tensor& state, const at::Tensor& q, cons
     a.state_k_stride = state.stride(2);
     a.out = out.data_ptr(); a.out_batch_stride = out.stride(0); a.out_head_stride = out.stride(1);
     ok(ssm_linear_attn_update(&a, at::cuda::getCurrentCUDAStream().stream()));
+    // autograd has to see the write, or a backward that saved the state would read the new one (tensors made in
+    // inference mode have no version and cannot be saved)
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

@@ -1,0 +1,31 @@
+"""What autograd sees of the linear-attention operators beyond their gradients."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(cuda, seed=0, T=20):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    q, k, v = (torch.randn(2, T, 3, n, generator=g, device=cuda) for n in (16, 16, 24))
+    return q, k, v, torch.tensor([-0.1, -0.5, 0.0], device=cuda), torch.randn(2, 3, 16, 24, generator=g, device=cuda)
+
+
+def test_decode_step_counts_as_in_place_change(cuda):
+    from ssm_mamba_b200 import linear_attention_fn, linear_attention_update
+    q, k, v, g, state = _inputs(cuda)
+    before = state._version
+    linear_attention_update(state[1:], q[1:, 0], k[1:, 0], v[1:, 0], g)          # a view shares its base's version
+    assert state._version > before
+    x = q.clone().requires_grad_()
+    out = linear_attention_fn(x, k, v, g, initial_state=state)                   # saves the state
+    linear_attention_update(state, q[:, 0], k[:, 0], v[:, 0], g)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with torch.inference_mode():
+        fixed = state.clone()
+        linear_attention_update(fixed, q[:, 0], k[:, 0], v[:, 0], g)
+    linear_attention_update(fixed, q[:, 1], k[:, 1], v[:, 1], g)                 # has no version, and needs none
+    for t in range(2):
+        linear_attention_update(state, q[:, t], k[:, t], v[:, t], g)
+    assert torch.equal(state, fixed)
