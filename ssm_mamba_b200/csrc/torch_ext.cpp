@@ -761,19 +761,22 @@ at::Tensor contiguous_f32(const at::Tensor& t) {
 at::Tensor with_sizes(const at::Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
 at::Tensor unit_last_stride(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
-// Gradients that were asked for with a graph of their own: going through them is an error, not a zero.
-variable_list once_differentiable(const char* name, variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
+// Tensors through which a backward raises: going through them is an error, not a zero.
+variable_list no_way_back(std::string message, variable_list ts) {
     variable_list some;
-    for (at::Tensor& g : grads)
-        if (g.defined()) some.push_back(g.detach().requires_grad_(true));
-    auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative",
-                                                               (int64_t)some.size());
+    for (at::Tensor& t : ts)
+        if (t.defined()) some.push_back(t.detach().requires_grad_(true));
+    auto err = std::make_shared<torch::autograd::DelayedError>(std::move(message), (int64_t)some.size());
     some = (*err)(std::move(some));
     size_t i = 0;
-    for (at::Tensor& g : grads)
-        if (g.defined()) g = some[i++];
-    return grads;
+    for (at::Tensor& t : ts)
+        if (t.defined()) t = some[i++];
+    return ts;
+}
+// gradients that were asked for with a graph of their own
+variable_list once_differentiable(const char* name, variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    return no_way_back(std::string(name) + " has no second derivative", std::move(grads));
 }
 
 struct LinearAttention : torch::autograd::Function<LinearAttention> {
@@ -838,9 +841,16 @@ std::vector<at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& 
 at::Tensor linear_attention_update(const at::Tensor& state, const at::Tensor& q, const at::Tensor& k,
                                    const at::Tensor& v, const at::Tensor& log_decay, std::optional<double> scale) {
     check_la("linear_attention_update", q, k, v, log_decay);
-    return linear_attn_update(state, unit_last_stride(q), unit_last_stride(k), unit_last_stride(v),
-                              contiguous_f32(log_decay),
-                              scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1))));
+    const bool grad = at::GradMode::is_enabled();
+    TORCH_CHECK_VALUE(!(grad && state.requires_grad()),
+                      "linear_attention_update: state requires a gradient, and the update has none; pass state.detach() "
+                      "or call it under torch.no_grad()");
+    at::Tensor out = linear_attn_update(state, unit_last_stride(q), unit_last_stride(k), unit_last_stride(v),
+                                        contiguous_f32(log_decay),
+                                        scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(1, q.size(-1))));
+    if (grad && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+        return no_way_back("linear_attention_update is not differentiable", {out})[0];
+    return out;
 }
 
 // x as (rows, dim) with unit element stride: a view where its strides allow

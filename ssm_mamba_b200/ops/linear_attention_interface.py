@@ -44,8 +44,10 @@ def linear_attention_update(state: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     """One decode step; `state` (batch, heads, dk, dv) float32 is updated in place.
 
     q, k: (batch, heads, dk); v: (batch, heads, dv), fewer heads as in linear_attention_fn.
-    Returns out (batch, heads, dv) in q's dtype.  Not differentiable.  Autograd counts the update as any
-    in-place change: a backward that needs the state as it was before raises."""
+    Returns out (batch, heads, dv) in q's dtype.  Not differentiable: in grad mode a state that requires a
+    gradient is refused, and a backward through out raises where q, k or v require one; the new state
+    has no history.  Autograd counts the update as any in-place change: a backward that needs the
+    state as it was before raises."""
     return _C.linear_attention_update(state, q, k, v, log_decay, scale)
 
 

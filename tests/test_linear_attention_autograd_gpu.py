@@ -29,3 +29,30 @@ def test_decode_step_counts_as_in_place_change(cuda):
     for t in range(2):
         linear_attention_update(state, q[:, t], k[:, t], v[:, t], g)
     assert torch.equal(state, fixed)
+
+
+def test_decode_step_has_no_silent_gradient(cuda):
+    from ssm_mamba_b200 import linear_attention_fn, linear_attention_update
+    q, k, v, g, state = _inputs(cuda)
+    want = linear_attention_update(state.clone(), q[:, 0], k[:, 0], v[:, 0], g)
+    for i in range(3):
+        xs = [t[:, 0].clone() for t in (q, k, v)]
+        xs[i].requires_grad_()
+        new = state.clone()
+        out = linear_attention_update(new, *xs, g)
+        assert torch.equal(out, want) and not new.requires_grad
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not linear_attention_update(new, *xs, g).requires_grad
+    x = q.clone().requires_grad_()
+    _, last = linear_attention_fn(x, k, v, g, initial_state=state, return_last_state=True)
+    for s in (last, state.clone().requires_grad_()):
+        before = s.detach().clone()
+        with pytest.raises(ValueError, match="detach"):
+            linear_attention_update(s, q[:, 0], k[:, 0], v[:, 0], g)
+        assert torch.equal(s, before)                          # refused before it is written
+        out = linear_attention_update(s.detach(), q[:, 0], k[:, 0], v[:, 0], g)
+        with torch.no_grad():
+            linear_attention_update(s, q[:, 0], k[:, 0], v[:, 0], g)
+        assert not out.requires_grad and not torch.equal(s, before)
