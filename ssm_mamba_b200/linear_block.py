@@ -64,15 +64,20 @@ def linear_block_forward(w: LinearBlockWeights, hidden: torch.Tensor, lengths: O
                          cache: Optional[LinearBlockCache] = None) -> torch.Tensor:
     """hidden (batch, seqlen, model) -> (batch, seqlen, model), differentiable.  `lengths`
     (batch,): tokens of each row that count.  With `cache` the sequence continues from its state
-    and leaves the state after each row's last token in it."""
+    and leaves the state after each row's last token in it.  Gradients stop at the cache: the state it
+    brings is a constant, and the one it takes has no history."""
     x = layer_norm_fn(hidden, w.norm_weight, w.norm_bias)
     q, k, v = w.split(F.linear(x, w.qkv_weight))
     if cache is None:
         o = linear_attention_fn(q, k, v, w.log_decay, lengths=lengths)
     else:
-        o, last = linear_attention_fn(q, k, v, w.log_decay, initial_state=cache.state, lengths=lengths,
+        if torch.is_grad_enabled() and cache.state.requires_grad:
+            raise ValueError("linear_block_forward: gradients stop at the cache, whose state must not require one")
+        # a backward reads the state from before the cache takes the new one
+        state = cache.state.clone() if q.requires_grad else cache.state
+        o, last = linear_attention_fn(q, k, v, w.log_decay, initial_state=state, lengths=lengths,
                                       return_last_state=True)
-        cache.state.copy_(last)
+        cache.state.copy_(last.detach())
     return _finish(w, hidden, x, o)
 
 
