@@ -340,8 +340,8 @@ SSM_API int ssm_linear_attn_fwd(const ssm_linear_attn_args* args, void* workspac
 SSM_API int ssm_linear_attn_bwd(const ssm_linear_attn_args* args, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
-/* One decode step: state (batch, heads, dk, dv) float32 with unit dv stride becomes
- * w state + k v^T in place; out (batch, heads, dv) = scale * q^T state.  q, k (batch, heads, dk)
+/* One decode step: state (batch, heads, dk, dv) float32 with unit dv stride, no two elements of
+ * which share memory, becomes w state + k v^T in place; out (batch, heads, dv) = scale * q^T state.  q, k (batch, heads, dk)
  * and v (batch, heads, dv) as above without the token dimension.  Launched with programmatic
  * dependent launch: it waits for the previous kernel in the stream before reading any input. */
 typedef struct ssm_linear_attn_update_args {

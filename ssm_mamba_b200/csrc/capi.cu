@@ -13,6 +13,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "../../include/ssm_b200.h"
 #include "linattn.h"
@@ -1271,6 +1272,26 @@ int ssm_linear_attn_bwd(const ssm_linear_attn_args* a, void* workspace, size_t w
     return la_impl("ssm_linear_attn_bwd", a, 1, workspace, ws_bytes, stream);
 }
 
+// May two elements of a state (batch, heads, dk, dv) share memory?  Not if every dimension, by rising
+// stride, steps past all that those before it reach, as in any view of a tensor without repeated elements.
+static bool la_state_overlaps(const ssm_linear_attn_update_args* a) {
+    int64_t n[3] = {a->batch, a->heads, a->dk}, s[3] = {a->state_batch_stride, a->state_head_stride, a->state_k_stride};
+    for (int64_t& x : s) x = x < 0 ? -x : x;
+    for (int i = 0; i < 2; i++)
+        for (int j = 0; j < 2 - i; j++)
+            if (s[j] > s[j + 1]) {
+                std::swap(s[j], s[j + 1]);
+                std::swap(n[j], n[j + 1]);
+            }
+    int64_t reach = a->dv;
+    for (int i = 0; i < 3; i++) {
+        if (n[i] == 1) continue;
+        if (s[i] < reach) return true;
+        reach += (n[i] - 1) * s[i];
+    }
+    return false;
+}
+
 int ssm_linear_attn_update(const ssm_linear_attn_update_args* a, void* stream) {
     NvtxRange r_("ssm_linear_attn_update");
     const char* name = "ssm_linear_attn_update";
@@ -1286,6 +1307,8 @@ int ssm_linear_attn_update(const ssm_linear_attn_update_args* a, void* stream) {
     if (!valid_dtype(a->dtype)) return fail(SSM_ERR_INVALID, "%s: dtype must be SSM_F32 or SSM_BF16", name);
     if (!a->q || !a->k || !a->v || !a->log_decay || !a->state || !a->out)
         return fail(SSM_ERR_INVALID, "%s: q, k, v, log_decay, state and out are required", name);
+    if (la_state_overlaps(a))
+        return fail(SSM_ERR_INVALID, "%s: elements of state share memory; clone a broadcast state first", name);
     LaUpdParams p;
     memset(&p, 0, sizeof(p));
     p.batch = (int)a->batch; p.heads = (int)a->heads; p.dk = (int)a->dk; p.dv = (int)a->dv; p.scale = a->scale;

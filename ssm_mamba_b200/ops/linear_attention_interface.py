@@ -41,7 +41,8 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
 
 def linear_attention_update(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                             log_decay: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
-    """One decode step; `state` (batch, heads, dk, dv) float32 is updated in place.
+    """One decode step; `state` (batch, heads, dk, dv) float32 with unit dv stride is updated in place.
+    A state whose elements share memory (an expanded one) is refused.
 
     q, k: (batch, heads, dk); v: (batch, heads, dv), fewer heads as in linear_attention_fn.
     Returns out (batch, heads, dv) in q's dtype.  Not differentiable: in grad mode a state that requires a
