@@ -806,6 +806,12 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     }
 };
 
+// A forward-mode tangent would be dropped where no input requires a gradient: refused instead.
+void check_no_tangent(const char* name, std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative");
+}
+
 void check_la(const char* name, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
               const at::Tensor& log_decay) {
     TORCH_CHECK_TYPE(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16, name,
@@ -814,6 +820,7 @@ void check_la(const char* name, const at::Tensor& q, const at::Tensor& k, const 
                      ": q, k and v must share a dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
     TORCH_CHECK_VALUE(!log_decay.requires_grad(), name,
                       ": log_decay is a constant of the layer and has no gradient; pass log_decay.detach()");
+    check_no_tangent(name, {&q, &k, &v, &log_decay});
     TORCH_CHECK(q.dim() > 0 && k.dim() > 0 && v.dim() > 0, name, ": q, k and v must not be scalars");
 }
 
@@ -826,6 +833,7 @@ std::vector<at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& 
     if (initial_state) {
         TORCH_CHECK_TYPE(initial_state->scalar_type() == at::kFloat,
                          "linear_attention_fn: initial_state must be float32, got ", initial_state->scalar_type());
+        check_no_tangent("linear_attention_fn", {&*initial_state});
         s0 = initial_state->contiguous();
     }
     if (lengths) len = lengths->to(q.device(), at::kLong).contiguous();
@@ -841,6 +849,7 @@ std::vector<at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& 
 at::Tensor linear_attention_update(const at::Tensor& state, const at::Tensor& q, const at::Tensor& k,
                                    const at::Tensor& v, const at::Tensor& log_decay, std::optional<double> scale) {
     check_la("linear_attention_update", q, k, v, log_decay);
+    check_no_tangent("linear_attention_update", {&state});
     const bool grad = at::GradMode::is_enabled();
     TORCH_CHECK_VALUE(!(grad && state.requires_grad()),
                       "linear_attention_update: state requires a gradient, and the update has none; pass state.detach() "
@@ -887,6 +896,9 @@ at::Tensor layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& weig
     TORCH_CHECK_TYPE(x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16,
                      "layer_norm_fn: x must be float32 or bfloat16, got ", x.scalar_type());
     TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm_fn: x must have at least one dimension");
+    check_no_tangent("layer_norm_fn", {&x});
+    for (auto* t : {&weight, &bias})
+        if (*t) check_no_tangent("layer_norm_fn", {&**t});
     std::optional<at::Tensor> w, b;
     if (weight) w = contiguous_f32(*weight);
     if (bias) b = contiguous_f32(*bias);
