@@ -521,10 +521,12 @@ void check_blhd(const at::Tensor& t, const char* name, int64_t B, int64_t L, int
     TORCH_CHECK(t.stride(3) == 1 || d == 1, name, " must have unit channel stride");
 }
 
-void check_state(const std::optional<at::Tensor>& t, const char* name, int64_t B, int64_t H, int64_t K, int64_t V) {
+void check_state(const std::optional<at::Tensor>& t, const char* name, const at::Tensor& q, int64_t B, int64_t H,
+                 int64_t K, int64_t V) {
     if (!t) return;
     check_f32(*t, name, {B, H, K, V});
     TORCH_CHECK(t->is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(t->device() == q.device(), name, " must be on the device of q, ", q.device(), ", not on ", t->device());
 }
 
 ssm_linear_attn_args la_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -546,7 +548,7 @@ ssm_linear_attn_args la_args(const at::Tensor& q, const at::Tensor& k, const at:
     check_blhd(v, "v", B, L, H, V, q.scalar_type());
     for (auto* t : {&k, &v, &log_decay})
         TORCH_CHECK(t->device() == q.device(), "q, k, v and log_decay must be on one device");
-    check_state(initial_state, "initial_state", B, H, K, V);
+    check_state(initial_state, "initial_state", q, B, H, K, V);
     if (length)
         TORCH_CHECK(length->is_cuda() && length->scalar_type() == at::kLong && length->dim() == 1 &&
                         length->size(0) == B && length->is_contiguous(),
@@ -603,8 +605,9 @@ std::vector<at::Tensor> linear_attn_bwd(const at::Tensor& q, const at::Tensor& k
     ssm_linear_attn_args a = la_args(q, k, v, log_decay, scale, initial_state, length);
     c10::cuda::CUDAGuard guard(q.device());
     check_blhd(dout, "dout", a.batch, a.seqlen, a.heads, a.dv, q.scalar_type());
-    TORCH_CHECK(dout.size(2) == a.heads, "dout must have ", a.heads, " heads");
-    check_state(dlast_state, "dlast_state", a.batch, a.heads, a.dk, a.dv);
+    TORCH_CHECK(dout.size(2) == a.heads && dout.device() == q.device(), "dout must have ", a.heads,
+                " heads, on the device of q");
+    check_state(dlast_state, "dlast_state", q, a.batch, a.heads, a.dk, a.dv);
     at::Tensor dq = at::empty(q.sizes(), q.options());
     at::Tensor dk = at::empty(k.sizes(), k.options());
     at::Tensor dv = at::empty(v.sizes(), v.options());
@@ -724,6 +727,7 @@ std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& x, const std::optional<
     ssm_layer_norm_args a = ln_args(x, weight, std::nullopt, 0.0);
     c10::cuda::CUDAGuard guard(x.device());
     check_rows(dy, "dy", a.rows, a.dim, x.scalar_type());
+    TORCH_CHECK(dy.device() == x.device(), "dy must be on the device of x");
     check_f32(mean, "mean", {a.rows});
     check_f32(rstd, "rstd", {a.rows});
     const auto f32 = x.options().dtype(at::kFloat);
