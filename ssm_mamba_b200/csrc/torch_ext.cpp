@@ -822,7 +822,7 @@ void check_la(const char* name, const at::Tensor& q, const at::Tensor& k, const 
                      ": q must be float32 or bfloat16, got ", q.scalar_type());
     TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), name,
                      ": q, k and v must share a dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
-    TORCH_CHECK_VALUE(!log_decay.requires_grad(), name,
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && log_decay.requires_grad()), name,
                       ": log_decay is a constant of the layer and has no gradient; pass log_decay.detach()");
     check_no_tangent(name, {&q, &k, &v, &log_decay});
     TORCH_CHECK(q.dim() > 0 && k.dim() > 0 && v.dim() > 0, name, ": q, k and v must not be scalars");

@@ -12,7 +12,7 @@ q, k (batch, seqlen, heads, dk), v (batch, seqlen, heads, dv) in float32 or bflo
 batch, token and head strides (column blocks of one projection need no copy), dk and dv up to
 128; q, k and v may have fewer heads than log_decay, each count dividing it (head h reads head
 h // (heads / count)).  log_decay (heads,) float32 is a constant of the layer: it has no
-gradient, and -inf is a decay of zero.  States are (batch, heads, dk, dv) float32.
+gradient (in grad mode one that requires it is refused), and -inf is a decay of zero.  States are (batch, heads, dk, dv) float32.
 """
 from __future__ import annotations
 

@@ -56,3 +56,22 @@ def test_decode_step_has_no_silent_gradient(cuda):
         with torch.no_grad():
             linear_attention_update(s, q[:, 0], k[:, 0], v[:, 0], g)
         assert not out.requires_grad and not torch.equal(s, before)
+
+
+def test_log_decay_that_requires_a_gradient(cuda):
+    """Refused where a gradient could be asked for, and a constant where none is."""
+    from ssm_mamba_b200 import linear_attention_fn, linear_attention_update
+    q, k, v, g, state = _inputs(cuda)
+    want = linear_attention_fn(q, k, v, g, initial_state=state)
+    one = linear_attention_update(state.clone(), q[:, 0], k[:, 0], v[:, 0], g)
+    for p in (torch.nn.Parameter(g), torch.nn.Parameter(g.bfloat16().double())):
+        for call in (lambda: linear_attention_fn(q, k, v, p, initial_state=state),
+                     lambda: linear_attention_update(state.clone(), q[:, 0], k[:, 0], v[:, 0], p)):
+            with pytest.raises(ValueError, match="log_decay"):
+                call()
+            with torch.no_grad():
+                got = call()
+            with torch.inference_mode():
+                assert torch.equal(call(), got)
+            if p.dtype == torch.float32:
+                assert torch.equal(got, want if got.dim() == 4 else one)
