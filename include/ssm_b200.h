@@ -305,7 +305,9 @@ SSM_API int ssm_conv1d_update(const ssm_conv1d_args* args, void* stream);
  * `heads`; head h reads head h / (heads / count)).  dk and dv are 1 to 128.  States are
  * (batch, heads, dk, dv) float32 contiguous.  `length` (batch) int64, clamped to [0, seqlen]:
  * tokens from length[b] on take no part, out and the gradients are zero there, and last_state
- * is the state after length[b] tokens.  log_decay = -inf is a decay of zero. */
+ * is the state after length[b] tokens.  log_decay = -inf is a decay of zero.
+ * An infinity in q, k, v, dout or a state may come out as a NaN; one, or a NaN, in a token's k or v may also
+ * reach the outputs of up to 127 tokens before it (gradients: on either side). */
 typedef struct ssm_linear_attn_args {
     int64_t batch, seqlen, heads, dk, dv;
     int64_t q_heads, k_heads, v_heads;

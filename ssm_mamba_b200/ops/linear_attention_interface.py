@@ -33,8 +33,10 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
     With return_last_state also the float32 state after the last token of each row (after
     lengths[b] tokens), differentiable, from which linear_attention_update continues.
 
-    Tokens are worked on in chunks: a NaN or an infinity in a token's k or v may also reach the
-    outputs of up to 127 tokens before it."""
+    Infinities and NaN: an infinity in q, k, v or a state may come out as a NaN, since operands are split
+    into parts.  Tokens are worked on in chunks: a NaN or an infinity in a token's k or v may also
+    reach the outputs of up to 127 tokens before it, and in a backward the gradients of up to 127
+    tokens on either side.  Other heads and batch rows are not touched."""
     r = _C.linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_last_state)
     return (r[0], r[1]) if return_last_state else r[0]
 
