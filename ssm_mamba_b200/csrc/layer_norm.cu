@@ -442,6 +442,8 @@ cudaError_t launch_bwd(LnParams& p, cudaStream_t stream) {
     cudaError_t e = resident_ctas(layer_norm_bwd_kernel<T, VT, E, TPR>, TPR * RPC, bytes, known, &resident);
     if (e != cudaSuccess) return e;
     if (p.nparts > resident) p.nparts = resident;
+    // and no CTA without a row
+    if (p.nparts > (p.rows + RPC - 1) / RPC) p.nparts = (int)((p.rows + RPC - 1) / RPC);
     layer_norm_bwd_kernel<T, VT, E, TPR><<<p.nparts, TPR * RPC, bytes, stream>>>(p);
     return cudaGetLastError();
 }
@@ -512,9 +514,10 @@ cudaError_t dispatch_wide(const LnParams& p, int backward, cudaStream_t stream) 
 
 }  // namespace
 
-// Partial rows of dw and db there is room for: one per CTA of the backward, none without a row, at most
-// four CTAs per SM, or eight of those with 64 threads (32768 rows of 801 bfloat16: 80 and 53 us); for wide
-// rows 64 slices of the rows.
+// Partial rows of dw and db there is room for: one per CTA of the backward, at most four CTAs per SM, or eight
+// of those with 64 threads (32768 rows of 801 bfloat16: 80 and 53 us); for wide rows 64 slices of the rows.
+// Which kernel runs goes by the alignment too, so the launch may take fewer: bfloat16 vectors of 513 to
+// 768 have four rows to a CTA.
 int layer_norm_parts(int64_t rows, int dim, int sms) {
     if (dim > kLnMaxDim) return (int)(rows < 64 ? rows : 64);
     const int rpc = dim <= 512 ? 4 : 1;
