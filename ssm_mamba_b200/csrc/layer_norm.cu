@@ -6,15 +6,16 @@
 // second reading.  All sums are float32.
 //
 // Measured (32768 rows, forward and backward): 2564 float32 99 us (6.8 TB/s) and 170 (5.9); 2565 float32,
-// whose rows allow no vectors, 121 (5.6) and 187 (5.4); 2560 bfloat16 70 (4.8) and 116 (4.3), where
-// the conversions and sums of each element weigh twice as much against its bytes.
+// whose rows allow no vectors, 121 (5.6) and 187 (5.4); 2560 bfloat16 70 (4.8) and 116 (4.3): half of the
+// bytes in flight per row, and the warps wait for them (at 16384 x 768 the first stall, with issue at 38 to 46%).
 //
 // Backward: a thread owns the same columns of every row it meets, so the sums of dw and db
 // stay in its registers over all rows of a CTA; each CTA leaves one partial row, and a second
 // kernel adds the partial rows in a fixed order (deterministic, no floating-point atomics).
 //
 // Rows of more than 8192 elements do not fit the registers: they are read again for each pass
-// (from L2), and dw and db get a pass of their own.
+// (from L2), element by element, and dw and db get a pass of their own.  4096 rows of 16384: bfloat16 97 us
+// forward (2.8 TB/s) and 238 backward (1.7), float32 117 (4.6) and 328 (2.5).
 #include <atomic>
 
 #include "common.cuh"

@@ -11,12 +11,13 @@
 // x = hi + lo with hi rounded to tf32 (11 bits), and hi hi' + lo hi' + hi lo' misses x x' by about
 // 2^-22.  On B200 that has 92 TFLOP/s of float32 products against 74 on the FMA pipe, and a sixth of its
 // shared-memory traffic, which bounded a version on packed FMAs (67% of the wavefronts, 35% of
-// the FMAs); tcgen05 takes tf32 operands from shared memory along K only and would need the split
-// tiles stored, more than a CTA has at 128 channels.  An infinity becomes a NaN when it is split.
+// the FMAs).  On tcgen05 both halves of a, b, c and S would have to be stored in shared memory: 224 KB at 128
+// channels and 64 columns (a and b 64 KB each, c 32, S 64) of the 227 that a CTA has, without room for the next
+// chunk; at 64 channels 128 KB would do, which is not built.  An infinity becomes a NaN when it is split.
 //
 // Measured: 2 x 1024 tokens of 24 heads of 64, forward and backward, 193 us (325 us on FMAs); 11 x 94
 // tokens of 40 heads, 96 and 80 channels, forward, 113 us.  What bounds it is the latency of a
-// chunk's steps at 16 warps an SM: the tensor pipe is busy 30 to 40% of the time, issue 40 to 50%
+// chunk's steps with 8 to 14 warps on an SM: the tensor pipe is busy 20 to 40% of the time, issue 34 to 49%
 // (two tiles' products interleaved by hand: 191 us and 115 us).
 //
 // Shared-memory rows are strided so that a fragment's 32 elements lie on different banks: 4 (mod

@@ -27,7 +27,7 @@
 // chunk's first 64 tokens and lanes 64-127 the last 64, all warps at once, and the state is kept in two
 // parts, each decayed alike and with the U of its half; A S sums over both, and they are joined
 // where the state leaves the CTA.  Their smaller tiles have four stages.  1280 tokens of 148 heads:
-// 35.0 us without parts and with two stages, 33.0 so.
+// 35.0 us without parts and with two stages, 33.0 so (before the lower halves; 44 with them).
 //
 // With more rows than SMs the CTAs share the chunks of all rows evenly: each takes a contiguous
 // range, so its first row may have been begun by the CTA before it and its last may be finished
@@ -36,12 +36,14 @@
 // parts of a row together are no longer than a CTA's range.  With ragged lengths a row can be longer than several
 // ranges: its CTAs then run one after the other, each waiting for the one before.
 //
-// Measured: 4 x 2048 tokens of 40 heads of 128, forward, 83 us (4.2 TB/s of its 346 MB): 3.9 us a chunk, where
-// HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 2.5 us against 1.5.  What bounds
-// it is the chain of a chunk: six times the compute warps wait for a product and hand one on, 150 to 250
-// cycles each, between 600 and 1200 cycles of conversions.  Groups of warps with one step each took
-// twice as long (their code together misses the instruction cache), 16 compute warps 4.5 us a chunk
-// (104 registers: spills), three planes of C' 3.7 us, but 1.6e-6 of error in the state.
+// Measured: 4 x 2048 tokens of 40 heads of 128, forward, 100 us (3.5 TB/s of its 346 MB): 4.8 us a chunk, where
+// HBM would allow 3.0 (four tiles of 32 KB on 148 SMs); heads of 64 3.2 us against 1.5.  What bounds
+// it is the chain of a chunk: six times (seven at 128 x 128) the compute warps wait for a product and hand one
+// on, 150 to 250 cycles each, between 500 and 1800 cycles of conversions.  Without the lower halves
+// of P and S a chunk took 3.9 and 2.5 us (their products, conversions and code; see above for what they are for).
+// Measured against those: groups of warps with one step each took twice as long (their code together misses the
+// instruction cache), 16 compute warps 4.5 us a chunk (104 registers: spills), three planes of C' 3.7 us, but
+// 1.6e-6 of error in the state.
 //
 // Every wait is bounded: the first that runs out sets the device error word and a flag that
 // ends all others.
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1) linattn_tc_kernel(const __grid_co
 // in one of two places by turns, and is added to the sum in registers, rounded, while the next one is formed
 // (summed in the unit over 128 chunks of k and v with means of one, the state was 4.9e-5 off).  C'^T has two
 // buffers of 64 tokens; the threads fill one while the product reads the other, and bound it (42 rows of 8
-// segments of 20 chunks, 128 channels: 83 us, 65 at HBM's rate).
+// segments of 20 chunks, 128 channels: 95 us, 65 at HBM's rate).
 constexpr int kStages = 3;
 constexpr int kStateThreads = (kWarps + 2) * 32;
 template <int KB, int KC>
